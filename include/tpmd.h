@@ -30,6 +30,7 @@ extern "C" {
 /* storage/compute type of weights, feats and activations */
 #define TPMD_DTYPE_F32 0 /* fp32 storage, fp32 FFMA convs (parity mode)     */
 #define TPMD_DTYPE_F16 1 /* f16 storage, tcgen05 f16 convs, f32 accumulate   */
+#define TPMD_DTYPE_F8  2 /* e4m3 with f32 block scales: tpk_quant_f8 / tpk_gemm_f8 */
 
 #define TPMD_N_LEVELS 7
 #define TPMD_STYLE_DIM 512
@@ -323,6 +324,71 @@ int tpk_chw_to_rgb24(const float *chw, int64_t n, int H, int W, uint8_t *rgb, vo
 int tpk_gemm(const void *X, int64_t ldx, const void *W, int64_t ldw, float *Y, int64_t ldy, int M, int N, int K,
              int batch, int x_row_b, int x_col_b, int w_row_b, int w_col_b, int64_t y_batch, int dtype,
              const float *bias, float scale, int act, void *stream);
+
+/* The next entry points only enqueue on `stream` (no allocation, no host
+ * synchronisation: they can be captured into a CUDA graph). They run on the
+ * device that holds their pointers, whichever device is current; all
+ * pointers are memory of that one device, and `stream` is one of its
+ * streams (NULL: its legacy default stream). Rows and sequences of size 0
+ * are allowed and write nothing. Outputs may not overlap inputs. Whether
+ * every pipeline wait of the tensor-core kernels completed is known once
+ * tpk_device_status returns 0. */
+
+/* Quantise x [M][K] (TPMD_DTYPE_F32 or F16, row stride ldx elements) to
+ * 8-bit floating point with one scale per block of rows x 128 elements,
+ * rows = 1 (activations) or 128 (weights):
+ *   s[m / rows][k / 128] = max(max |x| over the block / 448, 2^-126)
+ *   q[m][k] = x[m][k] / s rounded to the nearest e4m3 value (ties to even),
+ * every step in IEEE float32. Blocks at the ends hold what is left; a block
+ * of zeros has the smallest scale. A NaN element quantises to NaN and does
+ * not count in its block's maximum; an infinite one makes the scale infinite
+ * (the other elements 0, itself NaN). q: one byte an element, row stride ldq
+ * bytes; s: f32, row stride lds elements. Any strides and alignments; the
+ * bytes between rows are not written. */
+int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq,
+                 float *s, int64_t lds, void *stream);
+
+/* Product of two matrices that tpk_quant_f8 quantised, X by rows = 1 and W
+ * by rows = 128, on the tcgen05 tensor cores:
+ *   Y[m][n] = act(sum_b sx[m][b] sw[n/128][b] (sum_{k in block b} X[m][k] W[n][k]) + bias[n])
+ * m < M, n < N, k < K, blocks of 128 along k; the sums are f32 and each
+ * block's sum is scaled and added in f32. Scales may be any float32 values. act as in
+ * tpk_gemm (0 to 3); bias may be NULL. y_dtype: TPMD_DTYPE_F32, F16, or F8:
+ * Y is then quantised as by tpk_quant_f8 with rows = 1, its scales in sy
+ * [M][ceil(N/128)] (row stride ldsy), which is NULL otherwise. X and W: 16-byte
+ * aligned with row strides of multiples of 16 bytes; everything else any
+ * stride and alignment. What lies between rows is neither read nor written. */
+int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t ldsx, const void *W, int64_t ldw,
+                const float *sw, int64_t ldsw, void *Y, int64_t ldy, int y_dtype, float *sy, int64_t ldsy, int M,
+                int N, int K, const float *bias, int act, void *stream);
+
+/* Attention over a sliding window, with first tokens that stay visible
+ * (sinks), for prompts, padded batches and single new tokens over a cache.
+ * Sequence b has L = kv_len[b] keys (Tk when kv_len is NULL) and n =
+ * q_len[b] query rows (Tq when NULL), the last n positions of its L: row i
+ * stands at p = L - n + i. It sees key j < L where
+ *   (right < 0 or j <= p + right) and (left < 0 or j >= p - left or j < sinks),
+ * and out = softmax over the visible keys of scale q.k, times v; a row that
+ * sees none gets zeros. Query head h reads key head h / (Hq / Hkv). Softmax
+ * and sums in f32. Rows i >= n of `out` are left as they were; keys j >= L,
+ * and keys that no row of the sequence sees, may hold anything (stale cache
+ * memory, NaN). Lengths outside [0, Tq] and [0, Tk] are clamped to them; a
+ * length q_len > kv_len puts the first rows before position 0.
+ *
+ * dtype: of q, k, v and out, TPMD_DTYPE_F32 or F16. strides, in elements:
+ * {batch, token, head} of q, k, v and out in this order, so packed rows
+ * (q | k | v) and either order of tokens and heads are read in place;
+ * the D elements of a head are contiguous. D <= 256; q_len and kv_len are
+ * device memory (int32). */
+int tpk_attn_window(const void *q, const void *k, const void *v, void *out, const int64_t strides[12], int dtype,
+                    int B, int Tq, int Tk, int Hq, int Hkv, int D, const int32_t *q_len, const int32_t *kv_len,
+                    int left, int right, int sinks, float scale, void *stream);
+
+/* Synchronises `stream` (a stream of the current device), then reads and
+ * clears the device's expired-wait word of tpk_gemm_f8 and tpk_attn_window.
+ * 0 when no wait expired since the last query, else -1 with the message in
+ * tpk_last_error ("... timed out (results invalid)"). */
+int tpk_device_status(void *stream);
 
 /* Message of the last failed tpk_* call on this thread. */
 const char *tpk_last_error(void);

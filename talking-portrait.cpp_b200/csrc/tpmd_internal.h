@@ -164,6 +164,39 @@ cudaError_t launch_chw_to_rgb24(const float *chw, int64_t n, int64_t hw, uint8_t
 // the last-error slot of the tpk_* entry points (sets it, returns -1)
 int tpk_fail(const std::string &msg);
 
+// The device that holds every non-null pointer of `ptrs`, made current until
+// the end of the scope. ok() is false (the reason in why) when a pointer is
+// no device memory or they lie on several devices.
+struct tpk_device_scope {
+    tpk_device_scope(const void *const *ptrs, int n);
+    ~tpk_device_scope();
+    tpk_device_scope(const tpk_device_scope &) = delete;
+    tpk_device_scope &operator=(const tpk_device_scope &) = delete;
+    bool ok() const { return !why; }
+    const char *why = nullptr;
+    int device = -1;
+
+  private:
+    int prev_ = -1;
+};
+// the current device's expired-wait word that tpk_device_status reads
+// (nullptr and a CUDA error pending when it cannot be had)
+int *tpk_err_word();
+
+// Sliding-window attention (tpk_attn_window): lens clamped, left and right
+// within [0, 2^30]; strides {batch, token, head} in elements
+struct attn_desc {
+    const void *q, *k, *v;
+    void *out;
+    int64_t qs[3], ks[3], vs[3], os[3];
+    bool f16;
+    int B, Tq, Tk, Hq, Hkv, D;
+    const int32_t *q_len, *kv_len;
+    int left, right, sinks;
+    float scale;
+};
+cudaError_t launch_attn_simt(const attn_desc &d, cudaStream_t st);
+
 // The tcgen05 GEMM of the sampler and the audio encoder (kernels_gemm_tc.cu):
 //   Y[m][n] = act((sum_k X[m][k] W[n][k] + bias[n]) * scale) (+ res[m][n]), m < M, n < N
 // X and W K-major with row strides ldx, ldw (elements, 16-byte multiples);

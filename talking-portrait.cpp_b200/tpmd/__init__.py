@@ -24,6 +24,7 @@ LIB_PATH = os.path.join(os.path.dirname(HERE), "libtpmd.so")
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_F8 = 2
 N_LEVELS = 7
 STYLE_DIM = 512
 IMG = 512
@@ -51,7 +52,8 @@ EXPORTS = ("tpmd_abi_version", "tpmd_create", "tpmd_create_error", "tpmd_destroy
            "tpmd_group_member", "tpmd_group_set_tensor", "tpmd_group_load_gguf", "tpmd_group_prepare",
            "tpmd_group_set_feats", "tpmd_group_set_feats_device", "tpmd_shard_range", "tpmd_group_decode",
            "tpmd_group_max", "tpmd_group_selftest_nccl", "tpmd_decode_rgb24", "tpmd_group_decode_rgb24",
-           "tpk_chw_to_rgb24", "tpk_gemm", "tpmd_decode_schedule")
+           "tpk_chw_to_rgb24", "tpk_gemm", "tpmd_decode_schedule",
+           "tpk_quant_f8", "tpk_gemm_f8", "tpk_attn_window", "tpk_device_status")
 
 _lib = None
 
@@ -121,6 +123,11 @@ def load_library(path: str = LIB_PATH):
     L.tpk_chw_to_rgb24.argtypes = [v, i64, C.c_int, C.c_int, v, v]
     L.tpk_gemm.argtypes = [v, i64, v, i64, v, i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                            C.c_int, C.c_int, i64, C.c_int, v, C.c_float, C.c_int, v]
+    L.tpk_quant_f8.argtypes = [v, C.c_int, i64, i64, i64, C.c_int, v, i64, v, i64, v]
+    L.tpk_gemm_f8.argtypes = [v, i64, v, i64, v, i64, v, i64, v, i64, C.c_int, v, i64, C.c_int, C.c_int, C.c_int, v,
+                              C.c_int, v]
+    L.tpk_attn_window.argtypes = [v, v, v, v, C.POINTER(i64)] + [C.c_int] * 7 + [v, v] + [C.c_int] * 3 + [C.c_float, v]
+    L.tpk_device_status.argtypes = [v]
     L.tpmd_group_selftest_nccl.argtypes = [C.c_int, C.c_int, C.c_double, C.POINTER(C.c_int), C.c_char_p,
                                            C.c_size_t]
     L.tpmd_debug_expire_wait.argtypes = [v, C.c_longlong]
@@ -441,6 +448,96 @@ def gemm(X, W, Y, M, N, K, ldx=None, ldw=None, ldy=None, batch=1, x_row_b=0, x_c
         C.c_void_p(Y.data_ptr()), ldy or Y.shape[-1], M, N, K, batch, x_row_b, x_col_b, w_row_b, w_col_b, y_batch,
         dt, C.c_void_p(bias.data_ptr() if bias is not None else None), scale, act, C.c_void_p(stream)))
     return Y
+
+
+def _rows2(t, what):
+    """(data pointer, row stride) of a matrix whose rows are contiguous"""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise TpmdError(f"{what}: a matrix with contiguous rows is needed")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+
+
+def _expect(ok, what):
+    if not ok:
+        raise TpmdError(what)
+
+
+def quant_f8(x, q, s, rows=1, stream=0):
+    """Quantise x [M, K] (torch CUDA, f32 or f16) to 8-bit floating point
+    with a scale per block of rows x 128 elements (see tpk_quant_f8 in
+    include/tpmd.h): q [M, K] torch.float8_e4m3fn, s [ceil(M / rows),
+    ceil(K / 128)] f32. rows = 1 for activations, 128 for weights."""
+    import torch
+    _expect(rows in (1, 128), "quant_f8: rows must be 1 or 128")
+    _expect(x.dtype in (torch.float16, torch.float32), "quant_f8: x must be float16 or float32")
+    _expect(q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32, "quant_f8: q must be float8_e4m3fn, s float32")
+    _expect(x.dim() == 2 and q.shape == x.shape and tuple(s.shape) == (-(-x.shape[0] // rows), -(-x.shape[1] // 128)),
+            "quant_f8: q must have x's shape, s one element per block")
+    (xp, ldx), (qp, ldq), (sp, lds) = _rows2(x, "quant_f8 x"), _rows2(q, "quant_f8 q"), _rows2(s, "quant_f8 s")
+    _tpk_check(load_library().tpk_quant_f8(xp, int(x.dtype == torch.float16), ldx, x.shape[0], x.shape[1], rows, qp,
+                                           ldq, sp, lds, stream))
+    return q, s
+
+
+def gemm_f8(X, sx, W, sw, Y, sy=None, bias=None, act=0, stream=0):
+    """Y = act(X . W^T + bias) of matrices quantised by quant_f8, X [M, K]
+    with sx (rows = 1), W [N, K] with sw (rows = 128) (see tpk_gemm_f8 in
+    include/tpmd.h). Y [M, N] float32, float16, or float8_e4m3fn with its
+    scales in sy [M, ceil(N / 128)]."""
+    import torch
+    f8 = torch.float8_e4m3fn
+    _expect(X.dtype == f8 and W.dtype == f8 and sx.dtype == torch.float32 and sw.dtype == torch.float32,
+            "gemm_f8: X and W must be float8_e4m3fn, their scales float32")
+    _expect(Y.dtype in (torch.float32, torch.float16, f8), "gemm_f8: Y must be float32, float16 or float8_e4m3fn")
+    _expect((sy is not None) == (Y.dtype == f8), "gemm_f8: sy goes with a float8_e4m3fn Y, and only with it")
+    _expect(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1], "gemm_f8: X [M, K] and W [N, K] must share K")
+    (M, K), N = X.shape, W.shape[0]
+    kb, nb = -(-K // 128), -(-N // 128)
+    _expect(tuple(Y.shape) == (M, N) and tuple(sx.shape) == (M, kb) and tuple(sw.shape) == (nb, kb),
+            "gemm_f8: Y must be [M, N], sx [M, ceil(K / 128)], sw [ceil(N / 128), ceil(K / 128)]")
+    _expect(sy is None or (sy.dtype == torch.float32 and tuple(sy.shape) == (M, nb)),
+            "gemm_f8: sy must be float32 [M, ceil(N / 128)]")
+    _expect(bias is None or (bias.dtype == torch.float32 and tuple(bias.shape) == (N,) and bias.is_contiguous()),
+            "gemm_f8: bias must be contiguous float32 [N]")
+    (xp, ldx), (sxp, ldsx), (wp, ldw) = _rows2(X, "gemm_f8 X"), _rows2(sx, "gemm_f8 sx"), _rows2(W, "gemm_f8 W")
+    (swp, ldsw), (yp, ldy) = _rows2(sw, "gemm_f8 sw"), _rows2(Y, "gemm_f8 Y")
+    syp, ldsy = _rows2(sy, "gemm_f8 sy") if sy is not None else (None, 0)
+    yd = DTYPE_F8 if sy is not None else DTYPE_F16 if Y.dtype == torch.float16 else DTYPE_F32
+    _tpk_check(load_library().tpk_gemm_f8(xp, ldx, sxp, ldsx, wp, ldw, swp, ldsw, yp, ldy, yd, syp, ldsy, M, N, K,
+                                          bias.data_ptr() if bias is not None else None, act, stream))
+    return Y
+
+
+def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv_len=None, stream=0):
+    """Attention over a sliding window with first tokens that stay visible
+    (see tpk_attn_window in include/tpmd.h): q and out [B, Tq, Hq, D], k and
+    v [B, Tk, Hkv, D] torch CUDA f32 or f16, any strides with a contiguous
+    last dimension; q_len, kv_len int32 [B] or None; left, right < 0: no
+    limit on that side; scale None: 1 / sqrt(D)."""
+    import torch
+    _expect(q.dtype in (torch.float16, torch.float32) and k.dtype == q.dtype and v.dtype == q.dtype and
+            out.dtype == q.dtype, "attn_window: q, k, v and out must share float16 or float32")
+    _expect(q.dim() == 4 and k.dim() == 4 and out.shape == q.shape and v.shape == k.shape and
+            k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3],
+            "attn_window: q and out [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")
+    (B, Tq, Hq, D), (_, Tk, Hkv, _) = q.shape, k.shape
+    for t in (q, k, v, out):
+        _expect(D == 1 or t.stride(3) == 1, "attn_window: the last dimension must be contiguous")
+    for t in (q_len, kv_len):
+        _expect(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous()),
+                "attn_window: q_len and kv_len must be contiguous int32 [B]")
+    st = (C.c_int64 * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+    _tpk_check(load_library().tpk_attn_window(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, int(q.dtype == torch.float16), B, Tq, Tk, Hq,
+        Hkv, D, q_len.data_ptr() if q_len is not None else None, kv_len.data_ptr() if kv_len is not None else None,
+        left, right, sinks, D ** -0.5 if scale is None else scale, stream))
+    return out
+
+
+def tpk_status(stream=0):
+    """Synchronise `stream` and raise if a pipeline wait of gemm_f8 or
+    attn_window expired on the current device (tpk_device_status)."""
+    _tpk_check(load_library().tpk_device_status(stream))
 
 
 def im2col_cf(src, IC, IW, IH, N, out, KW=3, KH=3, s0=1, s1=1, p0=1, p1=1, d0=1, d1=1,
