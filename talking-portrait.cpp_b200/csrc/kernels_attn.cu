@@ -16,71 +16,21 @@
 #include <string>
 
 #include "../../include/tpmd.h"
+#include "attn_row.cuh"
 #include "tpmd_internal.h"
 
 namespace tpmd {
 namespace {
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-
 template <typename T, int EPL>
-__global__ void __launch_bounds__(128) attn_row_kernel(const attn_desc p, int64_t rows) {
+__global__ void __launch_bounds__(128) attn_row_kernel(const __grid_constant__ attn_desc p, int64_t rows) {
     const int lane = threadIdx.x & 31;
     const int64_t g = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (g >= rows) return;
     const int i = (int) (g % p.Tq), h = (int) (g / p.Tq % p.Hq), b = (int) (g / p.Tq / p.Hq);
     const int n = p.q_len ? min(max(p.q_len[b], 0), p.Tq) : p.Tq;
     const int L = p.kv_len ? min(max(p.kv_len[b], 0), p.Tk) : p.Tk;
-    if (i >= n) return;
-    const int64_t pos = (int64_t) L - n + i;
-    const int hi = (int) max((int64_t) 0, p.right < 0 ? (int64_t) L : min((int64_t) L, pos + p.right + 1));
-    const int lo = p.left < 0 ? 0 : (int) min((int64_t) hi, max((int64_t) 0, pos - p.left));
-    const int first = min(p.sinks, lo);
-    const int hk = h / (p.Hq / p.Hkv);
-    const T *q = (const T *) p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
-    const T *kb = (const T *) p.k + b * p.ks[0] + hk * p.ks[2];
-    const T *vb = (const T *) p.v + b * p.vs[0] + hk * p.vs[2];
-    float qv[EPL], o[EPL];
-#pragma unroll
-    for (int e = 0; e < EPL; e++) {
-        const int d = lane + 32 * e;
-        qv[e] = d < p.D ? to_f(q[d]) * p.scale : 0.0f;
-        o[e] = 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int t = 0; t < first + hi - lo; t++) {
-        const int64_t j = t < first ? t : t - first + lo;
-        const T *k = kb + j * p.ks[1], *v = vb + j * p.vs[1];
-        float s = 0.0f, vv[EPL];
-#pragma unroll
-        for (int e = 0; e < EPL; e++) {
-            const int d = lane + 32 * e;
-            s = fmaf(qv[e], d < p.D ? to_f(k[d]) : 0.0f, s);
-            vv[e] = d < p.D ? to_f(v[d]) : 0.0f;
-        }
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn;
-        const float c = expf(m - base), w = expf(s - base);
-        m = mn;
-        l = l * c + w;
-#pragma unroll
-        for (int e = 0; e < EPL; e++) o[e] = fmaf(w, vv[e], o[e] * c);
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // NaN stays NaN
-    T *out = (T *) p.out + b * p.os[0] + i * p.os[1] + h * p.os[2];
-#pragma unroll
-    for (int e = 0; e < EPL; e++) {
-        const int d = lane + 32 * e;
-        if (d < p.D) out[d] = from_f<T>(l == 0.0f ? 0.0f : o[e] * inv);
-    }
+    if (i < n) attn_row<T, EPL>(p, b, h, i, n, L, lane);
 }
 
 template <typename T>
@@ -161,8 +111,8 @@ extern "C" int tpk_attn_window(const void *q, const void *k, const void *v, void
     const void *ptrs[] = {q, out, q_len, kv_len, Tk > 0 ? k : nullptr, Tk > 0 ? v : nullptr};
     tpk_device_scope dev(ptrs, 6);
     if (!dev.ok()) return fail(dev.why);
-    const cudaError_t e = launch_attn_simt(d, (cudaStream_t) stream);
-    if (e == cudaErrorInvalidValue) return fail("too many rows");
+    const cudaError_t e = attn_tc_supported(d) ? launch_attn_tc(d, (cudaStream_t) stream) : launch_attn_simt(d, (cudaStream_t) stream);
+    if (e == cudaErrorInvalidValue) return fail("too many rows, or the launch was refused");
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;
 }

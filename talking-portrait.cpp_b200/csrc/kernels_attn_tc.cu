@@ -1,0 +1,740 @@
+// Sliding-window attention with first tokens that stay visible
+// (tpk_attn_window, include/tpmd.h) on the tcgen05 tensor cores, for f16:
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i.k_j - m_i),
+//   over keys j < min(L, p + right + 1) with j >= p - left or j < sinks
+//
+// in one pass over the keys with a running maximum m and sum. Rows of the
+// MMA are (token, query head of the group) pairs, so the query heads that
+// share a key head read its keys once and a tile spans few positions. Keys
+// come in tiles of 128: those of the window from its first key on (TMA boxes
+// start at any row), then those of the sinks; the last tile of each is cut to
+// a multiple of 16 keys.
+//
+// Per tile S = Q K^T (f32, TMEM), a thread per row turns S into weights P
+// (f16, over S in TMEM), O += P V (f32, TMEM). The maximum that P is relative
+// to moves only when a row's maximum has grown by 2^8: until then P stays
+// below 2^8, far inside f16, and O needs no rescaling.
+//
+// Two softmax warpgroups work in turn with the MMA warp:
+//  * prompts: each has its own 128 rows, both go through the same key tiles;
+//  * few rows (SPLIT): both have the same rows and take alternate key tiles;
+//    rows that fill no more than half or a quarter of the MMA's lanes are
+//    loaded two or four times, and each copy's warps take that share of
+//    every tile's keys; and the tiles are shared out over a cluster of up to
+//    eight CTAs. Their parts (m, sum, O) join in shared memory, then over the
+//    cluster (distributed shared memory), always in the same order.
+//
+// A weight of zero times a value that is not finite is NaN: the values of
+// keys that no row of the CTA sees are cleared in shared memory, and a row
+// that still comes out not finite is computed again on the CUDA cores from
+// its visible keys alone.
+//
+// Every pipeline wait is bounded; an expired wait sets *err and the CTA
+// skips the rest of its work.
+#include <cuda_fp16.h>
+
+#include "attn_row.cuh"
+#include "tc_ptx.cuh"
+#include "tpmd_internal.h"
+
+#include <algorithm>
+#include <mutex>
+
+namespace tpmd {
+namespace {
+
+template <int DB, bool SPLIT>
+struct at_cfg {
+    static constexpr int TILE_BYTES = 128 * 128 * DB;    // 128 rows of DB 64-column boxes
+    static constexpr int NQ = SPLIT ? 1 : 2;
+    static constexpr int STAGES = DB == 2 ? (SPLIT ? 6 : 5) : 8;
+    static constexpr int THREADS = 320;                  // 8 softmax warps, TMA, MMA
+    static constexpr int OLD = DB * 64 + 4;              // floats a row of the joined parts (bank shift)
+    static constexpr int NBARS = 2 * STAGES + 2 + 2 + 2 + 4;
+    static constexpr int DATA = (NQ + STAGES) * TILE_BYTES;
+    static constexpr int SMEM = 1024 + DATA + NBARS * 8 + 16;
+    static_assert(SMEM <= 232448, "shared memory");
+    static_assert(!SPLIT || 256 * OLD * 4 <= STAGES * TILE_BYTES, "parts fit the stages");
+};
+constexpr uint32_t TMEM_COLS = 512;
+
+struct at_params {
+    attn_desc d;
+    int g, tb, reps, qtiles, splits;
+    float c;  // scale log2(e)
+    bool o_vec;
+    int *err;
+};
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+        "l"((uint64_t) tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
+}
+// A in TMEM
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    const uint32_t mask = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(mask));
+}
+// 128-byte swizzled rows along N (the MMA's K runs over rows): lbo = bytes
+// between 64-column boxes, sbo = bytes between groups of 8 rows
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    uint64_t d = (uint64_t) ((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t) ((lbo >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t) ((sbo >> 4) & 0x3FFFu) << 32;
+    d |= (uint64_t) 1u << 46;
+    d |= (uint64_t) 2u << 61;
+    return d;
+}
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float *f) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) f[i] = __uint_as_float(r[i]);
+}
+// a bounded wait of a whole warp, one answer for all lanes
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
+// the keys that a set of rows sees: [0, first) and [lo, hi), lo >= first
+struct key_range {
+    int first, lo, hi;
+};
+// of the rows at positions p0 .. p1
+__device__ __forceinline__ key_range keys_of(const attn_desc &d, int L, int64_t p0, int64_t p1) {
+    key_range k;
+    k.hi = d.right < 0 ? L : (int) max((int64_t) 0, min((int64_t) L, p1 + d.right + 1));
+    k.lo = d.left < 0 ? 0 : (int) min((int64_t) k.hi, max((int64_t) 0, p0 - d.left));
+    k.first = min(d.sinks, k.lo);
+    return k;
+}
+
+// bit c set: column base + c lies in [a, b), c < 32
+__device__ __forceinline__ uint32_t bits32(int a, int b, int base) {
+    const int lo = min(max(a - base, 0), 32), hi = min(max(b - base, 0), 32);
+    const uint32_t below_hi = hi == 32 ? 0xffffffffu : (1u << hi) - 1u;
+    const uint32_t below_lo = lo == 32 ? 0xffffffffu : (1u << lo) - 1u;
+    return below_hi & ~below_lo;
+}
+
+// what a part's sums count for once the maximum is M; a part that saw no key
+// has (-inf, 0), one whose scores were NaN a NaN sum
+__device__ __forceinline__ float part_factor(float2 ml, float M) {
+    return ml.x == -INFINITY ? ml.y : ex2(ml.x - M);
+}
+
+__device__ __forceinline__ void store_out(__half *o, const float *v, int d0, int n, int D, bool vec) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+        if (e >= n) break;
+        if (vec && d0 + e + 8 <= D) {
+            __half2 h[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(v[e + 2 * i], v[e + 2 * i + 1]);
+            *reinterpret_cast<uint4 *>(o + d0 + e) = *reinterpret_cast<const uint4 *>(h);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (d0 + e + i < D) o[d0 + e + i] = __float2half_rn(v[e + i]);
+        }
+    }
+}
+
+template <int DB, bool SPLIT>
+__global__ void __launch_bounds__(320, 1)
+attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ at_params p) {
+    using cfg = at_cfg<DB, SPLIT>;
+    constexpr int ST = cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
+    // SPLIT, once the products are in: (m, sum) of every part's rows, and its O
+    float2 *s_ml = (float2 *) smem;
+    float *parts = (float *) (smem + cfg::NQ * cfg::TILE_BYTES);
+    uint64_t *bars = (uint64_t *) (smem + cfg::DATA);
+    uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
+    const uint32_t sq = smem_u32(smem), skv = sq + cfg::NQ * cfg::TILE_BYTES;
+    auto bar = [&](int i) { return smem_u32(bars + i); };
+    auto stage = [&](int s) { return skv + s * cfg::TILE_BYTES; };
+    auto full = [&](int s) { return bar(s); };
+    auto empty = [&](int s) { return bar(ST + s); };
+    auto s_full = [&](int t) { return bar(2 * ST + t); };      // S of warpgroup t is in TMEM
+    auto p_full = [&](int t) { return bar(2 * ST + 2 + t); };  // its P is in TMEM, S read, O rescaled
+    auto o_done = [&](int t) { return bar(2 * ST + 4 + t); };  // its O += P V is done
+    // the values of keys that no row sees are cleared: at most two tiles a CTA,
+    // the window's last and the sinks' last, each with a barrier of its own
+    auto v_fixed = [&](int i) { return bar(2 * ST + 6 + i); };
+    const uint32_t q_full = bar(2 * ST + 8), fin = bar(2 * ST + 9);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const attn_desc &d = p.d;
+    // block -> (cluster rank,) batch and key head, query tile (the last ones,
+    // which see most keys, first)
+    int idx = blockIdx.x;
+    const int rank = SPLIT ? idx % p.splits : 0;
+    if (SPLIT) idx /= p.splits;
+    const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);
+    const int b = bh / d.Hkv, hk = bh % d.Hkv;
+    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
+    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
+    const int tok0 = qt * p.tb * cfg::NQ;                        // the CTA's first token
+    const int toks = min(n - tok0, p.tb * cfg::NQ);              // and how many exist
+    if (toks <= 0) return;                                       // (the whole cluster alike)
+    const int64_t pos0 = (int64_t) L - n + tok0;
+    const key_range kr = keys_of(d, L, pos0, pos0 + toks - 1);
+    // tiles of the window, then of the sinks; SPLIT: this CTA's share of them
+    const int nwin = (kr.hi - kr.lo + 127) / 128, nall = nwin + (kr.first + 127) / 128;
+    const int i0 = SPLIT ? (int) ((int64_t) nall * rank / p.splits) : 0;
+    const int nt = (SPLIT ? (int) ((int64_t) nall * (rank + 1) / p.splits) : nall) - i0;
+    auto tile_key = [&](int j) { return i0 + j < nwin ? kr.lo + (i0 + j) * 128 : (i0 + j - nwin) * 128; };
+    auto tile_end = [&](int j) { return i0 + j < nwin ? kr.hi : kr.first; };
+    auto tile_keys = [&](int j) { return min(128, tile_end(j) - tile_key(j)); };
+    auto tile_w = [&](int j) { return (tile_keys(j) + 15) & ~15; };
+    // prompts: whether warpgroup t's rows see anything of tile j
+    const int toks0 = min(toks, p.tb), toks1 = toks - toks0;
+    const key_range kr0 = SPLIT ? kr : keys_of(d, L, pos0, pos0 + toks0 - 1);
+    const key_range kr1 = SPLIT ? kr : keys_of(d, L, pos0 + toks0, pos0 + toks - 1);
+    auto active = [&](int t, int j) {
+        if (SPLIT) return (j & 1) == t;
+        if (t == 1 && toks1 <= 0) return false;
+        const key_range &k = t ? kr1 : kr0;
+        const int a = tile_key(j);
+        return i0 + j >= nwin ? a < k.hi : a < k.hi && (a + 128 > k.lo || a < d.sinks);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(s_full(t), 1);
+            mbar_init(p_full(t), 4);
+            mbar_init(o_done(t), 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(v_fixed(0), 1);
+        mbar_init(v_fixed(1), 1);
+        mbar_init(fin, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto t_s = [&](int t) { return tmem + t * 128; };
+    auto t_o = [&](int t) { return tmem + 256 + t * DB * 64; };
+    bool ok = true;
+    // loads in the order that the MMA warp uses them: K(0) (K(1)), then V(j), K(j + AHEAD)
+    constexpr int AHEAD = SPLIT ? 2 : 1;
+
+    if (warp == 8) {
+        int cnt = 0, fixes = 0;
+        auto load = [&](const CUtensorMap *tm, int j) {
+            const int s = cnt % ST;
+            if (cnt >= ST && !warp_wait(empty(s), ((cnt / ST) - 1) & 1)) return false;
+            if (lane == 0) {
+                mbar_expect_tx(full(s), cfg::TILE_BYTES);
+                for (int x = 0; x < DB; x++) tma_load_4d(stage(s) + x * 16384, tm, full(s), x * 64, tile_key(j), hk, b);
+            }
+            cnt++;
+            return true;
+        };
+        if (lane == 0 && nt > 0) {
+            const uint32_t box = p.tb * p.g * 128;
+            mbar_expect_tx(q_full, box * DB * (SPLIT ? p.reps : 2));
+            for (int x = 0; x < DB; x++)
+                for (int r = 0; r < (SPLIT ? p.reps : 2); r++)
+                    tma_load_5d(sq + (SPLIT ? r * (128 / p.reps) * 128 : r * cfg::TILE_BYTES) + x * 16384, &tmQ, q_full,
+                                x * 64, 0, tok0 + (SPLIT ? 0 : r * p.tb), hk, b);
+        }
+        for (int j = 0; ok && j < min(AHEAD, nt); j++) ok = load(&tmK, j);
+        for (int j = 0; ok && j < nt; j++) {
+            const int s = cnt % ST, ph = (cnt / ST) & 1;
+            ok = load(&tmV, j);
+            const int keys = tile_keys(j), w = tile_w(j);
+            if (ok && keys < w) {
+                // values of keys that no row sees: cleared (their weights are zero)
+                ok = warp_wait(full(s), ph);
+                if (!ok) break;
+                for (int i = lane; i < (w - keys) * 8 * DB; i += 32) {
+                    const int x = i / ((w - keys) * 8), o = i % ((w - keys) * 8);
+                    *reinterpret_cast<uint4 *>(smem + (stage(s) - sq) + x * 16384 + keys * 128 + o * 16) =
+                        make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_fixed(fixes));
+                fixes++;
+            }
+            if (ok && j + AHEAD < nt) ok = load(&tmK, j + AHEAD);
+        }
+        // the copies in flight land before the CTA goes on
+        for (int i = max(0, cnt - ST); i < cnt; i++)
+            if (!warp_wait(full(i % ST), (i / ST) & 1)) ok = false;
+        if (nt > 0 && !warp_wait(q_full, 0)) ok = false;
+        if (!ok && lane == 0) atomicExch(p.err, 1);
+    } else if (warp == 9) {
+        if (lane == 0 && nt > 0) {
+            // D f32 (bit 4), f16 operands; M >> 4 at bit 24, N >> 3 at bit 17; B along N (bit 16) for V
+            const uint32_t id_base = (1u << 4) | (8u << 24);
+            const int ksteps = (d.D + 15) / 16;
+            const uint32_t id_pv = id_base | (1u << 16) | ((uint32_t) (ksteps * 2) << 17);
+            int cnt = 0, fixes = 0;
+            auto wait_tile = [&](int c) { return mbar_wait(full(c % ST), (c / ST) & 1); };
+            auto qk = [&](int t, int j, int c) {
+                const uint32_t a = sq + (SPLIT ? 0 : t * cfg::TILE_BYTES), bb = stage(c % ST);
+                const uint32_t id = id_base | ((uint32_t) (tile_w(j) >> 3) << 17);
+                for (int k = 0; k < ksteps; k++) {
+                    const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
+                    umma_f16(t_s(t), smem_desc(a + o, 1024, 2), smem_desc(bb + o, 1024, 2), id, k > 0);
+                }
+                umma_commit(s_full(t));
+            };
+            int done[2] = {0, 0};
+            int kc[AHEAD + 1];  // load number of K(j + x)
+            ok = mbar_wait(q_full, 0);
+            for (int j = 0; ok && j < min(AHEAD, nt); j++) {
+                kc[j] = cnt++;
+                ok = wait_tile(kc[j]);
+                if (!ok) break;
+                tc_fence_after();
+                for (int t = 0; t < 2; t++)
+                    if (active(t, j)) qk(t, j, kc[j]);
+                umma_commit(empty(kc[j] % ST));
+            }
+            for (int j = 0; ok && j < nt; j++) {
+                const int vc = cnt++;
+                ok = wait_tile(vc);
+                if (ok && tile_keys(j) < tile_w(j)) ok = mbar_wait(v_fixed(fixes++), 0);
+                const bool more = j + AHEAD < nt;
+                const int nkc = more ? cnt++ : 0;
+                bool k_here = false;
+                for (int t = 0; ok && t < 2; t++) {
+                    if (active(t, j)) {
+                        ok = mbar_wait(p_full(t), done[t] & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t v = stage(vc % ST);
+                        for (int k = 0; k < tile_w(j) / 16; k++)
+                            umma_f16_ts(t_o(t), t_s(t) + k * 8, smem_desc_mn(v + k * 2048, 16384, 1024), id_pv,
+                                        done[t] > 0 || k > 0);
+                        umma_commit(o_done(t));
+                        done[t]++;
+                    }
+                    if (more && active(t, j + AHEAD)) {
+                        if (!k_here) {
+                            ok = wait_tile(nkc);
+                            if (!ok) break;
+                            k_here = true;
+                            tc_fence_after();
+                        }
+                        qk(t, j + AHEAD, nkc);
+                    }
+                }
+                if (ok && more && !k_here) ok = wait_tile(nkc);
+                umma_commit(empty(vc % ST));
+                if (more) umma_commit(empty(nkc % ST));
+            }
+            // the MMAs in flight end before TMEM is freed
+            umma_commit(fin);
+            if (!mbar_wait(fin, 0)) ok = false;
+            if (!ok) atomicExch(p.err, 1);
+        }
+    } else {
+        const int t = warp >> 2, q4 = warp & 3;
+        const int per = SPLIT ? 128 / p.reps : 128;       // lanes of a copy of the rows
+        const int rep = SPLIT ? q4 * 32 / per : 0;
+        const int r = q4 * 32 + lane - rep * per;         // row of the tile
+        const int tok = tok0 + (SPLIT ? 0 : t * p.tb) + r / p.g, h = hk * p.g + r % p.g;
+        const bool row = r < p.tb * p.g && tok < n;
+        const bool rows = __any_sync(0xffffffffu, row);
+        const key_range kk = keys_of(d, L, (int64_t) L - n + tok, (int64_t) L - n + tok);
+        const uint32_t lanes = (uint32_t) (q4 * 32) << 16;
+        // the share of each tile's columns that this copy takes, in chunks of 32
+        const int c0 = SPLIT ? rep * (4 / p.reps) : 0, c1 = SPLIT ? c0 + 4 / p.reps : 4;
+        float m = -INFINITY, l = 0.0f;
+        int done = 0;
+        for (int j = 0; j < nt; j++) {
+            if (!active(t, j)) continue;
+            ok = warp_wait(s_full(t), done & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (rows) {
+                const int kb = tile_key(j), w = tile_w(j);
+                const bool win = i0 + j < nwin;
+                // of the window's tiles the row sees [lo, hi) and what lies below
+                // sinks, of the sinks' tiles [0, first) below hi
+                const int a0 = win ? kk.lo : 0, a1 = win ? kk.hi : min(kr.first, kk.hi);
+                const int a2 = win ? min(d.sinks, kk.hi) : 0;
+                const bool all = __all_sync(0xffffffffu, a0 <= kb && kb + 128 <= a1);
+                float s[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c * 32 < w && (!SPLIT || (c >= c0 && c < c1))) {
+                        tmem_ld32_async(t_s(t) + lanes + c * 32, s + c * 32);
+                        if (!all) {
+                            const uint32_t see = bits32(a0, a1, kb + c * 32) | bits32(0, a2, kb + c * 32);
+#pragma unroll
+                            for (int e = 0; e < 32; e++)
+                                if (!(see >> e & 1)) s[c * 32 + e] = -INFINITY;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) s[c * 32 + e] = -INFINITY;
+                    }
+                }
+                float mx[4] = {m, m, m, m};
+#pragma unroll
+                for (int e = 0; e < 128; e++) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // (m - m_old) scale log2(e) above 8, or a first finite maximum
+                const bool up = mn > m && !((mn - m) * p.c <= 8.0f);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float f = up ? ex2((m - mn) * p.c) : 1.0f;
+                    if (up) m = mn;
+                    l *= f;
+                    if (done > 0) {  // O so far, once the last product is in
+                        ok = warp_wait(o_done(t), (done - 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int x = 0; x < DB * 64; x += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o(t) + lanes + x, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(t_o(t) + lanes + x, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.0f : m * p.c;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c * 32 >= w) break;
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float x = ex2(fmaf(s[c * 32 + e], p.c, -mc)), y = ex2(fmaf(s[c * 32 + e + 1], p.c, -mc));
+                        sum[e & 2] += x;
+                        sum[(e & 2) + 1] += y;
+                        const __half2 hh = __floats2half2_rn(x, y);
+                        pk[e / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                    }
+                    tmem_st16(t_s(t) + lanes + c * 16, pk);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(t));
+            done++;
+        }
+        if (ok && done > 0) ok = warp_wait(o_done(t), (done - 1) & 1);
+        tc_fence_after();
+        if (!ok && lane == 0) atomicExch(p.err, 1);
+        if constexpr (!SPLIT) {
+            if (ok && rows) {
+                const float inv = 1.0f / l;
+                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
+                bool bad = false;
+#pragma unroll 1
+                for (int x = 0; x < DB * 64; x += 32) {
+                    float o[32];
+                    if (done > 0) tmem_ld32_async(t_o(t) + lanes + x, o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+                        bad = bad || (x + e < d.D && !(fabsf(o[e]) <= 65504.0f));
+                    }
+                    if (row) store_out(out, o, x, 32, d.D, p.o_vec);
+                }
+                uint32_t redo = __ballot_sync(0xffffffffu, bad && row);
+                __syncwarp();
+                for (; redo; redo &= redo - 1) {
+                    const int src = __ffs(redo) - 1;
+                    attn_row<__half, 4>(d, b, __shfl_sync(0xffffffffu, h, src), __shfl_sync(0xffffffffu, tok, src), n, L,
+                                        lane);
+                }
+            }
+        } else {
+            // every part's (m, sum) and O to shared memory: part = warpgroup, copy
+            named_sync(1, 256);  // (both warpgroups' products are in: Q and the stages are free)
+            if (row) s_ml[(t * p.reps + rep) * per + r] = make_float2(m == -INFINITY ? -INFINITY : m * p.c, l);
+            if (rows) {
+#pragma unroll 1
+                for (int x = 0; x < DB * 64; x += 32) {
+                    float o[32];
+                    if (done > 0) {
+                        tmem_ld32_async(t_o(t) + lanes + x, o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.0f;
+                    }
+                    if (row) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4 *>(parts + ((t * p.reps + rep) * per + r) * cfg::OLD + x + e) =
+                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+            }
+            named_sync(1, 256);
+            // join the CTA's parts into part 0
+            constexpr int C4 = DB * 16;  // 4-column pieces a row
+            const int np = 2 * p.reps, items = min(p.tb, toks) * p.g * C4;
+            for (int base = warp * 32; base < items; base += 256) {
+                const int i = min(base + lane, items - 1), rr = i / C4, x = i % C4 * 4;
+                float M = -INFINITY;
+                for (int k = 0; k < np; k++) M = fmaxf(M, s_ml[k * per + rr].x);
+                float sl = 0.0f;
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int k = 0; k < np; k++) {
+                    const float2 ml = s_ml[k * per + rr];
+                    const float f = part_factor(ml, M);
+                    const float4 v = *reinterpret_cast<const float4 *>(parts + (k * per + rr) * cfg::OLD + x);
+                    sl = fmaf(f, ml.y, sl);
+                    o.x = fmaf(f, v.x, o.x);
+                    o.y = fmaf(f, v.y, o.y);
+                    o.z = fmaf(f, v.z, o.z);
+                    o.w = fmaf(f, v.w, o.w);
+                }
+                __syncwarp();  // (a row's lanes are of one warp: all have read its first part)
+                if (base + lane < items) {
+                    *reinterpret_cast<float4 *>(parts + rr * cfg::OLD + x) = o;
+                    if (x == 0) s_ml[rr] = make_float2(M, sl);
+                }
+            }
+            named_sync(1, 256);
+        }
+    }
+    if constexpr (SPLIT) {
+        if (p.splits > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        if (warp < 8) {
+            constexpr int C4 = DB * 16;
+            const int nrow = min(p.tb, toks) * p.g, items = nrow * C4;
+            const uint32_t a_ml = smem_u32(s_ml), a_o = smem_u32(parts);
+            for (int i0b = rank * 256; i0b < items; i0b += p.splits * 256) {
+                const int i = i0b + threadIdx.x, rr = min(i, items - 1) / C4, x = i % C4 * 4;
+                float M = -INFINITY, sl = 0.0f;
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int k = 0; k < p.splits; k++) M = fmaxf(M, ld_cluster2(cluster_addr(a_ml + rr * 8, k)).x);
+                for (int k = 0; k < p.splits; k++) {
+                    const float2 ml = ld_cluster2(cluster_addr(a_ml + rr * 8, k));
+                    const float f = part_factor(ml, M);
+                    const float4 v = ld_cluster4(cluster_addr(a_o + (rr * cfg::OLD + x) * 4, k));
+                    sl = fmaf(f, ml.y, sl);
+                    o.x = fmaf(f, v.x, o.x);
+                    o.y = fmaf(f, v.y, o.y);
+                    o.z = fmaf(f, v.z, o.z);
+                    o.w = fmaf(f, v.w, o.w);
+                }
+                const float inv = 1.0f / sl;
+                float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+                const int tok = tok0 + rr / p.g, h = hk * p.g + rr % p.g;
+                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
+                bool bad = false;
+                if (i < items) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (sl == 0.0f) v[e] = 0.0f;
+                        bad = bad || (x + e < d.D && !(fabsf(v[e]) <= 65504.0f));
+                    }
+                    if (p.o_vec && x + 4 <= d.D) {
+                        const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
+                        uint2 w2;
+                        w2.x = *reinterpret_cast<const uint32_t *>(&h0);
+                        w2.y = *reinterpret_cast<const uint32_t *>(&h1);
+                        *reinterpret_cast<uint2 *>(out + x) = w2;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (x + e < d.D) out[x + e] = __float2half_rn(v[e]);
+                    }
+                }
+                uint32_t redo = __ballot_sync(0xffffffffu, bad);
+                while (redo) {
+                    const int src = __ffs(redo) - 1;
+                    // C4 lanes (all of the warp, or half) hold a row
+                    redo &= C4 == 32 ? 0u : src < 16 ? 0xffff0000u : 0u;
+                    __syncwarp();
+                    attn_row<__half, 4>(d, b, __shfl_sync(0xffffffffu, h, src), __shfl_sync(0xffffffffu, tok, src), n, L,
+                                        lane);
+                }
+            }
+        }
+        // no CTA leaves while others read its parts
+        if (p.splits > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// a tensor map over f16 memory: dims and strides (elements) innermost first,
+// the innermost contiguous
+bool encode_f16(CUtensorMap *tm, const void *base, int rank, const int64_t *dims, const int64_t *strides,
+                const int *box) {
+    auto enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t gd[5], gs[4];
+    cuuint32_t bx[5], es[5];
+    for (int i = 0; i < rank; i++) {
+        gd[i] = (cuuint64_t) dims[i];
+        bx[i] = (cuuint32_t) box[i];
+        es[i] = 1;
+        // a dimension of one element has no stride of its own
+        if (i) gs[i - 1] = (cuuint64_t) (dims[i] > 1 ? strides[i] * 2 : 16);
+    }
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, (void *) base, gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DB, bool SPLIT>
+cudaError_t run_tc(const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, const at_params &p,
+                   unsigned ctas, cudaStream_t st) {
+    using cfg = at_cfg<DB, SPLIT>;
+    static std::mutex mu;
+    static uint64_t attr_set = 0;  // one bit per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    {
+        std::lock_guard<std::mutex> g(mu);
+        if (!(attr_set >> (dev & 63) & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<DB, SPLIT>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, cfg::SMEM);
+            if (e != cudaSuccess) return e;
+            attr_set |= 1ull << (dev & 63);
+        }
+    }
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(ctas, 1, 1);
+    lc.blockDim = dim3(cfg::THREADS, 1, 1);
+    lc.dynamicSmemBytes = cfg::SMEM;
+    lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) p.splits;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    lc.attrs = at;
+    lc.numAttrs = p.splits > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&lc, attn_tc_kernel<DB, SPLIT>, tmQ, tmK, tmV, p);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+// whether TMA can address a tensor: 16-byte aligned base and strides, no
+// stride of 0 or backwards over more than one element
+bool tma_ok(const void *base, const int64_t *s, int64_t n0, int64_t n1, int64_t n2) {
+    const int64_t dim[3] = {n0, n1, n2};
+    if ((uintptr_t) base & 15) return false;
+    for (int i = 0; i < 3; i++)
+        if (dim[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= 1ll << 38)) return false;
+    return true;
+}
+
+}  // namespace
+
+bool attn_tc_supported(const attn_desc &d) {
+    return d.f16 && d.D <= 128 && d.Tk > 0 && d.Hq / d.Hkv <= 128 && d.scale > 0.0f &&
+           tma_ok(d.q, d.qs, d.B, d.Tq, d.Hq) && tma_ok(d.k, d.ks, d.B, d.Tk, d.Hkv) &&
+           tma_ok(d.v, d.vs, d.B, d.Tk, d.Hkv) && d.qs[2] * (d.Hq / d.Hkv) < 1ll << 38;
+}
+
+cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st) {
+    at_params p{};
+    p.d = d;
+    p.g = d.Hq / d.Hkv;
+    p.c = d.scale * 1.4426950408889634f;
+    p.o_vec = !((uintptr_t) d.out & 15) && (d.B == 1 || d.os[0] % 8 == 0) && (d.Tq == 1 || d.os[1] % 8 == 0) &&
+              (d.Hq == 1 || d.os[2] % 8 == 0);
+    p.err = tpk_err_word();
+    if (!p.err) return cudaErrorUnknown;
+    const int64_t bh = (int64_t) d.B * d.Hkv;
+    const int sms = sm_count(), tb = 128 / p.g;
+    // two row tiles a CTA where that fills the SMs; otherwise one, its keys
+    // shared out over both warpgroups and a cluster
+    const bool split = bh * ((d.Tq + 2 * tb - 1) / (2 * tb)) < sms;
+    p.tb = split ? std::min(tb, d.Tq) : tb;
+    const int rows = p.tb * p.g;
+    p.reps = !split || rows > 64 ? 1 : rows > 32 ? 2 : 4;
+    const int per_cta = split ? p.tb : 2 * p.tb;
+    p.qtiles = (d.Tq + per_cta - 1) / per_cta;
+    p.splits = 1;
+    if (split) {
+        int64_t keys = d.Tk;
+        if (d.left >= 0 && d.right >= 0) keys = std::min<int64_t>(keys, (int64_t) p.tb + d.left + d.right + d.sinks);
+        const int64_t tiles = (keys + 127) / 128, ctas = bh * p.qtiles;
+        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>({8, sms / ctas, (tiles + 1) / 2}));
+    }
+    const int64_t ctas = bh * p.qtiles * p.splits;
+    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+    CUtensorMap tmQ, tmK, tmV;
+    const int64_t qd[5] = {d.D, p.g, d.Tq, d.Hkv, d.B}, qs[5] = {1, d.qs[2], d.qs[1], d.qs[2] * p.g, d.qs[0]};
+    const int64_t kd[4] = {d.D, d.Tk, d.Hkv, d.B};
+    const int64_t ks[4] = {1, d.ks[1], d.ks[2], d.ks[0]}, vs[4] = {1, d.vs[1], d.vs[2], d.vs[0]};
+    const int qb[5] = {64, p.g, p.tb, 1, 1}, kb[4] = {64, 128, 1, 1};
+    if (!encode_f16(&tmQ, d.q, 5, qd, qs, qb) || !encode_f16(&tmK, d.k, 4, kd, ks, kb) ||
+        !encode_f16(&tmV, d.v, 4, kd, vs, kb))
+        return cudaErrorInvalidValue;
+    const unsigned n = (unsigned) ctas;
+    if (d.D <= 64)
+        return split ? run_tc<1, true>(tmQ, tmK, tmV, p, n, st) : run_tc<1, false>(tmQ, tmK, tmV, p, n, st);
+    return split ? run_tc<2, true>(tmQ, tmK, tmV, p, n, st) : run_tc<2, false>(tmQ, tmK, tmV, p, n, st);
+}
+
+}  // namespace tpmd

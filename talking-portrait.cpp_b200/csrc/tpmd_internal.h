@@ -196,6 +196,9 @@ struct attn_desc {
     float scale;
 };
 cudaError_t launch_attn_simt(const attn_desc &d, cudaStream_t st);
+// the tensor-core form: f16, D <= 128, what TMA can address
+bool attn_tc_supported(const attn_desc &d);
+cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st);
 
 // The tcgen05 GEMM of the sampler and the audio encoder (kernels_gemm_tc.cu):
 //   Y[m][n] = act((sum_k X[m][k] W[n][k] + bias[n]) * scale) (+ res[m][n]), m < M, n < N

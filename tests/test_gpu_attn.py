@@ -109,6 +109,43 @@ def test_shapes(case, dtype):
     check(*make(B, Tq, Tk, Hq, Hkv, D, dtype), left, right, sinks)
 
 
+# many rows: enough work for every SM without sharing out keys
+MANY = [(8, 600, 600, 12, 6, 64, 99, 0, 3), (3, 1300, 1300, 40, 10, 128, 200, 31, 140), (2, 2049, 2049, 16, 16, 80, 64, 0, 1),
+        (40, 250, 300, 12, 4, 128, -1, 0, 0), (1, 2000, 2000, 30, 30, 32, 3, 3, 5), (4, 515, 515, 100, 20, 40, 0, -1, 2),
+        (150, 1, 700, 4, 2, 128, 300, 0, 4), (160, 3, 200, 2, 1, 64, -1, 0, 0)]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(map(str, c)))
+def test_many_rows(case):
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = case
+    q, k, v = make(B, Tq, Tk, Hq, Hkv, D, "f16", gain=3.0)
+    check(q, k, v, left, right, sinks)
+    # lengths of their own; NaN and infinities behind the ends
+    n = lens(*[Tq * (7 * i % (B + 1)) // B for i in range(B)])
+    L = lens(*[x if Tq == Tk else max(x, Tk * (5 * i % (B + 1)) // B) for i, x in enumerate(n.tolist())])
+    for b, x in enumerate(L.tolist()):
+        k[b, x:], v[b, x:] = float("nan"), float("inf")
+    check(q, k, v, left, right, sinks, q_len=n, kv_len=L)
+
+
+def test_poison_in_many_rows():
+    """as test_poison_beside_the_window, with the rows of many heads"""
+    T, H = 400, 80
+    q, k, v = make(1, T, T, 2 * H, H, 64, "f16")
+    v[0, 150, :, 3] = float("inf")
+    clean = v.clone()
+    clean[0, 150, :, 3] = 0.0
+    out = torch.empty_like(q)
+    tpmd.attn_window(q, k, v, out, 10, 0, 0)
+    tpmd.tpk_status()
+    ref, bound, _ = reference(q, k, clean, 10, 0, 0, 64 ** -0.5)
+    got = out.cpu().double()[0]
+    bad = torch.zeros(T, 2 * H, 64, dtype=torch.bool)
+    bad[150:161, :, 3] = True
+    assert not bool(got[bad].isfinite().any())
+    assert bool(((got - ref[0]).abs() <= bound[0])[~bad].all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_large_scores(dtype):
     """scores in the hundreds: the running maximum carries the softmax"""
