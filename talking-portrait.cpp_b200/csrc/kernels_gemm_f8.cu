@@ -4,21 +4,28 @@
 //   Y[m][n] = act( sum_b sx[m][b] sw[n/128][b] P_b[m][n] + bias[n] ),
 //   P_b[m][n] = sum_{k in block b} X[m][k] W[n][k],  blocks of 128 along k
 //
-// A CTA owns a 128 x 128 output tile: 128 rows of X are the MMA's M side
-// (TMEM lanes), one block of 128 rows of W its N side, so all of a tile's
-// W scales of one k block are one number and a lane's factor sx sw is one
-// number for all its columns. Each k block of 128 is one pipeline stage (one
+// An output tile is 128 x 128 or 128 x 256: 128 rows of X are the MMA's M
+// side (TMEM lanes), one or two blocks of 128 rows of W its N side, so a
+// block's W scale of one k block is one number and a lane's factor sx sw is
+// one number for all its 128 columns. Each k block of 128 is one pipeline stage (one
 // 128-byte swizzled row a matrix row) and one MMA group into an accumulator
-// of its own out of a ring in TMEM; eight warps read it (each a lane
-// quarter and half of the columns), scale it and add it to f32 registers
-// while the next blocks multiply. The products of e4m3 values are exact in
+// of its own out of a ring in TMEM; the epilogue warps (each a lane quarter
+// and 64 columns) read it, scale it and add it to f32 registers while the
+// next blocks multiply. The products of e4m3 values are exact in
 // f32; sums are f32 throughout.
+//
+// With 128 x 256 tiles (products that fill the SMs) CTAs are persistent: the
+// loads and products of the next tile run on while a tile is written. With
+// 128 x 128 tiles a CTA has one, and where SMs are left the k blocks of a
+// tile are shared out over a cluster of up to eight CTAs; each leaves its
+// partial tile in its shared memory, and each adds its rows of all of them
+// (distributed shared memory), always in the same order.
 //
 // Every pipeline wait is bounded; an expired wait sets *err and the CTA
 // skips the rest of its work.
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
+#include "f8.cuh"
 #include "tc_ptx.cuh"
 #include "tpmd_internal.h"
 #include "../../include/tpmd.h"
@@ -31,9 +38,6 @@
 namespace tpmd {
 namespace {
 
-constexpr float F8_MAX = 448.0f;
-constexpr float S_MIN = 1.17549435e-38f;  // 2^-126
-
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
     const uint32_t mask = 0;
@@ -44,28 +48,40 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(mask));
 }
 
-__device__ __forceinline__ float act_fn(float v, int act) {
+__device__ __forceinline__ float act_one(float v, int act) {
     if (act == 1) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    if (act == 2) return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * (v + 0.044715f * v * v * v)));
+    // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
+    if (act == 2) return __fdividef(v, 1.0f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
     if (act == 3) return fmaxf(v, 0.2f * v);
     return v;
 }
+// of four values; a call, so that the epilogues stay within the instruction caches
+__device__ __noinline__ float4 act4_call(float4 v, int act) {
+    return make_float4(act_one(v.x, act), act_one(v.y, act), act_one(v.z, act), act_one(v.w, act));
+}
+__device__ __forceinline__ float4 act4(float4 v, int act) { return act == 0 ? v : act4_call(v, act); }
 
+// NB: blocks of 128 columns a tile
+template <int NB>
 struct f8_cfg {
-    static constexpr int BM = 128, BN = 128, KB = 128;
+    static constexpr int BM = 128, BN = 128 * NB, KB = 128;
     static constexpr int A_BYTES = BM * KB, B_BYTES = BN * KB, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 6, NACC = 4;
-    static constexpr uint32_t TMEM_COLS = NACC * BN;
+    static constexpr int STAGES = NB == 2 ? 4 : 6, NACC = 4 / NB;
+    static constexpr uint32_t TMEM_COLS = 512;
     // D f32 (bit 4); A and B e4m3 (0 at bits 7 and 10); K-major both; N >> 3 at bit 17; M >> 4 at bit 24
     static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (BN >> 3) << 17) | ((uint32_t) (BM >> 4) << 24);
-    static constexpr int NEPI = 8, THREADS = 64 + 32 * NEPI;
+    static constexpr int NEPI = 8 * NB, THREADS = 64 + 32 * NEPI;
     static constexpr int NBARS = 2 * STAGES + 2 * NACC;
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + NBARS * 8 + 16;
+    // a warp's staged 32 x 16 floats; floats a row of a split's partial tile (16-byte bank shifts)
+    static constexpr int PIECE = 32 * 16, PART_LD = 132;
+    static constexpr int PIECE_BYTES = NEPI * PIECE * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + PIECE_BYTES + NBARS * 8 + 16;
     static_assert(SMEM <= 232448, "shared memory");
+    static_assert(BM * PART_LD * 4 <= STAGES * STAGE_BYTES, "a partial tile fits the stages");
 };
 
 struct f8_params {
-    int M, N, K, kblocks, tiles_n;
+    int M, N, K, kblocks, tiles_n, tiles, splits, kb_per_split;
     const float *sx, *sw, *bias;
     int64_t ldsx, ldsw;
     void *Y;
@@ -73,79 +89,104 @@ struct f8_params {
     float *sy;
     int64_t ldsy;
     int act;
-    bool y_vec;  // Y takes 16-byte stores
+    bool y_vec;  // Y takes stores of four elements
     int *err;
 };
 
-// N values of one row to Y columns [n, n + CNT)
-template <typename TY, int CNT>
-__device__ __forceinline__ void store_cols(TY *y, const TY (&v)[CNT], int n, int N, bool vec) {
-    constexpr int PER = 16 / sizeof(TY);
-#pragma unroll
-    for (int c = 0; c < CNT; c += PER) {
-        if (vec && n + c + PER <= N) {
-            *reinterpret_cast<uint4 *>(y + n + c) = *reinterpret_cast<const uint4 *>(v + c);
+// (a0, a1) += (x0, x1) * s, two f32 multiply-adds in one instruction
+__device__ __forceinline__ void fma2(float &a0, float &a1, uint32_t x0, uint32_t x1, float s) {
+    asm("{\n\t.reg .b64 a, x, f;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 f, {%4, %4};\n\t"
+        "fma.rn.f32x2 a, x, f, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "r"(x0), "r"(x1), "f"(s));
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_rank4(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
+// four values of a row to Y columns n .. n + 3 (F8: quantised by s)
+template <int YT>
+__device__ __forceinline__ void store4(const f8_params &p, int64_t m, int n, const float (&v)[4], f8_scale s) {
+    if constexpr (YT == TPMD_DTYPE_F8) {
+        uint8_t *y = (uint8_t *) p.Y + m * p.ldy + n;
+        const uint32_t q = f8_quant4(v[0], v[1], v[2], v[3], s);
+        if (p.y_vec && n + 4 <= p.N) {
+            *reinterpret_cast<uint32_t *>(y) = q;
         } else {
-#pragma unroll
-            for (int e = 0; e < PER; e++)
-                if (n + c + e < N) y[n + c + e] = v[c + e];
+#pragma unroll 1
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.N) y[e] = (uint8_t) (q >> 8 * e);
+        }
+    } else if constexpr (YT == TPMD_DTYPE_F16) {
+        __half *y = (__half *) p.Y + m * p.ldy + n;
+        if (p.y_vec && n + 4 <= p.N) {
+            const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+            uint2 w;
+            w.x = *reinterpret_cast<const uint32_t *>(&a);
+            w.y = *reinterpret_cast<const uint32_t *>(&b);
+            *reinterpret_cast<uint2 *>(y) = w;
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.N) y[e] = __float2half_rn(e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]);
+        }
+    } else {
+        float *y = (float *) p.Y + m * p.ldy + n;
+        if (p.y_vec && n + 4 <= p.N) {
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.N) y[e] = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
         }
     }
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// AND of v over the epilogue threads (named barrier 1)
-__device__ __forceinline__ bool epi_all(bool v) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.and.pred q, 1, 256, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((uint32_t) v)
-        : "memory");
-    return r != 0;
-}
-
 // YT: TPMD_DTYPE_* of Y
-template <int YT>
-__global__ void __launch_bounds__(f8_cfg::THREADS, 1)
-gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const f8_params p) {
-    using cfg = f8_cfg;
+template <int YT, int NB>
+__global__ void __launch_bounds__(f8_cfg<NB>::THREADS, 1)
+gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+               const __grid_constant__ f8_params p) {
+    using cfg = f8_cfg<NB>;
+    constexpr int ST = cfg::STAGES, NA = cfg::NACC;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ float red[2][cfg::BM];
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    uint64_t *bars = (uint64_t *) (smem + cfg::STAGES * cfg::STAGE_BYTES);
+    float *pieces = (float *) (smem + ST * cfg::STAGE_BYTES);
+    uint64_t *bars = (uint64_t *) (smem + ST * cfg::STAGE_BYTES + cfg::PIECE_BYTES);
     uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
     auto A = [&](int s) { return smem_u32(smem) + s * cfg::STAGE_BYTES; };
     auto B = [&](int s) { return A(s) + cfg::A_BYTES; };
     auto full = [&](int s) { return smem_u32(&bars[s]); };
-    auto empty = [&](int s) { return smem_u32(&bars[cfg::STAGES + s]); };
-    auto tfull = [&](int a) { return smem_u32(&bars[2 * cfg::STAGES + a]); };
-    auto tempty = [&](int a) { return smem_u32(&bars[2 * cfg::STAGES + cfg::NACC + a]); };
+    auto empty = [&](int s) { return smem_u32(&bars[ST + s]); };
+    auto tfull = [&](int a) { return smem_u32(&bars[2 * ST + a]); };
+    auto tempty = [&](int a) { return smem_u32(&bars[2 * ST + NA + a]); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nb = blockIdx.x % p.tiles_n, n0 = nb * cfg::BN, m0 = (blockIdx.x / p.tiles_n) * cfg::BM;
-    const int nk = p.kblocks;
+    const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits, ctas = gridDim.x / p.splits;
+    const int kb0 = split * p.kb_per_split, nk = min(p.kblocks - kb0, p.kb_per_split);  // nk >= 1 (host)
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < cfg::STAGES; s++) {
+        for (int s = 0; s < ST; s++) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        for (int a = 0; a < cfg::NACC; a++) {
+        for (int a = 0; a < NA; a++) {
             mbar_init(tfull(a), 1);
             mbar_init(tempty(a), cfg::NEPI);
         }
@@ -166,114 +207,250 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 
     if (warp == 0) {
         if (lane == 0) {  // TMA producer
-            int issued = 0;
-            for (int i = 0; i < nk; i++) {
-                const int s = i % cfg::STAGES;
-                if (i >= cfg::STAGES && !mbar_wait(empty(s), ((i / cfg::STAGES) - 1) & 1)) {
-                    ok = false;
-                    break;
+            int c = 0;
+            for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
+                const int n0 = tile % p.tiles_n * cfg::BN, m0 = tile / p.tiles_n * cfg::BM;
+                for (int i = 0; i < nk; i++, c++) {
+                    const int s = c % ST;
+                    if (c >= ST && !mbar_wait(empty(s), ((c / ST) - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(full(s), cfg::STAGE_BYTES);
+                    tma_load_2d(A(s), &tmX, full(s), (kb0 + i) * cfg::KB, m0);
+                    tma_load_2d(B(s), &tmW, full(s), (kb0 + i) * cfg::KB, n0);
                 }
-                mbar_expect_tx(full(s), cfg::STAGE_BYTES);
-                tma_load_2d(A(s), &tmX, full(s), i * cfg::KB, m0);
-                tma_load_2d(B(s), &tmW, full(s), i * cfg::KB, n0);
-                issued++;
             }
             // the copies in flight land before the CTA goes on
-            for (int j = issued > cfg::STAGES ? issued - cfg::STAGES : 0; j < issued; j++)
-                if (!mbar_wait(full(j % cfg::STAGES), (j / cfg::STAGES) & 1)) ok = false;
+            for (int j = max(0, c - ST); j < c; j++)
+                if (!mbar_wait(full(j % ST), (j / ST) & 1)) ok = false;
             if (!ok) atomicExch(p.err, 1);
         }
     } else if (warp == 1) {
         if (lane == 0) {  // MMA issuer
-            int done = 0;
-            for (int i = 0; i < nk; i++, done++) {
-                const int s = i % cfg::STAGES, a = i % cfg::NACC;
-                if (!mbar_wait(full(s), (i / cfg::STAGES) & 1) ||
-                    (i >= cfg::NACC && !mbar_wait(tempty(a), ((i / cfg::NACC) - 1) & 1))) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
+            int c = 0;
+            for (int tile = cta; ok && tile < p.tiles; tile += ctas)
+                for (int i = 0; i < nk; i++, c++) {
+                    const int s = c % ST, a = c % NA;
+                    if (!mbar_wait(full(s), (c / ST) & 1) || (c >= NA && !mbar_wait(tempty(a), ((c / NA) - 1) & 1))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < cfg::KB / 32; kk++)
-                    umma_f8(tmem + a * cfg::BN, smem_desc(A(s) + kk * 32, 1024, 2), smem_desc(B(s) + kk * 32, 1024, 2),
-                            cfg::IDESC, kk > 0);
-                umma_commit(empty(s));
-                umma_commit(tfull(a));
-            }
+                    for (int kk = 0; kk < cfg::KB / 32; kk++)
+                        umma_f8(tmem + a * cfg::BN, smem_desc(A(s) + kk * 32, 1024, 2),
+                                smem_desc(B(s) + kk * 32, 1024, 2), cfg::IDESC, kk > 0);
+                    umma_commit(empty(s));
+                    umma_commit(tfull(a));
+                }
             // the MMAs in flight end before TMEM is freed
-            for (int j = max(0, done - cfg::NACC); j < done; j++)
-                if (!mbar_wait(tfull(j % cfg::NACC), (j / cfg::NACC) & 1)) ok = false;
+            for (int j = max(0, c - NA); j < c; j++)
+                if (!mbar_wait(tfull(j % NA), (j / NA) & 1)) ok = false;
             if (!ok) atomicExch(p.err, 1);
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane, m = m0 + row;
-        const uint32_t taddr = tmem + ((uint32_t) (q * 32) << 16) + half * 64;
-        const float *sxr = p.sx + (int64_t) (m < p.M ? m : 0) * p.ldsx, *swr = p.sw + (int64_t) nb * p.ldsw;
-        float acc[64];
+        // a warp: a lane quarter (32 rows) and half of a block of 128 columns
+        const int q = warp & 3, blk = (warp - 2) >> 3, half = (warp - 2) >> 2 & 1, pair = blk * 4 + q;
+        const uint32_t taddr = tmem + ((uint32_t) (q * 32) << 16) + blk * 128 + half * 64;
+        float *piece = pieces + (warp - 2) * cfg::PIECE;
+        int c = 0;
+        for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
+            const int nb = tile % p.tiles_n * NB + blk, n0 = nb * 128 + half * 64, m0 = tile / p.tiles_n * cfg::BM + q * 32;
+            const int m = m0 + lane;
+            // the factors sx sw of the warp's 32 rows, eight k blocks at a time,
+            // through the warp's shared memory (two buffers of 8 x 32): a load
+            // takes eight blocks of four rows (whole sectors), the next eight
+            // blocks' loads go out one a step. Row r of block e is at
+            // e * 32 + (r ^ 4 e), free of bank conflicts either way. (Rows and
+            // blocks behind the last one have factors of the last one.)
+            const int fe = lane % 8, fr = lane / 8;
+            const float *swr = p.sw + (int64_t) min(nb, (p.N - 1) / 128) * p.ldsw + kb0;
+            const float *sxr = p.sx + kb0;
+            auto factor = [&](int i0, int j) {  // of block i0 + fe, row 4 j + fr
+                const int e = min(i0 + fe, nk - 1);
+                return __ldg(sxr + (int64_t) min(m0 + 4 * j + fr, p.M - 1) * p.ldsx + e) * __ldg(swr + e);
+            };
+            auto keep = [&](int buf, int j, float f) { piece[buf * 256 + fe * 32 + ((4 * j + fr) ^ (4 * fe))] = f; };
+            float acc[64];
 #pragma unroll
-        for (int c = 0; c < 64; c++) acc[c] = 0.0f;
-        float sc = __ldg(sxr) * __ldg(swr);
-        for (int i = 0; i < nk; i++) {
-            const int a = i % cfg::NACC;
-            const float next = i + 1 < nk ? __ldg(sxr + i + 1) * __ldg(swr + i + 1) : 0.0f;
-            if (!mbar_wait(tfull(a), (i / cfg::NACC) & 1)) {
-                ok = false;
+            for (int e = 0; e < 64; e++) acc[e] = 0.0f;
+            {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = factor(0, j);
+#pragma unroll
+                for (int j = 0; j < 8; j++) keep(0, j, f[j]);
+                __syncwarp();
+            }
+            float f = 0.0f;  // on its way to the next buffer
+            for (int i = 0; i < nk; i++, c++) {
+                const int a = c % NA, e = i & 7, buf = i >> 3 & 1;
+                if (e > 0) keep(buf ^ 1, e - 1, f);
+                f = factor((i & ~7) + 8, e);
+                ok = warp_wait(tfull(a), (c / NA) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const float scale = piece[buf * 256 + e * 32 + (lane ^ (4 * e))];
+#pragma unroll
+                for (int x = 0; x < 64; x += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(taddr + a * cfg::BN + x, r);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) fma2(acc[x + j], acc[x + j + 1], r[j], r[j + 1], scale);
+                }
+                tc_fence_before();
+                if (e == 7) keep(buf ^ 1, 7, f);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty(a));
+            }
+            if (NB == 1) {  // the (partial) tile into the stages (one tile a CTA, its products are in)
+                if (!ok) break;
+#pragma unroll
+                for (int e = 0; e < 64; e += 4)
+                    *reinterpret_cast<float4 *>((float *) smem + (q * 32 + lane) * cfg::PART_LD + half * 64 + e) =
+                        make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
                 break;
             }
-            __syncwarp();
-            tc_fence_after();
+            // 32 x 16 at a time through shared memory, 16-byte units of row r at
+            // unit ^ (r / 2 mod 4) against bank conflicts: bias and activation
+            // on four columns a lane, rows go out in whole pieces
+            const int own = lane * 16, own_x = lane >> 1 & 3, sub = lane / 4, unit = lane % 4;
+            auto put = [&](int x) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(taddr + a * cfg::BN + c, r);
+                for (int u = 0; u < 4; u++)
+                    *reinterpret_cast<float4 *>(piece + own + (u ^ own_x) * 4) =
+                        make_float4(acc[x + 4 * u], acc[x + 4 * u + 1], acc[x + 4 * u + 2], acc[x + 4 * u + 3]);
+                __syncwarp();
+            };
+            auto at = [&](int row) { return reinterpret_cast<float4 *>(piece + row * 16 + (unit ^ (row >> 1 & 3)) * 4); };
+            f8_scale s = {1.0f, 1.0f};
+            float top = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 32; j++) acc[c + j] = fmaf(__uint_as_float(r[j]), sc, acc[c + j]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty(a));
-            sc = next;
-        }
-        ok = epi_all(ok);
-        if (!ok) {
-            if (threadIdx.x == 64) atomicExch(p.err, 1);
-        } else {
-            const int n = n0 + half * 64;
+            for (int x = 0; x < 64; x += 16) {
+                put(x);
+                const int n = n0 + x + unit * 4;
+                float bias[4];
 #pragma unroll
-            for (int c = 0; c < 64; c++)
-                acc[c] = act_fn(acc[c] + (p.bias && n + c < p.N ? __ldg(p.bias + n + c) : 0.0f), p.act);
-            if constexpr (YT == TPMD_DTYPE_F8) {
-                float a = 0.0f;
+                for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
+#pragma unroll 1
+                for (int r = 0; r < 32; r += 8) {
+                    float4 f = *at(r + sub);
+                    f = act4(make_float4(f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]), p.act);
+                    const float v[4] = {f.x, f.y, f.z, f.w};
+                    if constexpr (YT == TPMD_DTYPE_F8)
+                        *at(r + sub) = f;
+                    else if (m0 + r + sub < p.M && n < p.N)
+                        store4<YT>(p, m0 + r + sub, n, v, s);
+                }
+                __syncwarp();
+                if constexpr (YT == TPMD_DTYPE_F8) {  // back to a lane's own row, for its maximum
 #pragma unroll
-                for (int c = 0; c < 64; c++)
-                    if (n + c < p.N) a = fmaxf(a, fabsf(acc[c]));
-                red[half][row] = a;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float s = fmaxf(__fdiv_rn(fmaxf(red[0][row], red[1][row]), F8_MAX), S_MIN);
-                if (m < p.M) {
-                    alignas(16) uint8_t v[64];
+                    for (int u = 0; u < 4; u++) {
+                        const float4 f = *reinterpret_cast<const float4 *>(piece + own + (u ^ own_x) * 4);
+                        acc[x + 4 * u] = f.x;
+                        acc[x + 4 * u + 1] = f.y;
+                        acc[x + 4 * u + 2] = f.z;
+                        acc[x + 4 * u + 3] = f.w;
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
-                        const uint16_t two = __nv_cvt_float2_to_fp8x2(
-                            make_float2(__fdiv_rn(acc[c], s), __fdiv_rn(acc[c + 1], s)), __NV_SATFINITE, __NV_E4M3);
-                        v[c] = (uint8_t) two;
-                        v[c + 1] = (uint8_t) (two >> 8);
+                        for (int e = 0; e < 4; e++)
+                            if (n0 + x + 4 * u + e < p.N) top = fmaxf(top, fabsf(acc[x + 4 * u + e]));
                     }
-                    store_cols((uint8_t *) p.Y + (int64_t) m * p.ldy, v, n, p.N, p.y_vec);
-                    if (half == 0) p.sy[(int64_t) m * p.ldsy + nb] = s;
-                }
-            } else if (m < p.M) {
-                if constexpr (YT == TPMD_DTYPE_F16) {
-                    alignas(16) __half v[64];
-#pragma unroll
-                    for (int c = 0; c < 64; c++) v[c] = __float2half_rn(acc[c]);
-                    store_cols((__half *) p.Y + (int64_t) m * p.ldy, v, n, p.N, p.y_vec);
-                } else {
-                    store_cols((float *) p.Y + (int64_t) m * p.ldy, acc, n, p.N, p.y_vec);
+                    __syncwarp();
                 }
             }
+            if constexpr (YT == TPMD_DTYPE_F8) {
+                // the other half's maximum, by a barrier of the two warps
+                piece[lane] = top;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
+                s = f8_scale_of(fmaxf(top, pieces[((warp - 2) ^ 4) * cfg::PIECE + lane]));
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
+                if (half == 0 && m < p.M && n0 < p.N) p.sy[(int64_t) m * p.ldsy + nb] = s.s;
+#pragma unroll
+                for (int x = 0; x < 64; x += 16) {
+                    put(x);
+#pragma unroll 1
+                    for (int r = 0; r < 32; r += 8) {
+                        const f8_scale sr = {__shfl_sync(0xffffffffu, s.s, r + sub), __shfl_sync(0xffffffffu, s.r, r + sub)};
+                        const float4 f = *at(r + sub);
+                        const float v[4] = {f.x, f.y, f.z, f.w};
+                        if (m0 + r + sub < p.M && n0 + x + unit * 4 < p.N)
+                            store4<YT>(p, m0 + r + sub, n0 + x + unit * 4, v, sr);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) break;
         }
+        if (!ok && lane == 0) atomicExch(p.err, 1);
+    }
+    if (NB == 1) {
+        // each CTA of the cluster adds its share of the rows over all
+        // splits (always in the same order), a warp a row
+        __syncthreads();
+        if (p.splits > 1) cluster_sync();
+        const int n0 = cta % p.tiles_n * 128, m0 = cta / p.tiles_n * cfg::BM, n = n0 + lane * 4;
+        const uint32_t part = smem_u32(smem) + lane * 16;
+        float bias[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
+        // four rows a warp at a time, their loads in flight together
+        constexpr int RB = 4, NW = cfg::THREADS / 32;
+        const int rows = min(cfg::BM, p.M - m0);
+#pragma unroll 1
+        for (int r0 = (split * NW + warp) * RB; r0 < rows; r0 += p.splits * NW * RB) {
+            if (p.splits > 1) {
+                float4 v[RB];
+#pragma unroll
+                for (int j = 0; j < RB; j++) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                for (int k0 = 0; k0 < p.splits; k0 += 2) {
+                    float4 f[2][RB];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        // every CTA starts with its own part: no two read one CTA's at a time
+                        int from = split + k0 + k;
+                        if (from >= p.splits) from -= p.splits;
+#pragma unroll
+                        for (int j = 0; j < RB; j++)
+                            f[k][j] = k0 + k < p.splits ? ld_rank4(part + (r0 + j) * cfg::PART_LD * 4, from)
+                                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int j = 0; j < RB; j++) {
+                            v[j].x += f[k][j].x;
+                            v[j].y += f[k][j].y;
+                            v[j].z += f[k][j].z;
+                            v[j].w += f[k][j].w;
+                        }
+                }
+                // (this CTA's copy of its own rows: nobody else reads it)
+#pragma unroll
+                for (int j = 0; j < RB; j++)
+                    *reinterpret_cast<float4 *>((float *) smem + (r0 + j) * cfg::PART_LD + lane * 4) = v[j];
+            }
+#pragma unroll 1
+            for (int r = r0; r < min(r0 + RB, rows); r++) {
+                const float4 f = *reinterpret_cast<const float4 *>((const float *) smem + r * cfg::PART_LD + lane * 4);
+                const float4 t = act4(make_float4(f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]), p.act);
+                const float y[4] = {t.x, t.y, t.z, t.w};
+                f8_scale s = {1.0f, 1.0f};
+                if constexpr (YT == TPMD_DTYPE_F8) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < p.N) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+                    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    s = f8_scale_of(top);
+                    if (lane == 0) p.sy[(int64_t) (m0 + r) * p.ldsy + n0 / 128] = s.s;
+                }
+                if (n < p.N) store4<YT>(p, m0 + r, n, y, s);
+            }
+        }
+        if (p.splits > 1) cluster_sync();  // no CTA leaves while others read its partial
     }
     tc_fence_before();
     __syncthreads();
@@ -293,9 +470,9 @@ bool encode_bytes(CUtensorMap *tm, const void *base, int64_t cols, int64_t rows,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int YT>
-cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, unsigned tiles,
-                   cudaStream_t st) {
+template <int YT, int NB>
+cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
+    using cfg = f8_cfg<NB>;
     static std::mutex mu;
     static uint64_t attr_set = 0;  // one bit per device
     int dev = 0;
@@ -303,14 +480,30 @@ cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_para
     {
         std::lock_guard<std::mutex> g(mu);
         if (!(attr_set >> (dev & 63) & 1)) {
-            const cudaError_t e = cudaFuncSetAttribute(gemm_f8_kernel<YT>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg::SMEM);
+            const cudaError_t e = cudaFuncSetAttribute(gemm_f8_kernel<YT, NB>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, cfg::SMEM);
             if (e != cudaSuccess) return e;
             attr_set |= 1ull << (dev & 63);
         }
     }
-    gemm_f8_kernel<YT><<<tiles, f8_cfg::THREADS, f8_cfg::SMEM, st>>>(tmX, tmW, p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned) (NB == 1 ? p.tiles * p.splits : std::min(p.tiles, sm_count())), 1, 1);
+    lc.blockDim = dim3(cfg::THREADS, 1, 1);
+    lc.dynamicSmemBytes = cfg::SMEM;
+    lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) p.splits;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    lc.attrs = at;
+    lc.numAttrs = p.splits > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&lc, gemm_f8_kernel<YT, NB>, tmX, tmW, p);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+template <int YT>
+cudaError_t run_f8(int nb, const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
+    return nb == 2 ? run_f8<YT, 2>(tmX, tmW, p, st) : run_f8<YT, 1>(tmX, tmW, p, st);
 }
 
 }  // namespace
@@ -347,7 +540,6 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     p.N = N;
     p.K = K;
     p.kblocks = kblocks;
-    p.tiles_n = (N + 127) / 128;
     p.sx = sx;
     p.sw = sw;
     p.bias = bias;
@@ -359,19 +551,29 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     p.ldsy = ldsy;
     p.act = act;
     const int es = y_dtype == TPMD_DTYPE_F32 ? 4 : y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
-    p.y_vec = !((uintptr_t) Y & 15) && (M == 1 || ldy * es % 16 == 0);
+    p.y_vec = !((uintptr_t) Y & (4 * es - 1)) && (M == 1 || ldy % 4 == 0);
     p.err = tpk_err_word();
-    const int64_t tiles = (int64_t) p.tiles_n * ((M + 127) / 128);
+    const int64_t tiles_m = (M + 127) / 128, nblk = (N + 127) / 128;
+    // 128 x 256 tiles where they fill the SMs; else 128 x 128, their k blocks
+    // shared out over a cluster of up to 8 CTAs while SMs are left and each
+    // keeps two blocks
+    const int nb = tiles_m * ((nblk + 1) / 2) >= sm_count() ? 2 : 1;
+    const int64_t tiles = tiles_m * ((nblk + nb - 1) / nb);
     if (tiles > INT32_MAX) return fail("too many tiles");
+    p.tiles = (int) tiles;
+    p.tiles_n = (int) ((nblk + nb - 1) / nb);
+    const int splits = nb == 2 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>({8, sm_count() / tiles, kblocks / 2}));
+    p.kb_per_split = (kblocks + splits - 1) / splits;
+    p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
     CUtensorMap tmX, tmW;
-    if (!p.err || !encode_bytes(&tmX, X, K, M, ldx, 128) || !encode_bytes(&tmW, W, K, N, ldw, 128)) {
+    if (!p.err || !encode_bytes(&tmX, X, K, M, ldx, 128) || !encode_bytes(&tmW, W, K, N, ldw, 128 * nb)) {
         cudaGetLastError();
         return fail("set-up failed");
     }
     cudaStream_t st = (cudaStream_t) stream;
-    const cudaError_t e = y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(tmX, tmW, p, (unsigned) tiles, st)
-                          : y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(tmX, tmW, p, (unsigned) tiles, st)
-                                                      : run_f8<TPMD_DTYPE_F8>(tmX, tmW, p, (unsigned) tiles, st);
+    const cudaError_t e = y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(nb, tmX, tmW, p, st)
+                          : y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(nb, tmX, tmW, p, st)
+                                                      : run_f8<TPMD_DTYPE_F8>(nb, tmX, tmW, p, st);
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;
 }

@@ -3,23 +3,19 @@
 //   s = max(amax |x| / 448, 2^-126),  q = x / s rounded to e4m3 (nearest even).
 // Byte movers: each element is read once into registers, the block's maximum
 // formed by shuffles (1 x 128: the lanes that hold the block; 128 x 128: the
-// CTA), and written once. Both divisions are IEEE, so the bytes are the ones
-// the definition gives.
+// CTA), and written once.
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <string>
 
 #include "../../include/tpmd.h"
+#include "f8.cuh"
 #include "tpmd_internal.h"
 
 namespace tpmd {
 namespace {
-
-constexpr float F8_MAX = 448.0f;
-constexpr float S_MIN = 1.17549435e-38f;  // 2^-126
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) vec_of {
@@ -40,17 +36,12 @@ __device__ __forceinline__ void load_row(const T *r, int64_t c, int64_t K, float
         for (int e = 0; e < VEC; e++) x[e] = c + e < K ? to_f(r[c + e]) : 0.0f;
     }
 }
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(__fdiv_rn(amax, F8_MAX), S_MIN); }
 template <int VEC, bool ALIGNED>
-__device__ __forceinline__ void store_row(uint8_t *r, int64_t c, int64_t K, float s, const float (&x)[VEC]) {
+__device__ __forceinline__ void store_row(uint8_t *r, int64_t c, int64_t K, f8_scale s, const float (&x)[VEC]) {
     vec_of<uint8_t, VEC> t;
 #pragma unroll
-    for (int e = 0; e < VEC; e += 2) {
-        const uint16_t two = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[e], s), __fdiv_rn(x[e + 1], s)),
-                                                      __NV_SATFINITE, __NV_E4M3);
-        t.v[e] = (uint8_t) two;
-        t.v[e + 1] = (uint8_t) (two >> 8);
-    }
+    for (int e = 0; e < VEC; e += 4)
+        *reinterpret_cast<uint32_t *>(t.v + e) = f8_quant4(x[e], x[e + 1], x[e + 2], x[e + 3], s);
     if (ALIGNED && c + VEC <= K) {
         *reinterpret_cast<vec_of<uint8_t, VEC> *>(r + c) = t;
     } else {
@@ -77,9 +68,9 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x
         const unsigned mask = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
 #pragma unroll
         for (int w = LANES / 2; w > 0; w >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, w));
-        const float sc = block_scale(a);
+        const f8_scale sc = f8_scale_of(a);
         store_row<VEC, ALIGNED>(q + m * ldq, c, K, sc, v);
-        if (lane == 0) s[m * lds + b] = sc;
+        if (lane == 0) s[m * lds + b] = sc.s;
     }
 }
 
@@ -107,11 +98,11 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; w++) a = fmaxf(a, red[w]);
-    const float sc = block_scale(a);
+    const f8_scale sc = f8_scale_of(a);
 #pragma unroll
     for (int i = 0; i < N; i++)
         if (r0 + i * ROWS < M) store_row<VEC, ALIGNED>(q + (r0 + i * ROWS) * ldq, c, K, sc, v[i]);
-    if (threadIdx.x == 0) s[mb * lds + b] = sc;
+    if (threadIdx.x == 0) s[mb * lds + b] = sc.s;
 }
 
 template <typename T, int VEC, bool ALIGNED>

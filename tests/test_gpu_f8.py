@@ -150,7 +150,7 @@ def run_gemm(M, N, K, out, act=0, bias=True, seed=0):
 
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 1024, 1024), (2, 130, 257), (60, 1024, 512), (128, 128, 4096), (129, 129, 129),
           (180, 1024, 1024), (180, 1024, 4096), (180, 4096, 1024), (257, 264, 40), (777, 1000, 528), (1000, 2048, 768),
-          (3000, 640, 1024), (64, 8192, 1024)]
+          (3000, 640, 1024), (64, 8192, 1024), (5000, 1100, 400), (2500, 2050, 256), (19000, 200, 130)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.float16])
@@ -167,7 +167,7 @@ def test_gemm(M, N, K, out):
 
 
 @pytest.mark.parametrize("act", [0, 1, 2, 3])
-@pytest.mark.parametrize("M,N,K", [(180, 1024, 1024), (50, 200, 4096), (700, 3000, 384)])
+@pytest.mark.parametrize("M,N,K", [(180, 1024, 1024), (50, 200, 4096), (700, 3000, 384), (4100, 1300, 140)])
 def test_gemm_activations(M, N, K, act):
     a, Y = run_gemm(M, N, K, torch.float32, act=act)
     y, bound = gemm_ref(*a, act)
@@ -176,7 +176,7 @@ def test_gemm_activations(M, N, K, act):
 
 @pytest.mark.parametrize("act", [0, 2])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 1024, 1024), (180, 4096, 1024), (130, 200, 300), (777, 1000, 528),
-                                   (60, 130, 4096), (3000, 640, 256)])
+                                   (60, 130, 4096), (3000, 640, 256), (5000, 1100, 144)])
 def test_gemm_f8_output_is_the_quantised_f32_output(M, N, K, act):
     (X, sx, W, sw, b), Y = run_gemm(M, N, K, torch.float32, act=act)
     q, raw = padded(M, N, extra=16)
