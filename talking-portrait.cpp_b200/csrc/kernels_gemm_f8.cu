@@ -71,11 +71,15 @@ struct f8_cfg {
     // D f32 (bit 4); A and B e4m3 (0 at bits 7 and 10); K-major both; N >> 3 at bit 17; M >> 4 at bit 24
     static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (BN >> 3) << 17) | ((uint32_t) (BM >> 4) << 24);
     static constexpr int NEPI = 8 * NB, THREADS = 64 + 32 * NEPI;
-    static constexpr int NBARS = 2 * STAGES + 2 * NACC;
-    // a warp's staged 32 x 16 floats; floats a row of a split's partial tile (16-byte bank shifts)
-    static constexpr int PIECE = 32 * 16, PART_LD = 132;
+    static constexpr int FR = 16;  // k blocks of factors kept
+    static constexpr int NBARS = 2 * STAGES + 2 * NACC + FR;
+    // a warp's staged 32 x 8 floats; floats a row of a partial tile (16-byte bank shifts)
+    static constexpr int PIECE = 32 * 8, PART_LD = 132;
     static constexpr int PIECE_BYTES = NEPI * PIECE * 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + PIECE_BYTES + NBARS * 8 + 16;
+    static constexpr int FACTORS = FR * (BM + NB);  // floats: sx of the rows, sw of the blocks
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + PIECE_BYTES + FACTORS * 4 + NBARS * 8 + 16;
+    static_assert(FR >= STAGES + NACC, "factors outlive the products before them");
+    static_assert(FACTORS % 2 == 0, "barrier alignment");
     static_assert(SMEM <= 232448, "shared memory");
     static_assert(BM * PART_LD * 4 <= STAGES * STAGE_BYTES, "a partial tile fits the stages");
 };
@@ -168,7 +172,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
     float *pieces = (float *) (smem + ST * cfg::STAGE_BYTES);
-    uint64_t *bars = (uint64_t *) (smem + ST * cfg::STAGE_BYTES + cfg::PIECE_BYTES);
+    float *fsx = pieces + cfg::PIECE_BYTES / 4, *fsw = fsx + cfg::FR * cfg::BM;  // [FR][BM], [FR][NB]
+    uint64_t *bars = (uint64_t *) (fsx + cfg::FACTORS);
     uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
     auto A = [&](int s) { return smem_u32(smem) + s * cfg::STAGE_BYTES; };
     auto B = [&](int s) { return A(s) + cfg::A_BYTES; };
@@ -176,6 +181,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     auto empty = [&](int s) { return smem_u32(&bars[ST + s]); };
     auto tfull = [&](int a) { return smem_u32(&bars[2 * ST + a]); };
     auto tempty = [&](int a) { return smem_u32(&bars[2 * ST + NA + a]); };
+    auto ffull = [&](int i) { return smem_u32(&bars[2 * ST + 2 * NA + i]); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits, ctas = gridDim.x / p.splits;
@@ -190,6 +196,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             mbar_init(tfull(a), 1);
             mbar_init(tempty(a), cfg::NEPI);
         }
+        for (int i = 0; i < cfg::FR; i++) mbar_init(ffull(i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -206,26 +213,47 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     bool ok = true;
 
     if (warp == 0) {
-        if (lane == 0) {  // TMA producer
-            int c = 0;
-            for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
-                const int n0 = tile % p.tiles_n * cfg::BN, m0 = tile / p.tiles_n * cfg::BM;
-                for (int i = 0; i < nk; i++, c++) {
-                    const int s = c % ST;
-                    if (c >= ST && !mbar_wait(empty(s), ((c / ST) - 1) & 1)) {
-                        ok = false;
-                        break;
-                    }
+        // TMA producer, and the factors of each k block into their ring: four
+        // rows' sx a lane, loaded a block ahead. Block c's slot was last read
+        // for block c - FR, and its stage is free only when the products of
+        // block c - ST are done, which began after block c - ST - NA was read.
+        int c = 0;
+        for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
+            const int n0 = tile % p.tiles_n * cfg::BN, m0 = tile / p.tiles_n * cfg::BM;
+            // (rows and blocks behind the last one have factors of the last one)
+            const float *sx[4], *sw = p.sw + (int64_t) min(n0 / 128 + lane % NB, (p.N - 1) / 128) * p.ldsw + kb0;
+            float x[4], w = __ldg(sw);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                sx[r] = p.sx + (int64_t) min(m0 + lane + 32 * r, p.M - 1) * p.ldsx + kb0;
+                x[r] = __ldg(sx[r]);
+            }
+            for (int i = 0; i < nk; i++, c++) {
+                const int s = c % ST, f = c % cfg::FR;
+                if (c >= ST && !warp_wait(empty(s), ((c / ST) - 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
                     mbar_expect_tx(full(s), cfg::STAGE_BYTES);
                     tma_load_2d(A(s), &tmX, full(s), (kb0 + i) * cfg::KB, m0);
                     tma_load_2d(B(s), &tmW, full(s), (kb0 + i) * cfg::KB, n0);
                 }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    fsx[f * cfg::BM + lane + 32 * r] = x[r];
+                    if (i + 1 < nk) x[r] = __ldg(sx[r] + i + 1);
+                }
+                if (lane < NB) fsw[f * NB + lane] = w;
+                if (i + 1 < nk) w = __ldg(sw + i + 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ffull(f));
             }
-            // the copies in flight land before the CTA goes on
-            for (int j = max(0, c - ST); j < c; j++)
-                if (!mbar_wait(full(j % ST), (j / ST) & 1)) ok = false;
-            if (!ok) atomicExch(p.err, 1);
         }
+        // the copies in flight land before the CTA goes on
+        for (int j = max(0, c - ST); j < c; j++)
+            if (!warp_wait(full(j % ST), (j / ST) & 1)) ok = false;
+        if (!ok && lane == 0) atomicExch(p.err, 1);
     } else if (warp == 1) {
         if (lane == 0) {  // MMA issuer
             int c = 0;
@@ -258,40 +286,16 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
             const int nb = tile % p.tiles_n * NB + blk, n0 = nb * 128 + half * 64, m0 = tile / p.tiles_n * cfg::BM + q * 32;
             const int m = m0 + lane;
-            // the factors sx sw of the warp's 32 rows, eight k blocks at a time,
-            // through the warp's shared memory (two buffers of 8 x 32): a load
-            // takes eight blocks of four rows (whole sectors), the next eight
-            // blocks' loads go out one a step. Row r of block e is at
-            // e * 32 + (r ^ 4 e), free of bank conflicts either way. (Rows and
-            // blocks behind the last one have factors of the last one.)
-            const int fe = lane % 8, fr = lane / 8;
-            const float *swr = p.sw + (int64_t) min(nb, (p.N - 1) / 128) * p.ldsw + kb0;
-            const float *sxr = p.sx + kb0;
-            auto factor = [&](int i0, int j) {  // of block i0 + fe, row 4 j + fr
-                const int e = min(i0 + fe, nk - 1);
-                return __ldg(sxr + (int64_t) min(m0 + 4 * j + fr, p.M - 1) * p.ldsx + e) * __ldg(swr + e);
-            };
-            auto keep = [&](int buf, int j, float f) { piece[buf * 256 + fe * 32 + ((4 * j + fr) ^ (4 * fe))] = f; };
             float acc[64];
 #pragma unroll
             for (int e = 0; e < 64; e++) acc[e] = 0.0f;
-            {
-                float f[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) f[j] = factor(0, j);
-#pragma unroll
-                for (int j = 0; j < 8; j++) keep(0, j, f[j]);
-                __syncwarp();
-            }
-            float f = 0.0f;  // on its way to the next buffer
             for (int i = 0; i < nk; i++, c++) {
-                const int a = c % NA, e = i & 7, buf = i >> 3 & 1;
-                if (e > 0) keep(buf ^ 1, e - 1, f);
-                f = factor((i & ~7) + 8, e);
-                ok = warp_wait(tfull(a), (c / NA) & 1);
+                const int a = c % NA, f = c % cfg::FR;
+                ok = warp_wait(ffull(f), (c / cfg::FR) & 1);
+                const float scale = fsx[f * cfg::BM + q * 32 + lane] * fsw[f * NB + blk];
+                ok = warp_wait(tfull(a), (c / NA) & 1) && ok;
                 if (!ok) break;
                 tc_fence_after();
-                const float scale = piece[buf * 256 + e * 32 + (lane ^ (4 * e))];
 #pragma unroll
                 for (int x = 0; x < 64; x += 16) {
                     uint32_t r[16];
@@ -300,7 +304,6 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     for (int j = 0; j < 16; j += 2) fma2(acc[x + j], acc[x + j + 1], r[j], r[j + 1], scale);
                 }
                 tc_fence_before();
-                if (e == 7) keep(buf ^ 1, 7, f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty(a));
             }
@@ -312,29 +315,29 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                         make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
                 break;
             }
-            // 32 x 16 at a time through shared memory, 16-byte units of row r at
-            // unit ^ (r / 2 mod 4) against bank conflicts: bias and activation
+            // 32 x 8 at a time through shared memory, 16-byte units of row r at
+            // unit ^ (r / 4 mod 2) against bank conflicts: bias and activation
             // on four columns a lane, rows go out in whole pieces
-            const int own = lane * 16, own_x = lane >> 1 & 3, sub = lane / 4, unit = lane % 4;
+            const int own = lane * 8, own_x = lane >> 2 & 1, sub = lane / 2, unit = lane % 2;
             auto put = [&](int x) {
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+                for (int u = 0; u < 2; u++)
                     *reinterpret_cast<float4 *>(piece + own + (u ^ own_x) * 4) =
                         make_float4(acc[x + 4 * u], acc[x + 4 * u + 1], acc[x + 4 * u + 2], acc[x + 4 * u + 3]);
                 __syncwarp();
             };
-            auto at = [&](int row) { return reinterpret_cast<float4 *>(piece + row * 16 + (unit ^ (row >> 1 & 3)) * 4); };
+            auto at = [&](int row) { return reinterpret_cast<float4 *>(piece + row * 8 + (unit ^ (row >> 2 & 1)) * 4); };
             f8_scale s = {1.0f, 1.0f};
             float top = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 64; x += 16) {
+            for (int x = 0; x < 64; x += 8) {
                 put(x);
                 const int n = n0 + x + unit * 4;
                 float bias[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
 #pragma unroll 1
-                for (int r = 0; r < 32; r += 8) {
+                for (int r = 0; r < 32; r += 16) {
                     float4 f = *at(r + sub);
                     f = act4(make_float4(f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]), p.act);
                     const float v[4] = {f.x, f.y, f.z, f.w};
@@ -346,7 +349,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 __syncwarp();
                 if constexpr (YT == TPMD_DTYPE_F8) {  // back to a lane's own row, for its maximum
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
+                    for (int u = 0; u < 2; u++) {
                         const float4 f = *reinterpret_cast<const float4 *>(piece + own + (u ^ own_x) * 4);
                         acc[x + 4 * u] = f.x;
                         acc[x + 4 * u + 1] = f.y;
@@ -367,10 +370,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
                 if (half == 0 && m < p.M && n0 < p.N) p.sy[(int64_t) m * p.ldsy + nb] = s.s;
 #pragma unroll
-                for (int x = 0; x < 64; x += 16) {
+                for (int x = 0; x < 64; x += 8) {
                     put(x);
 #pragma unroll 1
-                    for (int r = 0; r < 32; r += 8) {
+                    for (int r = 0; r < 32; r += 16) {
                         const f8_scale sr = {__shfl_sync(0xffffffffu, s.s, r + sub), __shfl_sync(0xffffffffu, s.r, r + sub)};
                         const float4 f = *at(r + sub);
                         const float v[4] = {f.x, f.y, f.z, f.w};
