@@ -4,17 +4,19 @@
 //   Y[m][n] = act( sum_b sx[m][b] sw[n/128][b] P_b[m][n] + bias[n] ),
 //   P_b[m][n] = sum_{k in block b} X[m][k] W[n][k],  blocks of 128 along k
 //
-// An output tile is 128 x 128 or 128 x 256: 128 rows of X are the MMA's M
-// side (TMEM lanes), one or two blocks of 128 rows of W its N side, so a
-// block's W scale of one k block is one number and a lane's factor sx sw is
-// one number for all its 128 columns. Each k block of 128 is one pipeline stage (one
+// An output tile is 128 x 128, or 256 x 256 of a pair of CTAs (cta_group::2:
+// each loads 128 rows of X and 128 of W a k block, half of what it
+// multiplies; a tile of its own would need more from L2 than the SMs get).
+// Rows of X are the MMA's M side (TMEM lanes), blocks of 128 rows of W its N
+// side, so a block's W scale of one k block is one number and a lane's
+// factor sx sw is one number for all its 128 columns. Each k block of 128 is one pipeline stage (one
 // 128-byte swizzled row a matrix row) and one MMA group into an accumulator
 // of its own out of a ring in TMEM; the epilogue warps (each a lane quarter
 // and 64 columns) read it, scale it and add it to f32 registers while the
 // next blocks multiply. The products of e4m3 values are exact in
 // f32; sums are f32 throughout.
 //
-// With 128 x 256 tiles (products that fill the SMs) CTAs are persistent: the
+// With 256 x 256 tiles (products that fill the SMs) CTAs are persistent: the
 // loads and products of the next tile run on while a tile is written. With
 // 128 x 128 tiles a CTA has one, and where SMs are left the k blocks of a
 // tile are shared out over a cluster of up to eight CTAs; each leaves its
@@ -38,14 +40,78 @@
 namespace tpmd {
 namespace {
 
+// NB = 2: of a pair of CTAs, issued by its first one
+template <int NB>
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
     const uint32_t mask = 0;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(mask));
+    if constexpr (NB == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(mask));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(mask));
+}
+// arrival on `bar` (NB = 2: of both CTAs) once the MMAs issued so far are done
+template <int NB>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (NB == 1)
+        umma_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t) 3)
+            : "memory");
+}
+__device__ __forceinline__ uint32_t first_cta(uint32_t saddr) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(saddr));
+    return a;
+}
+// a 128 x 128 tile; NB = 2: its bytes count on the first CTA's barrier
+template <int NB>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int c0, int c1) {
+    if constexpr (NB == 1)
+        tma_load_2d(dst, tm, bar, c0, c1);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"((uint64_t) tm), "r"(first_cta(bar)), "r"(c0), "r"(c1)
+            : "memory");
+}
+// arrival on the first CTA's barrier, after reads of TMEM that a wait has
+// ended: nothing in memory to publish, so no cluster-scope release (its memory
+// barrier took over half of the warps' time here)
+template <int NB>
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+    if constexpr (NB == 1)
+        mbar_arrive(bar);
+    else
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first_cta(bar)) : "memory");
+}
+template <int NB>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+    if constexpr (NB == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int NB>
+__device__ __forceinline__ void tmem_dealloc(uint32_t tmem, uint32_t cols) {
+    if constexpr (NB == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
 __device__ __forceinline__ float act_one(float v, int act) {
@@ -64,12 +130,14 @@ __device__ __forceinline__ float4 act4(float4 v, int act) { return act == 0 ? v 
 // NB: blocks of 128 columns a tile
 template <int NB>
 struct f8_cfg {
+    // rows of a CTA; CTAs a tile (NB of them share an MMA: each holds 128 rows
+    // of X and 128 of W, and the accumulators of its rows for all columns)
     static constexpr int BM = 128, BN = 128 * NB, KB = 128;
-    static constexpr int A_BYTES = BM * KB, B_BYTES = BN * KB, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = NB == 2 ? 4 : 6, NACC = 4 / NB;
+    static constexpr int A_BYTES = BM * KB, B_BYTES = 128 * KB, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 6, NACC = 4 / NB;
     static constexpr uint32_t TMEM_COLS = 512;
     // D f32 (bit 4); A and B e4m3 (0 at bits 7 and 10); K-major both; N >> 3 at bit 17; M >> 4 at bit 24
-    static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (BN >> 3) << 17) | ((uint32_t) (BM >> 4) << 24);
+    static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (BN >> 3) << 17) | ((uint32_t) (BM * NB >> 4) << 24);
     static constexpr int NEPI = 8 * NB, THREADS = 64 + 32 * NEPI;
     static constexpr int FR = 16;  // k blocks of factors kept
     static constexpr int NBARS = 2 * STAGES + 2 * NACC + FR;
@@ -184,7 +252,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     auto ffull = [&](int i) { return smem_u32(&bars[2 * ST + 2 * NA + i]); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits, ctas = gridDim.x / p.splits;
+    const int rank = NB == 2 ? blockIdx.x % 2 : 0;  // of the CTA pair (its even CTA issues the MMAs)
+    const int split = NB == 1 ? blockIdx.x % p.splits : 0;
+    const int cta = NB == 1 ? blockIdx.x / p.splits : blockIdx.x / 2, ctas = NB == 1 ? gridDim.x / p.splits : gridDim.x / 2;
     const int kb0 = split * p.kb_per_split, nk = min(p.kblocks - kb0, p.kb_per_split);  // nk >= 1 (host)
 
     if (threadIdx.x == 0) {
@@ -194,68 +264,80 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         }
         for (int a = 0; a < NA; a++) {
             mbar_init(tfull(a), 1);
-            mbar_init(tempty(a), cfg::NEPI);
+            mbar_init(tempty(a), cfg::NEPI * NB);
         }
         for (int i = 0; i < cfg::FR; i++) mbar_init(ffull(i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(cfg::TMEM_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<NB>(smem_u32(tmem_slot), cfg::TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    if (NB == 2) cluster_sync();  // the pair's barriers are set up
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
 
     if (warp == 0) {
         // TMA producer, and the factors of each k block into their ring: four
-        // rows' sx a lane, loaded a block ahead. Block c's slot was last read
+        // rows' sx a lane, loaded four blocks ahead. Block c's slot was last read
         // for block c - FR, and its stage is free only when the products of
         // block c - ST are done, which began after block c - ST - NA was read.
         int c = 0;
         for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
-            const int n0 = tile % p.tiles_n * cfg::BN, m0 = tile / p.tiles_n * cfg::BM;
+            const int n0 = tile % p.tiles_n * cfg::BN, m0 = (tile / p.tiles_n * NB + rank) * cfg::BM;
             // (rows and blocks behind the last one have factors of the last one)
             const float *sx[4], *sw = p.sw + (int64_t) min(n0 / 128 + lane % NB, (p.N - 1) / 128) * p.ldsw + kb0;
-            float x[4], w = __ldg(sw);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                sx[r] = p.sx + (int64_t) min(m0 + lane + 32 * r, p.M - 1) * p.ldsx + kb0;
-                x[r] = __ldg(sx[r]);
-            }
-            for (int i = 0; i < nk; i++, c++) {
-                const int s = c % ST, f = c % cfg::FR;
-                if (c >= ST && !warp_wait(empty(s), ((c / ST) - 1) & 1)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) {
-                    mbar_expect_tx(full(s), cfg::STAGE_BYTES);
-                    tma_load_2d(A(s), &tmX, full(s), (kb0 + i) * cfg::KB, m0);
-                    tma_load_2d(B(s), &tmW, full(s), (kb0 + i) * cfg::KB, n0);
-                }
+            for (int r = 0; r < 4; r++) sx[r] = p.sx + (int64_t) min(m0 + lane + 32 * r, p.M - 1) * p.ldsx + kb0;
+            float x[4][4], w[4], nx[4][4], nw[4];  // of four blocks, and of the four after them
+            auto fetch = [&](int i0) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    fsx[f * cfg::BM + lane + 32 * r] = x[r];
-                    if (i + 1 < nk) x[r] = __ldg(sx[r] + i + 1);
+                for (int e = 0; e < 4; e++) {
+                    const int i = min(i0 + e, nk - 1);
+                    nw[e] = __ldg(sw + i);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) nx[e][r] = __ldg(sx[r] + i);
                 }
-                if (lane < NB) fsw[f * NB + lane] = w;
-                if (i + 1 < nk) w = __ldg(sw + i + 1);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ffull(f));
+            };
+            fetch(0);
+            for (int i0 = 0; ok && i0 < nk; i0 += 4) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    w[e] = nw[e];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[e][r] = nx[e][r];
+                }
+                if (i0 + 4 < nk) fetch(i0 + 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (i0 + e >= nk) break;
+                    const int s = c % ST, f = c % cfg::FR;
+                    if (c >= ST && !warp_wait(empty(s), ((c / ST) - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        // the bytes of both CTAs of a pair count on its first one's barrier
+                        if (rank == 0) mbar_expect_tx(full(s), cfg::STAGE_BYTES * NB);
+                        load_tile<NB>(A(s), &tmX, full(s), (kb0 + i0 + e) * cfg::KB, m0);
+                        load_tile<NB>(B(s), &tmW, full(s), (kb0 + i0 + e) * cfg::KB, n0 + rank * 128);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; r++) fsx[f * cfg::BM + lane + 32 * r] = x[e][r];
+                    if (lane < NB) fsw[f * NB + lane] = w[e];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ffull(f));
+                    c++;
+                }
             }
         }
-        // the copies in flight land before the CTA goes on
+        // the copies in flight land (and are read) before the CTA goes on
         for (int j = max(0, c - ST); j < c; j++)
-            if (!warp_wait(full(j % ST), (j / ST) & 1)) ok = false;
+            if (!warp_wait(empty(j % ST), (j / ST) & 1)) ok = false;
         if (!ok && lane == 0) atomicExch(p.err, 1);
     } else if (warp == 1) {
-        if (lane == 0) {  // MMA issuer
+        if (lane == 0 && rank == 0) {  // MMA issuer
             int c = 0;
             for (int tile = cta; ok && tile < p.tiles; tile += ctas)
                 for (int i = 0; i < nk; i++, c++) {
@@ -267,10 +349,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < cfg::KB / 32; kk++)
-                        umma_f8(tmem + a * cfg::BN, smem_desc(A(s) + kk * 32, 1024, 2),
-                                smem_desc(B(s) + kk * 32, 1024, 2), cfg::IDESC, kk > 0);
-                    umma_commit(empty(s));
-                    umma_commit(tfull(a));
+                        umma_f8<NB>(tmem + a * cfg::BN, smem_desc(A(s) + kk * 32, 1024, 2),
+                                    smem_desc(B(s) + kk * 32, 1024, 2), cfg::IDESC, kk > 0);
+                    commit<NB>(empty(s));
+                    commit<NB>(tfull(a));
                 }
             // the MMAs in flight end before TMEM is freed
             for (int j = max(0, c - NA); j < c; j++)
@@ -284,7 +366,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         float *piece = pieces + (warp - 2) * cfg::PIECE;
         int c = 0;
         for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
-            const int nb = tile % p.tiles_n * NB + blk, n0 = nb * 128 + half * 64, m0 = tile / p.tiles_n * cfg::BM + q * 32;
+            const int nb = tile % p.tiles_n * NB + blk, n0 = nb * 128 + half * 64;
+            const int m0 = (tile / p.tiles_n * NB + rank) * cfg::BM + q * 32;
             const int m = m0 + lane;
             float acc[64];
 #pragma unroll
@@ -305,7 +388,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tempty(a));
+                if (lane == 0) arrive_first<NB>(tempty(a));
             }
             if (NB == 1) {  // the (partial) tile into the stages (one tile a CTA, its products are in)
                 if (!ok) break;
@@ -457,9 +540,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cfg::TMEM_COLS)
-                     : "memory");
+    if (NB == 2) cluster_sync();  // no CTA leaves while its pair uses its memory
+    if (warp == 1) tmem_dealloc<NB>(tmem, cfg::TMEM_COLS);
 }
 
 bool encode_bytes(CUtensorMap *tm, const void *base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
@@ -490,17 +572,17 @@ cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_para
         }
     }
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned) (NB == 1 ? p.tiles * p.splits : std::min(p.tiles, sm_count())), 1, 1);
+    lc.gridDim = dim3((unsigned) (NB == 1 ? p.tiles * p.splits : 2 * std::min(p.tiles, sm_count() / 2)), 1, 1);
     lc.blockDim = dim3(cfg::THREADS, 1, 1);
     lc.dynamicSmemBytes = cfg::SMEM;
     lc.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned) p.splits;
+    at[0].val.clusterDim.x = (unsigned) (NB == 1 ? p.splits : 2);
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     lc.attrs = at;
-    lc.numAttrs = p.splits > 1 ? 1 : 0;
+    lc.numAttrs = NB == 2 || p.splits > 1 ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&lc, gemm_f8_kernel<YT, NB>, tmX, tmW, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -556,12 +638,12 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     const int es = y_dtype == TPMD_DTYPE_F32 ? 4 : y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
     p.y_vec = !((uintptr_t) Y & (4 * es - 1)) && (M == 1 || ldy % 4 == 0);
     p.err = tpk_err_word();
-    const int64_t tiles_m = (M + 127) / 128, nblk = (N + 127) / 128;
-    // 128 x 256 tiles where they fill the SMs; else 128 x 128, their k blocks
-    // shared out over a cluster of up to 8 CTAs while SMs are left and each
-    // keeps two blocks
-    const int nb = tiles_m * ((nblk + 1) / 2) >= sm_count() ? 2 : 1;
-    const int64_t tiles = tiles_m * ((nblk + nb - 1) / nb);
+    const int64_t nblk = (N + 127) / 128;
+    // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128,
+    // their k blocks shared out over a cluster of up to 8 CTAs while SMs are
+    // left and each keeps two blocks
+    const int nb = (M + 255) / 256 * ((nblk + 1) / 2) >= sm_count() / 2 ? 2 : 1;
+    const int64_t tiles = (M + nb * 128 - 1) / (nb * 128) * ((nblk + nb - 1) / nb);
     if (tiles > INT32_MAX) return fail("too many tiles");
     p.tiles = (int) tiles;
     p.tiles_n = (int) ((nblk + nb - 1) / nb);
@@ -569,7 +651,7 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     p.kb_per_split = (kblocks + splits - 1) / splits;
     p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
     CUtensorMap tmX, tmW;
-    if (!p.err || !encode_bytes(&tmX, X, K, M, ldx, 128) || !encode_bytes(&tmW, W, K, N, ldw, 128 * nb)) {
+    if (!p.err || !encode_bytes(&tmX, X, K, M, ldx, 128) || !encode_bytes(&tmW, W, K, N, ldw, 128)) {
         cudaGetLastError();
         return fail("set-up failed");
     }
