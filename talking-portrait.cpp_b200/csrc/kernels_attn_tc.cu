@@ -109,10 +109,6 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float *f) {
 #pragma unroll
     for (int i = 0; i < 32; i++) f[i] = __uint_as_float(r[i]);
 }
-// a bounded wait of a whole warp, one answer for all lanes
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

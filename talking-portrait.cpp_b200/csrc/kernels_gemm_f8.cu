@@ -12,7 +12,7 @@
 // factor sx sw is one number for all its 128 columns. Each k block of 128 is one pipeline stage (one
 // 128-byte swizzled row a matrix row) and one MMA group into an accumulator
 // of its own out of a ring in TMEM; the epilogue warps (each a lane quarter
-// and 64 columns) read it, scale it and add it to f32 registers while the
+// and half of the columns) read it, scale it and add it to f32 registers while the
 // next blocks multiply. The products of e4m3 values are exact in
 // f32; sums are f32 throughout.
 //
@@ -134,16 +134,17 @@ struct f8_cfg {
     // of X and 128 of W, and the accumulators of its rows for all columns)
     static constexpr int BM = 128, BN = 128 * NB, KB = 128;
     static constexpr int A_BYTES = BM * KB, B_BYTES = 128 * KB, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 6, NACC = 4 / NB;
+    static constexpr int STAGES = NB == 2 ? 5 : 6, NACC = 4 / NB;
     static constexpr uint32_t TMEM_COLS = 512;
     // D f32 (bit 4); A and B e4m3 (0 at bits 7 and 10); K-major both; N >> 3 at bit 17; M >> 4 at bit 24
     static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (BN >> 3) << 17) | ((uint32_t) (BM * NB >> 4) << 24);
-    static constexpr int NEPI = 8 * NB, THREADS = 64 + 32 * NEPI;
+    static constexpr int CW = 64 * NB;  // columns an epilogue warp
+    static constexpr int NEPI = 8, THREADS = 64 + 32 * NEPI;
     static constexpr int FR = 16;  // k blocks of factors kept
     static constexpr int NBARS = 2 * STAGES + 2 * NACC + FR;
-    // a warp's staged 32 x 8 floats; floats a row of a partial tile (16-byte bank shifts)
-    static constexpr int PIECE = 32 * 8, PART_LD = 132;
-    static constexpr int PIECE_BYTES = NEPI * PIECE * 4;
+    // NB = 2: a warp's staged 32 rows of 64 bytes; NB = 1: floats a row of a partial tile (16-byte bank shifts)
+    static constexpr int PIECE = NB == 2 ? 32 * 64 : 0, PART_LD = 132;
+    static constexpr int PIECE_BYTES = NEPI * PIECE;
     static constexpr int FACTORS = FR * (BM + NB);  // floats: sx of the rows, sw of the blocks
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + PIECE_BYTES + FACTORS * 4 + NBARS * 8 + 16;
     static_assert(FR >= STAGES + NACC, "factors outlive the products before them");
@@ -161,7 +162,7 @@ struct f8_params {
     float *sy;
     int64_t ldsy;
     int act;
-    bool y_vec;  // Y takes stores of four elements
+    bool y_vec;  // Y takes stores of four elements (NB = 2: of 16 bytes)
     int *err;
 };
 
@@ -176,9 +177,6 @@ __device__ __forceinline__ void fma2(float &a0, float &a1, uint32_t x0, uint32_t
         : "+f"(a0), "+f"(a1)
         : "r"(x0), "r"(x1), "f"(s));
 }
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
@@ -191,6 +189,15 @@ __device__ __forceinline__ float4 ld_rank4(uint32_t saddr, uint32_t rank) {
                  : "r"(a)
                  : "memory");
     return v;
+}
+// n elements of ES bytes, where rows start off 16-byte boundaries or end
+template <int ES>
+__device__ __noinline__ void copy_elements(uint8_t *y, const uint8_t *x, int n) {
+    for (int i = 0; i < n; i++) {
+        if (ES == 4) reinterpret_cast<uint32_t *>(y)[i] = reinterpret_cast<const uint32_t *>(x)[i];
+        else if (ES == 2) reinterpret_cast<uint16_t *>(y)[i] = reinterpret_cast<const uint16_t *>(x)[i];
+        else y[i] = x[i];
+    }
 }
 // four values of a row to Y columns n .. n + 3 (F8: quantised by s)
 template <int YT>
@@ -239,8 +246,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     constexpr int ST = cfg::STAGES, NA = cfg::NACC;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    float *pieces = (float *) (smem + ST * cfg::STAGE_BYTES);
-    float *fsx = pieces + cfg::PIECE_BYTES / 4, *fsw = fsx + cfg::FR * cfg::BM;  // [FR][BM], [FR][NB]
+    uint8_t *pieces = smem + ST * cfg::STAGE_BYTES;
+    float *fsx = (float *) (pieces + cfg::PIECE_BYTES), *fsw = fsx + cfg::FR * cfg::BM;  // [FR][BM], [FR][NB]
     uint64_t *bars = (uint64_t *) (fsx + cfg::FACTORS);
     uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
     auto A = [&](int s) { return smem_u32(smem) + s * cfg::STAGE_BYTES; };
@@ -251,7 +258,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     auto tempty = [&](int a) { return smem_u32(&bars[2 * ST + NA + a]); };
     auto ffull = [&](int i) { return smem_u32(&bars[2 * ST + 2 * NA + i]); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = NB == 2 ? blockIdx.x % 2 : 0;  // of the CTA pair (its even CTA issues the MMAs)
     const int split = NB == 1 ? blockIdx.x % p.splits : 0;
     const int cta = NB == 1 ? blockIdx.x / p.splits : blockIdx.x / 2, ctas = NB == 1 ? gridDim.x / p.splits : gridDim.x / 2;
@@ -337,41 +344,46 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             if (!warp_wait(empty(j % ST), (j / ST) & 1)) ok = false;
         if (!ok && lane == 0) atomicExch(p.err, 1);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {  // MMA issuer
+        if (rank == 0) {
+            // MMA issuer: the whole warp goes through the loop, so that what it
+            // computes stays in uniform registers, and one lane issues (a loop of
+            // one lane alone took longer to issue the MMAs than they run)
             int c = 0;
             for (int tile = cta; ok && tile < p.tiles; tile += ctas)
                 for (int i = 0; i < nk; i++, c++) {
                     const int s = c % ST, a = c % NA;
-                    if (!mbar_wait(full(s), (c / ST) & 1) || (c >= NA && !mbar_wait(tempty(a), ((c / NA) - 1) & 1))) {
-                        ok = false;
-                        break;
-                    }
+                    ok = warp_wait(full(s), (c / ST) & 1) && (c < NA || warp_wait(tempty(a), ((c / NA) - 1) & 1));
+                    if (!ok) break;
                     tc_fence_after();
+                    const uint64_t ad = smem_desc(A(s), 1024, 2), bd = smem_desc(B(s), 1024, 2);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < cfg::KB / 32; kk++)
-                        umma_f8<NB>(tmem + a * cfg::BN, smem_desc(A(s) + kk * 32, 1024, 2),
-                                    smem_desc(B(s) + kk * 32, 1024, 2), cfg::IDESC, kk > 0);
-                    commit<NB>(empty(s));
-                    commit<NB>(tfull(a));
+                        for (int kk = 0; kk < cfg::KB / 32; kk++)
+                            umma_f8<NB>(tmem + a * cfg::BN, ad + kk * 2, bd + kk * 2, cfg::IDESC, kk > 0);
+                        commit<NB>(tfull(a));
+                        commit<NB>(empty(s));
+                    }
+                    __syncwarp();
                 }
             // the MMAs in flight end before TMEM is freed
             for (int j = max(0, c - NA); j < c; j++)
-                if (!mbar_wait(tfull(j % NA), (j / NA) & 1)) ok = false;
-            if (!ok) atomicExch(p.err, 1);
+                if (!warp_wait(tfull(j % NA), (j / NA) & 1)) ok = false;
+            if (!ok && lane == 0) atomicExch(p.err, 1);
         }
     } else {
-        // a warp: a lane quarter (32 rows) and half of a block of 128 columns
-        const int q = warp & 3, blk = (warp - 2) >> 3, half = (warp - 2) >> 2 & 1, pair = blk * 4 + q;
-        const uint32_t taddr = tmem + ((uint32_t) (q * 32) << 16) + blk * 128 + half * 64;
-        float *piece = pieces + (warp - 2) * cfg::PIECE;
+        // a warp: a lane quarter (32 rows) and half of the columns (half a block
+        // of 128, or one of two)
+        constexpr int CW = cfg::CW;
+        const int q = warp & 3, half = (warp - 2) >> 2, blk = half * CW / 128;
+        const uint32_t taddr = tmem + ((uint32_t) (q * 32) << 16) + half * CW;
+        uint8_t *piece = pieces + (warp - 2) * cfg::PIECE;
         int c = 0;
         for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
-            const int nb = tile % p.tiles_n * NB + blk, n0 = nb * 128 + half * 64;
+            const int n0 = tile % p.tiles_n * cfg::BN + half * CW, nb = n0 / 128;
             const int m0 = (tile / p.tiles_n * NB + rank) * cfg::BM + q * 32;
-            const int m = m0 + lane;
-            float acc[64];
+            float acc[CW];
 #pragma unroll
-            for (int e = 0; e < 64; e++) acc[e] = 0.0f;
+            for (int e = 0; e < CW; e++) acc[e] = 0.0f;
             for (int i = 0; i < nk; i++, c++) {
                 const int a = c % NA, f = c % cfg::FR;
                 ok = warp_wait(ffull(f), (c / cfg::FR) & 1);
@@ -380,11 +392,11 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
-                for (int x = 0; x < 64; x += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(taddr + a * cfg::BN + x, r);
+                for (int x = 0; x < CW; x += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(taddr + a * cfg::BN + x, r);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) fma2(acc[x + j], acc[x + j + 1], r[j], r[j + 1], scale);
+                    for (int j = 0; j < 32; j += 2) fma2(acc[x + j], acc[x + j + 1], r[j], r[j + 1], scale);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -393,80 +405,75 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             if (NB == 1) {  // the (partial) tile into the stages (one tile a CTA, its products are in)
                 if (!ok) break;
 #pragma unroll
-                for (int e = 0; e < 64; e += 4)
-                    *reinterpret_cast<float4 *>((float *) smem + (q * 32 + lane) * cfg::PART_LD + half * 64 + e) =
+                for (int e = 0; e < CW; e += 4)
+                    *reinterpret_cast<float4 *>((float *) smem + (q * 32 + lane) * cfg::PART_LD + half * CW + e) =
                         make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
                 break;
             }
-            // 32 x 8 at a time through shared memory, 16-byte units of row r at
-            // unit ^ (r / 4 mod 2) against bank conflicts: bias and activation
-            // on four columns a lane, rows go out in whole pieces
-            const int own = lane * 8, own_x = lane >> 2 & 1, sub = lane / 2, unit = lane % 2;
-            auto put = [&](int x) {
+            if constexpr (NB == 2) {
+                if (!ok) break;
+                // bias and activation in place (the same columns in every lane)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-                    *reinterpret_cast<float4 *>(piece + own + (u ^ own_x) * 4) =
-                        make_float4(acc[x + 4 * u], acc[x + 4 * u + 1], acc[x + 4 * u + 2], acc[x + 4 * u + 3]);
-                __syncwarp();
-            };
-            auto at = [&](int row) { return reinterpret_cast<float4 *>(piece + row * 8 + (unit ^ (row >> 2 & 1)) * 4); };
-            f8_scale s = {1.0f, 1.0f};
-            float top = 0.0f;
+                for (int e = 0; e < CW; e += 4) {
+                    float bias[4];
 #pragma unroll
-            for (int x = 0; x < 64; x += 8) {
-                put(x);
-                const int n = n0 + x + unit * 4;
-                float bias[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
-#pragma unroll 1
-                for (int r = 0; r < 32; r += 16) {
-                    float4 f = *at(r + sub);
-                    f = act4(make_float4(f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]), p.act);
-                    const float v[4] = {f.x, f.y, f.z, f.w};
-                    if constexpr (YT == TPMD_DTYPE_F8)
-                        *at(r + sub) = f;
-                    else if (m0 + r + sub < p.M && n < p.N)
-                        store4<YT>(p, m0 + r + sub, n, v, s);
+                    for (int j = 0; j < 4; j++) bias[j] = p.bias ? __ldg(p.bias + min(n0 + e + j, p.N - 1)) : 0.0f;
+                    const float4 f = act4(make_float4(acc[e] + bias[0], acc[e + 1] + bias[1], acc[e + 2] + bias[2],
+                                                      acc[e + 3] + bias[3]),
+                                          p.act);
+                    acc[e] = f.x;
+                    acc[e + 1] = f.y;
+                    acc[e + 2] = f.z;
+                    acc[e + 3] = f.w;
                 }
-                __syncwarp();
-                if constexpr (YT == TPMD_DTYPE_F8) {  // back to a lane's own row, for its maximum
+                f8_scale k = {1.0f, 1.0f};
+                if constexpr (YT == TPMD_DTYPE_F8) {
+                    float top = 0.0f;
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const float4 f = *reinterpret_cast<const float4 *>(piece + own + (u ^ own_x) * 4);
-                        acc[x + 4 * u] = f.x;
-                        acc[x + 4 * u + 1] = f.y;
-                        acc[x + 4 * u + 2] = f.z;
-                        acc[x + 4 * u + 3] = f.w;
+                    for (int e = 0; e < CW; e++)
+                        if (n0 + e < p.N) top = fmaxf(top, fabsf(acc[e]));
+                    k = f8_scale_of(top);
+                    if (m0 + lane < p.M && n0 < p.N) p.sy[(int64_t) (m0 + lane) * p.ldsy + nb] = k.s;
+                }
+                // 64 bytes of each row at a time through shared memory, 16-byte
+                // unit u of row r at u ^ (r / 2 mod 4) against bank conflicts:
+                // a store covers eight rows
+                constexpr int ES = YT == TPMD_DTYPE_F32 ? 4 : YT == TPMD_DTYPE_F16 ? 2 : 1, PER = 16 / ES;
+                const int sub = lane / 4, unit = lane % 4;
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (n0 + x + 4 * u + e < p.N) top = fmaxf(top, fabsf(acc[x + 4 * u + e]));
+                for (int x = 0; x < CW; x += 4 * PER) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        uint4 w;
+                        const float *v = acc + x + u * PER;
+                        if constexpr (YT == TPMD_DTYPE_F32) {
+                            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                           __float_as_uint(v[3]));
+                        } else if constexpr (YT == TPMD_DTYPE_F16) {
+                            const __half2 h[4] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3]),
+                                                  __floats2half2_rn(v[4], v[5]), __floats2half2_rn(v[6], v[7])};
+                            w = *reinterpret_cast<const uint4 *>(h);
+                        } else {
+                            w = make_uint4(f8_quant4(v[0], v[1], v[2], v[3], k), f8_quant4(v[4], v[5], v[6], v[7], k),
+                                           f8_quant4(v[8], v[9], v[10], v[11], k),
+                                           f8_quant4(v[12], v[13], v[14], v[15], k));
+                        }
+                        *reinterpret_cast<uint4 *>(piece + lane * 64 + (u ^ (lane >> 1 & 3)) * 16) = w;
+                    }
+                    __syncwarp();
+                    const int n = n0 + x + unit * PER;
+#pragma unroll
+                    for (int r = 0; r < 32; r += 8) {
+                        const int row = r + sub;
+                        const uint4 *src = reinterpret_cast<const uint4 *>(piece + row * 64 + (unit ^ (row >> 1 & 3)) * 16);
+                        uint8_t *y = (uint8_t *) p.Y + ((int64_t) (m0 + row) * p.ldy + n) * ES;
+                        if (m0 + row >= p.M || n >= p.N) continue;
+                        if (p.y_vec && n + PER <= p.N) *reinterpret_cast<uint4 *>(y) = *src;
+                        else copy_elements<ES>(y, reinterpret_cast<const uint8_t *>(src), min(PER, p.N - n));
                     }
                     __syncwarp();
                 }
             }
-            if constexpr (YT == TPMD_DTYPE_F8) {
-                // the other half's maximum, by a barrier of the two warps
-                piece[lane] = top;
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
-                s = f8_scale_of(fmaxf(top, pieces[((warp - 2) ^ 4) * cfg::PIECE + lane]));
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
-                if (half == 0 && m < p.M && n0 < p.N) p.sy[(int64_t) m * p.ldsy + nb] = s.s;
-#pragma unroll
-                for (int x = 0; x < 64; x += 8) {
-                    put(x);
-#pragma unroll 1
-                    for (int r = 0; r < 32; r += 16) {
-                        const f8_scale sr = {__shfl_sync(0xffffffffu, s.s, r + sub), __shfl_sync(0xffffffffu, s.r, r + sub)};
-                        const float4 f = *at(r + sub);
-                        const float v[4] = {f.x, f.y, f.z, f.w};
-                        if (m0 + r + sub < p.M && n0 + x + unit * 4 < p.N)
-                            store4<YT>(p, m0 + r + sub, n0 + x + unit * 4, v, sr);
-                    }
-                    __syncwarp();
-                }
-            }
-            if (!ok) break;
         }
         if (!ok && lane == 0) atomicExch(p.err, 1);
     }
@@ -636,13 +643,14 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     p.ldsy = ldsy;
     p.act = act;
     const int es = y_dtype == TPMD_DTYPE_F32 ? 4 : y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
-    p.y_vec = !((uintptr_t) Y & (4 * es - 1)) && (M == 1 || ldy % 4 == 0);
     p.err = tpk_err_word();
     const int64_t nblk = (N + 127) / 128;
     // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128,
     // their k blocks shared out over a cluster of up to 8 CTAs while SMs are
     // left and each keeps two blocks
     const int nb = (M + 255) / 256 * ((nblk + 1) / 2) >= sm_count() / 2 ? 2 : 1;
+    const int unit = nb == 2 ? 16 : 4 * es;
+    p.y_vec = !((uintptr_t) Y & (unit - 1)) && (M == 1 || ldy * es % unit == 0);
     const int64_t tiles = (M + nb * 128 - 1) / (nb * 128) * ((nblk + nb - 1) / nb);
     if (tiles > INT32_MAX) return fail("too many tiles");
     p.tiles = (int) tiles;
