@@ -204,7 +204,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     auto v_fixed = [&](int i) { return bar(2 * ST + 6 + i); };
     const uint32_t q_full = bar(2 * ST + 8), fin = bar(2 * ST + 9);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const attn_desc &d = p.d;
     // block -> (cluster rank,) batch and key head, query tile (the last ones,
     // which see most keys, first)
@@ -320,54 +320,65 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (nt > 0 && !warp_wait(q_full, 0)) ok = false;
         if (!ok && lane == 0) atomicExch(p.err, 1);
     } else if (warp == 9) {
-        if (lane == 0 && nt > 0) {
+        if (nt > 0) {
+            // the whole warp goes through the loop, so that what it computes
+            // stays in uniform registers, and one lane issues the MMAs.
             // D f32 (bit 4), f16 operands; M >> 4 at bit 24, N >> 3 at bit 17; B along N (bit 16) for V
             const uint32_t id_base = (1u << 4) | (8u << 24);
             const int ksteps = (d.D + 15) / 16;
             const uint32_t id_pv = id_base | (1u << 16) | ((uint32_t) (ksteps * 2) << 17);
             int cnt = 0, fixes = 0;
-            auto wait_tile = [&](int c) { return mbar_wait(full(c % ST), (c / ST) & 1); };
+            auto wait_tile = [&](int c) { return warp_wait(full(c % ST), (c / ST) & 1); };
             auto qk = [&](int t, int j, int c) {
-                const uint32_t a = sq + (SPLIT ? 0 : t * cfg::TILE_BYTES), bb = stage(c % ST);
+                const uint64_t a = smem_desc(sq + (SPLIT ? 0 : t * cfg::TILE_BYTES), 1024, 2);
+                const uint64_t bb = smem_desc(stage(c % ST), 1024, 2);
                 const uint32_t id = id_base | ((uint32_t) (tile_w(j) >> 3) << 17);
-                for (int k = 0; k < ksteps; k++) {
-                    const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
-                    umma_f16(t_s(t), smem_desc(a + o, 1024, 2), smem_desc(bb + o, 1024, 2), id, k > 0);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < DB * 4; k++)
+                        if (k < ksteps)
+                            umma_f16(t_s(t), a + (k >> 2) * 1024 + (k & 3) * 2, bb + (k >> 2) * 1024 + (k & 3) * 2, id, k > 0);
+                    umma_commit(s_full(t));
                 }
-                umma_commit(s_full(t));
+                __syncwarp();
             };
             int done[2] = {0, 0};
-            int kc[AHEAD + 1];  // load number of K(j + x)
-            ok = mbar_wait(q_full, 0);
+            ok = warp_wait(q_full, 0);
             for (int j = 0; ok && j < min(AHEAD, nt); j++) {
-                kc[j] = cnt++;
-                ok = wait_tile(kc[j]);
+                const int c = cnt++;
+                ok = wait_tile(c);
                 if (!ok) break;
                 tc_fence_after();
                 for (int t = 0; t < 2; t++)
-                    if (active(t, j)) qk(t, j, kc[j]);
-                umma_commit(empty(kc[j] % ST));
+                    if (active(t, j)) qk(t, j, c);
+                if (elect_one()) umma_commit(empty(c % ST));
             }
             for (int j = 0; ok && j < nt; j++) {
                 const int vc = cnt++;
                 ok = wait_tile(vc);
-                if (ok && tile_keys(j) < tile_w(j)) ok = mbar_wait(v_fixed(fixes++), 0);
+                if (ok && tile_keys(j) < tile_w(j)) ok = warp_wait(v_fixed(fixes++), 0);
                 const bool more = j + AHEAD < nt;
                 const int nkc = more ? cnt++ : 0;
                 bool k_here = false;
-                for (int t = 0; ok && t < 2; t++) {
-                    if (active(t, j)) {
-                        ok = mbar_wait(p_full(t), done[t] & 1);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    if (ok && active(t, j)) {
+                        ok = warp_wait(p_full(t), done[t] & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t v = stage(vc % ST);
-                        for (int k = 0; k < tile_w(j) / 16; k++)
-                            umma_f16_ts(t_o(t), t_s(t) + k * 8, smem_desc_mn(v + k * 2048, 16384, 1024), id_pv,
-                                        done[t] > 0 || k > 0);
-                        umma_commit(o_done(t));
+                        const uint64_t v = smem_desc_mn(stage(vc % ST), 16384, 1024);
+                        const int steps = tile_w(j) / 16;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (k < steps)
+                                    umma_f16_ts(t_o(t), t_s(t) + k * 8, v + k * 128, id_pv, done[t] > 0 || k > 0);
+                            umma_commit(o_done(t));
+                        }
+                        __syncwarp();
                         done[t]++;
                     }
-                    if (more && active(t, j + AHEAD)) {
+                    if (ok && more && active(t, j + AHEAD)) {
                         if (!k_here) {
                             ok = wait_tile(nkc);
                             if (!ok) break;
@@ -378,13 +389,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                     }
                 }
                 if (ok && more && !k_here) ok = wait_tile(nkc);
-                umma_commit(empty(vc % ST));
-                if (more) umma_commit(empty(nkc % ST));
+                if (elect_one()) {
+                    umma_commit(empty(vc % ST));
+                    if (more) umma_commit(empty(nkc % ST));
+                }
+                __syncwarp();
             }
             // the MMAs in flight end before TMEM is freed
-            umma_commit(fin);
-            if (!mbar_wait(fin, 0)) ok = false;
-            if (!ok) atomicExch(p.err, 1);
+            if (elect_one()) umma_commit(fin);
+            if (!warp_wait(fin, 0)) ok = false;
+            if (!ok && lane == 0) atomicExch(p.err, 1);
         }
     } else {
         const int t = warp >> 2, q4 = warp & 3;
