@@ -95,19 +95,54 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t lbo, u
     d |= (uint64_t) 2u << 61;
     return d;
 }
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float *f) {
-    uint32_t r[32];
+// 32 columns of a row on their way into f; tmem_ld_wait ends all of a warp's loads
+__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, float *f) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
         "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]),
+          "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]),
+          "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]),
+          "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// uses of f stay behind the wait above this
+__device__ __forceinline__ void tmem_ld32_end(float *f) {
+    asm volatile(""
+                 : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]),
+                   "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]),
+                   "+f"(f[15]));
+    asm volatile(""
+                 : "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]),
+                   "+f"(f[23]), "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29]),
+                   "+f"(f[30]), "+f"(f[31]));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two f32 in one register pair
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -161,21 +196,9 @@ __device__ __forceinline__ float part_factor(float2 ml, float M) {
     return ml.x == -INFINITY ? ml.y : ex2(ml.x - M);
 }
 
-__device__ __forceinline__ void store_out(__half *o, const float *v, int d0, int n, int D, bool vec) {
-#pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-        if (e >= n) break;
-        if (vec && d0 + e + 8 <= D) {
-            __half2 h[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(v[e + 2 * i], v[e + 2 * i + 1]);
-            *reinterpret_cast<uint4 *>(o + d0 + e) = *reinterpret_cast<const uint4 *>(h);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (d0 + e + i < D) o[d0 + e + i] = __float2half_rn(v[e + i]);
-        }
-    }
+// n values of a row that is not aligned, or ends, for a vector store
+__device__ __noinline__ void copy_halves(__half *y, const __half *x, int n) {
+    for (int i = 0; i < n; i++) y[i] = x[i];
 }
 
 template <int DB, bool SPLIT>
@@ -427,26 +450,34 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 const int a0 = win ? kk.lo : 0, a1 = win ? kk.hi : min(kr.first, kk.hi);
                 const int a2 = win ? min(d.sinks, kk.hi) : 0;
                 const bool all = __all_sync(0xffffffffu, a0 <= kb && kb + 128 <= a1);
+                auto mine = [&](int c) { return c * 32 < w && (!SPLIT || (c >= c0 && c < c1)); };
                 float s[128];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    if (c * 32 < w && (!SPLIT || (c >= c0 && c < c1))) {
-                        tmem_ld32_async(t_s(t) + lanes + c * 32, s + c * 32);
-                        if (!all) {
-                            const uint32_t see = bits32(a0, a1, kb + c * 32) | bits32(0, a2, kb + c * 32);
-#pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (!(see >> e & 1)) s[c * 32 + e] = -INFINITY;
-                        }
+                    if (mine(c)) {
+                        tmem_ld32_begin(t_s(t) + lanes + c * 32, s + c * 32);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e++) s[c * 32 + e] = -INFINITY;
                     }
                 }
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32_end(s + c * 32);
+                if (!all) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if (!mine(c)) continue;
+                        const uint32_t see = bits32(a0, a1, kb + c * 32) | bits32(0, a2, kb + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (!(see >> e & 1)) s[c * 32 + e] = -INFINITY;
+                    }
+                }
                 float mx[4] = {m, m, m, m};
 #pragma unroll
-                for (int e = 0; e < 128; e++) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                for (int e = 0; e < 128; e += 2) mx[e >> 1 & 3] = max3(mx[e >> 1 & 3], s[e], s[e + 1]);
+                const float mn = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
                 // (m - m_old) scale log2(e) above 8, or a first finite maximum
                 const bool up = mn > m && !((mn - m) * p.c <= 8.0f);
                 if (__any_sync(0xffffffffu, up)) {
@@ -469,22 +500,29 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                     }
                 }
                 const float mc = m == -INFINITY ? 0.0f : m * p.c;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t c2 = pack2(p.c, p.c), mc2 = pack2(-mc, -mc);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     if (c * 32 >= w) break;
                     uint32_t pk[16];
+                    if (mine(c)) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float x = ex2(fmaf(s[c * 32 + e], p.c, -mc)), y = ex2(fmaf(s[c * 32 + e + 1], p.c, -mc));
-                        sum[e & 2] += x;
-                        sum[(e & 2) + 1] += y;
-                        const __half2 hh = __floats2half2_rn(x, y);
-                        pk[e / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 x = unpack2(fma2(pack2(s[c * 32 + e], s[c * 32 + e + 1]), c2, mc2));
+                            const float x0 = ex2(x.x), x1 = ex2(x.y);
+                            sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], pack2(x0, x1));
+                            const __half2 hh = __floats2half2_rn(x0, x1);
+                            pk[e / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) pk[e] = 0;
                     }
                     tmem_st16(t_s(t) + lanes + c * 16, pk);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 s01 = unpack2(add2(sum[0], sum[1]));
+                l += s01.x + s01.y;
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -496,20 +534,49 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         tc_fence_after();
         if (!ok && lane == 0) atomicExch(p.err, 1);
         if constexpr (!SPLIT) {
+            if (nt > 0 && done == 0) ok = warp_wait(q_full, 0);  // (Q lands before its memory is used)
             if (ok && rows) {
+                // f16 rows through this warp's part of its Q tile (read for the last
+                // time), 16-byte unit u of row i at u ^ (i mod 8) against bank
+                // conflicts: a store covers whole rows
+                constexpr int UNITS = DB * 8;
+                uint8_t *own = smem + t * cfg::TILE_BYTES + q4 * 32 * UNITS * 16;
                 const float inv = 1.0f / l;
-                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
+                const int64_t at = b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
                 bool bad = false;
 #pragma unroll 1
                 for (int x = 0; x < DB * 64; x += 32) {
                     float o[32];
-                    if (done > 0) tmem_ld32_async(t_o(t) + lanes + x, o);
+                    if (done > 0) tmem_ld32_begin(t_o(t) + lanes + x, o);
+                    tmem_ld_wait();
+                    tmem_ld32_end(o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         o[e] = l == 0.0f ? 0.0f : o[e] * inv;
                         bad = bad || (x + e < d.D && !(fabsf(o[e]) <= 65504.0f));
                     }
-                    if (row) store_out(out, o, x, 32, d.D, p.o_vec);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        __half2 hh[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) hh[i] = __floats2half2_rn(o[e + 2 * i], o[e + 2 * i + 1]);
+                        *reinterpret_cast<uint4 *>(own + lane * UNITS * 16 + (((x + e) / 8) ^ (lane & 7)) * 16) =
+                            *reinterpret_cast<const uint4 *>(hh);
+                    }
+                }
+                __syncwarp();
+                const int u = lane % UNITS;
+#pragma unroll 4
+                for (int i0r = 0; i0r < 32; i0r += 32 / UNITS) {
+                    const int i = i0r + lane / UNITS;
+                    const int64_t off = __shfl_sync(0xffffffffu, at, i);
+                    const bool real = __shfl_sync(0xffffffffu, (int) row, i) && u * 8 < d.D;
+                    const uint4 *src = reinterpret_cast<const uint4 *>(own + i * UNITS * 16 + (u ^ (i & 7)) * 16);
+                    __half *o = (__half *) d.out + off + u * 8;
+                    if (real) {
+                        if (p.o_vec && u * 8 + 8 <= d.D) *reinterpret_cast<uint4 *>(o) = *src;
+                        else copy_halves(o, reinterpret_cast<const __half *>(src), min(8, d.D - u * 8));
+                    }
                 }
                 uint32_t redo = __ballot_sync(0xffffffffu, bad && row);
                 __syncwarp();
@@ -520,15 +587,31 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 }
             }
         } else {
-            // every part's (m, sum) and O to shared memory: part = warpgroup, copy
+            // join the CTA's parts (part = warpgroup, copy). Each lane scales its
+            // part's row by exp(m - M) of the row's maximum M over all parts, and
+            // by 1 / sum where no other CTA has parts
             named_sync(1, 256);  // (both warpgroups' products are in: Q and the stages are free)
-            if (row) s_ml[(t * p.reps + rep) * per + r] = make_float2(m == -INFINITY ? -INFINITY : m * p.c, l);
+            const int np = 2 * p.reps, part = t * p.reps + rep;
+            if (row) s_ml[part * per + r] = make_float2(m == -INFINITY ? -INFINITY : m * p.c, l);
+            named_sync(1, 256);
             if (rows) {
+                float M = -INFINITY, sl = 0.0f, f = 0.0f;
+                if (row) {
+                    for (int k = 0; k < np; k++) M = fmaxf(M, s_ml[k * per + r].x);
+                    for (int k = 0; k < np; k++) {
+                        const float2 ml = s_ml[k * per + r];
+                        sl = fmaf(part_factor(ml, M), ml.y, sl);
+                    }
+                    f = part_factor(s_ml[part * per + r], M);
+                    if (p.splits == 1) f = sl == 0.0f ? 0.0f : f / sl;
+                }
 #pragma unroll 1
                 for (int x = 0; x < DB * 64; x += 32) {
                     float o[32];
                     if (done > 0) {
-                        tmem_ld32_async(t_o(t) + lanes + x, o);
+                        tmem_ld32_begin(t_o(t) + lanes + x, o);
+                        tmem_ld_wait();
+                        tmem_ld32_end(o);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e++) o[e] = 0.0f;
@@ -536,83 +619,83 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                     if (row) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4 *>(parts + ((t * p.reps + rep) * per + r) * cfg::OLD + x + e) =
-                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            *reinterpret_cast<float4 *>(parts + (part * per + r) * cfg::OLD + x + e) =
+                                make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
                     }
                 }
+                // (every lane of a row has read s_ml by the next barrier)
+                m = M;
+                l = sl;
             }
             named_sync(1, 256);
-            // join the CTA's parts into part 0
-            constexpr int C4 = DB * 16;  // 4-column pieces a row
-            const int np = 2 * p.reps, items = min(p.tb, toks) * p.g * C4;
-            for (int base = warp * 32; base < items; base += 256) {
-                const int i = min(base + lane, items - 1), rr = i / C4, x = i % C4 * 4;
-                float M = -INFINITY;
-                for (int k = 0; k < np; k++) M = fmaxf(M, s_ml[k * per + rr].x);
-                float sl = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = 0; k < np; k++) {
-                    const float2 ml = s_ml[k * per + rr];
-                    const float f = part_factor(ml, M);
-                    const float4 v = *reinterpret_cast<const float4 *>(parts + (k * per + rr) * cfg::OLD + x);
-                    sl = fmaf(f, ml.y, sl);
-                    o.x = fmaf(f, v.x, o.x);
-                    o.y = fmaf(f, v.y, o.y);
-                    o.z = fmaf(f, v.z, o.z);
-                    o.w = fmaf(f, v.w, o.w);
-                }
-                __syncwarp();  // (a row's lanes are of one warp: all have read its first part)
-                if (base + lane < items) {
-                    *reinterpret_cast<float4 *>(parts + rr * cfg::OLD + x) = o;
-                    if (x == 0) s_ml[rr] = make_float2(M, sl);
-                }
-            }
-            named_sync(1, 256);
+            if (row && part == 0) s_ml[r] = make_float2(m, l);
         }
     }
     if constexpr (SPLIT) {
-        if (p.splits > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-        if (warp < 8) {
-            constexpr int C4 = DB * 16;
-            const int nrow = min(p.tb, toks) * p.g, items = nrow * C4;
-            const uint32_t a_ml = smem_u32(s_ml), a_o = smem_u32(parts);
-            for (int i0b = rank * 256; i0b < items; i0b += p.splits * 256) {
-                const int i = i0b + threadIdx.x, rr = min(i, items - 1) / C4, x = i % C4 * 4;
-                float M = -INFINITY, sl = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = 0; k < p.splits; k++) M = fmaxf(M, ld_cluster2(cluster_addr(a_ml + rr * 8, k)).x);
-                for (int k = 0; k < p.splits; k++) {
-                    const float2 ml = ld_cluster2(cluster_addr(a_ml + rr * 8, k));
-                    const float f = part_factor(ml, M);
-                    const float4 v = ld_cluster4(cluster_addr(a_o + (rr * cfg::OLD + x) * 4, k));
-                    sl = fmaf(f, ml.y, sl);
-                    o.x = fmaf(f, v.x, o.x);
-                    o.y = fmaf(f, v.y, o.y);
-                    o.z = fmaf(f, v.z, o.z);
-                    o.w = fmaf(f, v.w, o.w);
+        constexpr int C4 = DB * 16;  // 4-column pieces a row
+        const int items = min(p.tb, toks) * p.g * C4, np = 2 * p.reps, per = 128 / p.reps;
+        auto sum_parts = [&](int rr, int x) {
+            float4 o = *reinterpret_cast<const float4 *>(parts + rr * cfg::OLD + x);
+            for (int k = 1; k < np; k++) {
+                const float4 v = *reinterpret_cast<const float4 *>(parts + (k * per + rr) * cfg::OLD + x);
+                o.x += v.x;
+                o.y += v.y;
+                o.z += v.z;
+                o.w += v.w;
+            }
+            return o;
+        };
+        if (p.splits > 1) {
+            if (warp < 8)
+                for (int i = threadIdx.x; i < items; i += 256) {
+                    const int rr = i / C4, x = i % C4 * 4;
+                    *reinterpret_cast<float4 *>(parts + rr * cfg::OLD + x) = sum_parts(rr, x);
                 }
-                const float inv = 1.0f / sl;
-                float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+            asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        }
+        if (warp < 8) {
+            const uint32_t a_ml = smem_u32(s_ml), a_o = smem_u32(parts);
+#pragma unroll 1
+            for (int base = rank * 256 + warp * 32; base < items; base += p.splits * 256) {
+                const int i = base + lane, rr = min(i, items - 1) / C4, x = i % C4 * 4;
+                float4 o;
+                if (p.splits == 1) {
+                    o = sum_parts(rr, x);
+                } else {
+                    float M = -INFINITY, sl = 0.0f;
+                    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float2 ml[8];
+                    float4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (k < p.splits) {
+                            ml[k] = ld_cluster2(cluster_addr(a_ml + rr * 8, k));
+                            v[k] = ld_cluster4(cluster_addr(a_o + (rr * cfg::OLD + x) * 4, k));
+                            M = fmaxf(M, ml[k].x);
+                        }
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (k < p.splits) {
+                            const float f = part_factor(ml[k], M);
+                            sl = fmaf(f, ml[k].y, sl);
+                            o.x = fmaf(f, v[k].x, o.x);
+                            o.y = fmaf(f, v[k].y, o.y);
+                            o.z = fmaf(f, v[k].z, o.z);
+                            o.w = fmaf(f, v[k].w, o.w);
+                        }
+                    const float inv = 1.0f / sl;
+                    o = sl == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                   : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                }
                 const int tok = tok0 + rr / p.g, h = hk * p.g + rr % p.g;
-                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
+                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2] + x;
                 bool bad = false;
-                if (i < items) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (sl == 0.0f) v[e] = 0.0f;
-                        bad = bad || (x + e < d.D && !(fabsf(v[e]) <= 65504.0f));
-                    }
-                    if (p.o_vec && x + 4 <= d.D) {
-                        const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
-                        uint2 w2;
-                        w2.x = *reinterpret_cast<const uint32_t *>(&h0);
-                        w2.y = *reinterpret_cast<const uint32_t *>(&h1);
-                        *reinterpret_cast<uint2 *>(out + x) = w2;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (x + e < d.D) out[x + e] = __float2half_rn(v[e]);
-                    }
+                if (i < items && x < d.D) {
+                    __half2 hh[2] = {__floats2half2_rn(o.x, o.y), __floats2half2_rn(o.z, o.w)};
+                    if (p.o_vec && x + 4 <= d.D) *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(hh);
+                    else copy_halves(out, reinterpret_cast<const __half *>(hh), min(4, d.D - x));
+                    bad = !(fabsf(o.x) <= 65504.0f) || (x + 1 < d.D && !(fabsf(o.y) <= 65504.0f)) ||
+                          (x + 2 < d.D && !(fabsf(o.z) <= 65504.0f)) || (x + 3 < d.D && !(fabsf(o.w) <= 65504.0f));
                 }
                 uint32_t redo = __ballot_sync(0xffffffffu, bad);
                 while (redo) {
