@@ -7,7 +7,7 @@
 // in one pass over the keys with a running maximum m and sum. Rows of the
 // MMA are (token, query head of the group) pairs, so the query heads that
 // share a key head read its keys once and a tile spans few positions. Keys
-// come in tiles of 128: those of the window from its first key on (TMA boxes
+// come in tiles of 64: those of the window from its first key on (TMA boxes
 // start at any row), then those of the sinks; the last tile of each is cut to
 // a multiple of 16 keys.
 //
@@ -46,16 +46,19 @@ namespace {
 
 template <int DB, bool SPLIT>
 struct at_cfg {
-    static constexpr int TILE_BYTES = 128 * 128 * DB;    // 128 rows of DB 64-column boxes
+    static constexpr int KT = 64;                        // keys a tile
+    static constexpr int Q_BYTES = 128 * 128 * DB;       // 128 rows of DB 64-column boxes
+    static constexpr int TILE_BYTES = KT * 128 * DB;
+    static constexpr int STAGE_BYTES = 2 * TILE_BYTES;   // a tile's V and a later one's K
     static constexpr int NQ = SPLIT ? 1 : 2;
     static constexpr int STAGES = DB == 2 ? (SPLIT ? 6 : 5) : 8;
     static constexpr int THREADS = 320;                  // 8 softmax warps, TMA, MMA
     static constexpr int OLD = DB * 64 + 4;              // floats a row of the joined parts (bank shift)
-    static constexpr int NBARS = 2 * STAGES + 2 + 2 + 2 + 4;
-    static constexpr int DATA = (NQ + STAGES) * TILE_BYTES;
+    static constexpr int NBARS = 2 * STAGES + 4 + 4 + 4 + 4;
+    static constexpr int DATA = NQ * Q_BYTES + STAGES * STAGE_BYTES;
     static constexpr int SMEM = 1024 + DATA + NBARS * 8 + 16;
     static_assert(SMEM <= 232448, "shared memory");
-    static_assert(!SPLIT || 256 * OLD * 4 <= STAGES * TILE_BYTES, "parts fit the stages");
+    static_assert(!SPLIT || 256 * OLD * 4 <= STAGES * STAGE_BYTES, "parts fit the stages");
 };
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -107,6 +110,14 @@ __device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, float *f) {
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16_begin(uint32_t taddr, float *f) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]),
+          "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15])
+        : "r"(taddr));
+}
 // uses of f stay behind the wait above this
 __device__ __forceinline__ void tmem_ld32_end(float *f) {
     asm volatile(""
@@ -211,21 +222,23 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
     // SPLIT, once the products are in: (m, sum) of every part's rows, and its O
     float2 *s_ml = (float2 *) smem;
-    float *parts = (float *) (smem + cfg::NQ * cfg::TILE_BYTES);
+    float *parts = (float *) (smem + cfg::NQ * cfg::Q_BYTES);
     uint64_t *bars = (uint64_t *) (smem + cfg::DATA);
     uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
-    const uint32_t sq = smem_u32(smem), skv = sq + cfg::NQ * cfg::TILE_BYTES;
+    const uint32_t sq = smem_u32(smem), skv = sq + cfg::NQ * cfg::Q_BYTES;
     auto bar = [&](int i) { return smem_u32(bars + i); };
-    auto stage = [&](int s) { return skv + s * cfg::TILE_BYTES; };
+    auto stage = [&](int s) { return skv + s * cfg::STAGE_BYTES; };
     auto full = [&](int s) { return bar(s); };
     auto empty = [&](int s) { return bar(ST + s); };
-    auto s_full = [&](int t) { return bar(2 * ST + t); };      // S of warpgroup t is in TMEM
-    auto p_full = [&](int t) { return bar(2 * ST + 2 + t); };  // its P is in TMEM, S read, O rescaled
-    auto o_done = [&](int t) { return bar(2 * ST + 4 + t); };  // its O += P V is done
+    // warpgroup t has two buffers of scores, used in turn: S of buffer x is in
+    // TMEM; its P is in TMEM in its place (S read, O rescaled)
+    auto s_full = [&](int t, int x) { return bar(2 * ST + 2 * t + x); };
+    auto p_full = [&](int t, int x) { return bar(2 * ST + 4 + 2 * t + x); };
+    auto o_done = [&](int t, int x) { return bar(2 * ST + 8 + 2 * t + x); };  // O += P V is done
     // the values of keys that no row sees are cleared: at most two tiles a CTA,
     // the window's last and the sinks' last, each with a barrier of its own
-    auto v_fixed = [&](int i) { return bar(2 * ST + 6 + i); };
-    const uint32_t q_full = bar(2 * ST + 8), fin = bar(2 * ST + 9);
+    auto v_fixed = [&](int i) { return bar(2 * ST + 12 + i); };
+    const uint32_t q_full = bar(2 * ST + 14), fin = bar(2 * ST + 15);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const attn_desc &d = p.d;
@@ -244,23 +257,32 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const int64_t pos0 = (int64_t) L - n + tok0;
     const key_range kr = keys_of(d, L, pos0, pos0 + toks - 1);
     // tiles of the window, then of the sinks; SPLIT: this CTA's share of them
-    const int nwin = (kr.hi - kr.lo + 127) / 128, nall = nwin + (kr.first + 127) / 128;
+    constexpr int KT = cfg::KT;
+    const int nwin = (kr.hi - kr.lo + KT - 1) / KT, nall = nwin + (kr.first + KT - 1) / KT;
     const int i0 = SPLIT ? (int) ((int64_t) nall * rank / p.splits) : 0;
     const int nt = (SPLIT ? (int) ((int64_t) nall * (rank + 1) / p.splits) : nall) - i0;
-    auto tile_key = [&](int j) { return i0 + j < nwin ? kr.lo + (i0 + j) * 128 : (i0 + j - nwin) * 128; };
-    auto tile_end = [&](int j) { return i0 + j < nwin ? kr.hi : kr.first; };
-    auto tile_keys = [&](int j) { return min(128, tile_end(j) - tile_key(j)); };
+    // (of tile j: its first key, how many of its keys some row sees, and these rounded up for the MMAs)
+    const int jwin = nwin - i0;  // the share's first tile of sinks
+    auto tile_key = [&](int j) { return j < jwin ? kr.lo + (i0 + j) * KT : (j - jwin) * KT; };
+    auto tile_keys = [&](int j) { return min(KT, (j < jwin ? kr.hi : kr.first) - tile_key(j)); };
     auto tile_w = [&](int j) { return (tile_keys(j) + 15) & ~15; };
-    // prompts: whether warpgroup t's rows see anything of tile j
+    // warpgroup t goes through tiles [from, to) and those of the sinks. Prompts:
+    // what its rows see of the window (all of it from the start where that
+    // begins within the sinks); SPLIT: every other tile
     const int toks0 = min(toks, p.tb), toks1 = toks - toks0;
-    const key_range kr0 = SPLIT ? kr : keys_of(d, L, pos0, pos0 + toks0 - 1);
-    const key_range kr1 = SPLIT ? kr : keys_of(d, L, pos0 + toks0, pos0 + toks - 1);
+    int to0 = nt, from1 = 0, to1 = nt;
+    if (!SPLIT) {
+        const key_range kr0 = keys_of(d, L, pos0, pos0 + toks0 - 1);
+        to0 = (kr0.hi - kr.lo + KT - 1) / KT;
+        if (toks1 > 0) {
+            const key_range kr1 = keys_of(d, L, pos0 + toks0, pos0 + toks - 1);
+            from1 = kr.lo < d.sinks ? 0 : (kr1.lo - kr.lo) / KT;
+            to1 = (kr1.hi - kr.lo + KT - 1) / KT;
+        }
+    }
     auto active = [&](int t, int j) {
         if (SPLIT) return (j & 1) == t;
-        if (t == 1 && toks1 <= 0) return false;
-        const key_range &k = t ? kr1 : kr0;
-        const int a = tile_key(j);
-        return i0 + j >= nwin ? a < k.hi : a < k.hi && (a + 128 > k.lo || a < d.sinks);
+        return t == 0 ? j < to0 || j >= jwin : toks1 > 0 && (j >= from1 && j < to1 || j >= jwin);
     };
 
     if (threadIdx.x == 0) {
@@ -269,9 +291,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             mbar_init(empty(s), 1);
         }
         for (int t = 0; t < 2; t++) {
-            mbar_init(s_full(t), 1);
-            mbar_init(p_full(t), 4);
-            mbar_init(o_done(t), 1);
+            for (int x = 0; x < 2; x++) {
+                mbar_init(s_full(t, x), 1);
+                mbar_init(p_full(t, x), 4);
+                mbar_init(o_done(t, x), 1);
+            }
         }
         mbar_init(q_full, 1);
         mbar_init(v_fixed(0), 1);
@@ -290,44 +314,61 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    auto t_s = [&](int t) { return tmem + t * 128; };
+    auto t_s = [&](int t, int x) { return tmem + t * 128 + x * KT; };
     auto t_o = [&](int t) { return tmem + 256 + t * DB * 64; };
     bool ok = true;
-    // loads in the order that the MMA warp uses them: K(0) (K(1)), then V(j), K(j + AHEAD)
-    constexpr int AHEAD = SPLIT ? 2 : 1;
+    // a stage for each step of the MMA warp: first the K of the first AHEAD
+    // tiles (two a warpgroup), two a stage, then V(j) with K(j + AHEAD)
+    constexpr int AHEAD = SPLIT ? 4 : 2;
 
     if (warp == 8) {
-        int cnt = 0, fixes = 0;
-        auto load = [&](const CUtensorMap *tm, int j) {
-            const int s = cnt % ST;
-            if (cnt >= ST && !warp_wait(empty(s), ((cnt / ST) - 1) & 1)) return false;
-            if (lane == 0) {
-                mbar_expect_tx(full(s), cfg::TILE_BYTES);
-                for (int x = 0; x < DB; x++) tma_load_4d(stage(s) + x * 16384, tm, full(s), x * 64, tile_key(j), hk, b);
+        int cnt = 0, slot = 0, ph = 0, fixes = 0;  // stage loads so far, the next one's slot and its phase
+        auto load = [&](const CUtensorMap *tm0, int j0, const CUtensorMap *tm1, int j1) {  // j1 < nt, or one tile
+            if (cnt >= ST && !warp_wait(empty(slot), ph ^ 1)) return false;
+            if (elect_one()) {
+                mbar_expect_tx(full(slot), j1 < nt ? cfg::STAGE_BYTES : cfg::TILE_BYTES);
+#pragma unroll
+                for (int x = 0; x < DB; x++)
+                    tma_load_4d(stage(slot) + x * (KT * 128), tm0, full(slot), x * 64, tile_key(j0), hk, b);
+                if (j1 < nt)
+#pragma unroll
+                    for (int x = 0; x < DB; x++)
+                        tma_load_4d(stage(slot) + cfg::TILE_BYTES + x * (KT * 128), tm1, full(slot), x * 64, tile_key(j1), hk,
+                                    b);
             }
-            cnt++;
+            __syncwarp();
             return true;
+        };
+        auto next = [&] {
+            cnt++;
+            if (++slot == ST) {
+                slot = 0;
+                ph ^= 1;
+            }
         };
         if (lane == 0 && nt > 0) {
             const uint32_t box = p.tb * p.g * 128;
             mbar_expect_tx(q_full, box * DB * (SPLIT ? p.reps : 2));
             for (int x = 0; x < DB; x++)
                 for (int r = 0; r < (SPLIT ? p.reps : 2); r++)
-                    tma_load_5d(sq + (SPLIT ? r * (128 / p.reps) * 128 : r * cfg::TILE_BYTES) + x * 16384, &tmQ, q_full,
+                    tma_load_5d(sq + (SPLIT ? r * (128 / p.reps) * 128 : r * cfg::Q_BYTES) + x * 16384, &tmQ, q_full,
                                 x * 64, 0, tok0 + (SPLIT ? 0 : r * p.tb), hk, b);
         }
-        for (int j = 0; ok && j < min(AHEAD, nt); j++) ok = load(&tmK, j);
+        __syncwarp();
+        for (int j = 0; ok && j < min(AHEAD, nt); j += 2) {
+            ok = load(&tmK, j, &tmK, j + 1);
+            next();
+        }
         for (int j = 0; ok && j < nt; j++) {
-            const int s = cnt % ST, ph = (cnt / ST) & 1;
-            ok = load(&tmV, j);
+            ok = load(&tmV, j, &tmK, j + AHEAD);
             const int keys = tile_keys(j), w = tile_w(j);
             if (ok && keys < w) {
                 // values of keys that no row sees: cleared (their weights are zero)
-                ok = warp_wait(full(s), ph);
+                ok = warp_wait(full(slot), ph);
                 if (!ok) break;
                 for (int i = lane; i < (w - keys) * 8 * DB; i += 32) {
                     const int x = i / ((w - keys) * 8), o = i % ((w - keys) * 8);
-                    *reinterpret_cast<uint4 *>(smem + (stage(s) - sq) + x * 16384 + keys * 128 + o * 16) =
+                    *reinterpret_cast<uint4 *>(smem + (stage(slot) - sq) + x * (KT * 128) + keys * 128 + o * 16) =
                         make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -335,7 +376,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 if (lane == 0) mbar_arrive(v_fixed(fixes));
                 fixes++;
             }
-            if (ok && j + AHEAD < nt) ok = load(&tmK, j + AHEAD);
+            next();
         }
         // the copies in flight land before the CTA goes on
         for (int i = max(0, cnt - ST); i < cnt; i++)
@@ -350,73 +391,70 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             const uint32_t id_base = (1u << 4) | (8u << 24);
             const int ksteps = (d.D + 15) / 16;
             const uint32_t id_pv = id_base | (1u << 16) | ((uint32_t) (ksteps * 2) << 17);
-            int cnt = 0, fixes = 0;
-            auto wait_tile = [&](int c) { return warp_wait(full(c % ST), (c / ST) & 1); };
-            auto qk = [&](int t, int j, int c) {
-                const uint64_t a = smem_desc(sq + (SPLIT ? 0 : t * cfg::TILE_BYTES), 1024, 2);
-                const uint64_t bb = smem_desc(stage(c % ST), 1024, 2);
+            int slot = 0, ph = 0, fixes = 0;
+            auto next = [&] {
+                if (++slot == ST) {
+                    slot = 0;
+                    ph ^= 1;
+                }
+            };
+            int issued[2] = {0, 0}, done[2] = {0, 0};
+            const uint64_t aq = smem_desc(sq, 1024, 2);
+            auto qk = [&](int t, int j, uint32_t k_tile) {
+                const int x = issued[t]++ & 1;
+                const uint64_t a = aq + (SPLIT ? 0 : t * (cfg::Q_BYTES / 16)), bb = smem_desc(k_tile, 1024, 2);
                 const uint32_t id = id_base | ((uint32_t) (tile_w(j) >> 3) << 17);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DB * 4; k++)
                         if (k < ksteps)
-                            umma_f16(t_s(t), a + (k >> 2) * 1024 + (k & 3) * 2, bb + (k >> 2) * 1024 + (k & 3) * 2, id, k > 0);
-                    umma_commit(s_full(t));
+                            umma_f16(t_s(t, x), a + (k >> 2) * 1024 + (k & 3) * 2, bb + (k >> 2) * (KT * 8) + (k & 3) * 2, id,
+                                     k > 0);
+                    umma_commit(s_full(t, x));
                 }
                 __syncwarp();
             };
-            int done[2] = {0, 0};
             ok = warp_wait(q_full, 0);
-            for (int j = 0; ok && j < min(AHEAD, nt); j++) {
-                const int c = cnt++;
-                ok = wait_tile(c);
+            for (int j = 0; ok && j < min(AHEAD, nt); j += 2) {
+                ok = warp_wait(full(slot), ph);
                 if (!ok) break;
                 tc_fence_after();
-                for (int t = 0; t < 2; t++)
-                    if (active(t, j)) qk(t, j, c);
-                if (elect_one()) umma_commit(empty(c % ST));
+                for (int e = 0; e < 2; e++)
+                    for (int t = 0; t < 2; t++)
+                        if (j + e < nt && active(t, j + e)) qk(t, j + e, stage(slot) + e * cfg::TILE_BYTES);
+                if (elect_one()) umma_commit(empty(slot));
+                __syncwarp();
+                next();
             }
             for (int j = 0; ok && j < nt; j++) {
-                const int vc = cnt++;
-                ok = wait_tile(vc);
-                if (ok && tile_keys(j) < tile_w(j)) ok = warp_wait(v_fixed(fixes++), 0);
-                const bool more = j + AHEAD < nt;
-                const int nkc = more ? cnt++ : 0;
-                bool k_here = false;
+                ok = warp_wait(full(slot), ph);
+                const int w = tile_w(j);
+                if (ok && tile_keys(j) < w) ok = warp_wait(v_fixed(fixes++), 0);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t v = smem_desc_mn(stage(slot), KT * 128, 1024);
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    if (ok && active(t, j)) {
-                        ok = warp_wait(p_full(t), done[t] & 1);
+                    if (active(t, j)) {
+                        const int x = done[t] & 1;
+                        ok = warp_wait(p_full(t, x), done[t] >> 1 & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t v = smem_desc_mn(stage(vc % ST), 16384, 1024);
-                        const int steps = tile_w(j) / 16;
                         if (elect_one()) {
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                if (k < steps)
-                                    umma_f16_ts(t_o(t), t_s(t) + k * 8, v + k * 128, id_pv, done[t] > 0 || k > 0);
-                            umma_commit(o_done(t));
+                            for (int k = 0; k < KT / 16; k++)
+                                if (k < w / 16)
+                                    umma_f16_ts(t_o(t), t_s(t, x) + k * 8, v + k * 128, id_pv, done[t] > 0 || k > 0);
+                            umma_commit(o_done(t, x));
                         }
                         __syncwarp();
                         done[t]++;
                     }
-                    if (ok && more && active(t, j + AHEAD)) {
-                        if (!k_here) {
-                            ok = wait_tile(nkc);
-                            if (!ok) break;
-                            k_here = true;
-                            tc_fence_after();
-                        }
-                        qk(t, j + AHEAD, nkc);
-                    }
+                    if (j + AHEAD < nt && active(t, j + AHEAD)) qk(t, j + AHEAD, stage(slot) + cfg::TILE_BYTES);
                 }
-                if (ok && more && !k_here) ok = wait_tile(nkc);
-                if (elect_one()) {
-                    umma_commit(empty(vc % ST));
-                    if (more) umma_commit(empty(nkc % ST));
-                }
+                if (elect_one()) umma_commit(empty(slot));
                 __syncwarp();
+                next();
             }
             // the MMAs in flight end before TMEM is freed
             if (elect_one()) umma_commit(fin);
@@ -433,41 +471,47 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         const bool rows = __any_sync(0xffffffffu, row);
         const key_range kk = keys_of(d, L, (int64_t) L - n + tok, (int64_t) L - n + tok);
         const uint32_t lanes = (uint32_t) (q4 * 32) << 16;
-        // the share of each tile's columns that this copy takes, in chunks of 32
+        // the share of each tile's columns that this copy takes, in pieces of 16
         const int c0 = SPLIT ? rep * (4 / p.reps) : 0, c1 = SPLIT ? c0 + 4 / p.reps : 4;
+        auto mine = [&](int c) { return !SPLIT || (c >= c0 && c < c1); };
         float m = -INFINITY, l = 0.0f;
         int done = 0;
         for (int j = 0; j < nt; j++) {
             if (!active(t, j)) continue;
-            ok = warp_wait(s_full(t), done & 1);
+            const int buf = done & 1;
+            ok = warp_wait(s_full(t, buf), done >> 1 & 1);
             if (!ok) break;
             tc_fence_after();
             if (rows) {
-                const int kb = tile_key(j), w = tile_w(j);
-                const bool win = i0 + j < nwin;
+                const uint32_t ts = t_s(t, buf) + lanes;
+                const int kb = tile_key(j);
+                const bool win = j < jwin;
                 // of the window's tiles the row sees [lo, hi) and what lies below
                 // sinks, of the sinks' tiles [0, first) below hi
                 const int a0 = win ? kk.lo : 0, a1 = win ? kk.hi : min(kr.first, kk.hi);
                 const int a2 = win ? min(d.sinks, kk.hi) : 0;
-                const bool all = __all_sync(0xffffffffu, a0 <= kb && kb + 128 <= a1);
-                auto mine = [&](int c) { return c * 32 < w && (!SPLIT || (c >= c0 && c < c1)); };
-                float s[128];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if (mine(c)) {
-                        tmem_ld32_begin(t_s(t) + lanes + c * 32, s + c * 32);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) s[c * 32 + e] = -INFINITY;
-                    }
-                }
-                tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32_end(s + c * 32);
-                if (!all) {
+                const bool all = __all_sync(0xffffffffu, a0 <= kb && kb + KT <= a1);
+                float s[KT];
+                if constexpr (SPLIT) {
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        if (!mine(c)) continue;
+                        if (mine(c)) {
+                            tmem_ld16_begin(ts + c * 16, s + c * 16);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e++) s[c * 16 + e] = -INFINITY;
+                        }
+                    }
+                } else {
+                    tmem_ld32_begin(ts, s);
+                    tmem_ld32_begin(ts + 32, s + 32);
+                }
+                tmem_ld_wait();
+                tmem_ld32_end(s);
+                tmem_ld32_end(s + 32);
+                if (!all) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
                         const uint32_t see = bits32(a0, a1, kb + c * 32) | bits32(0, a2, kb + c * 32);
 #pragma unroll
                         for (int e = 0; e < 32; e++)
@@ -476,7 +520,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 }
                 float mx[4] = {m, m, m, m};
 #pragma unroll
-                for (int e = 0; e < 128; e += 2) mx[e >> 1 & 3] = max3(mx[e >> 1 & 3], s[e], s[e + 1]);
+                for (int e = 0; e < KT; e += 2) mx[e >> 1 & 3] = max3(mx[e >> 1 & 3], s[e], s[e + 1]);
                 const float mn = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
                 // (m - m_old) scale log2(e) above 8, or a first finite maximum
                 const bool up = mn > m && !((mn - m) * p.c <= 8.0f);
@@ -485,7 +529,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                     if (up) m = mn;
                     l *= f;
                     if (done > 0) {  // O so far, once the last product is in
-                        ok = warp_wait(o_done(t), (done - 1) & 1);
+                        ok = warp_wait(o_done(t, buf ^ 1), (done - 1) >> 1 & 1);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -503,23 +547,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 const uint64_t c2 = pack2(p.c, p.c), mc2 = pack2(-mc, -mc);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if (c * 32 >= w) break;
+                for (int c = 0; c < 4; c += 2) {
                     uint32_t pk[16];
-                    if (mine(c)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float2 x = unpack2(fma2(pack2(s[c * 32 + e], s[c * 32 + e + 1]), c2, mc2));
-                            const float x0 = ex2(x.x), x1 = ex2(x.y);
-                            sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], pack2(x0, x1));
-                            const __half2 hh = __floats2half2_rn(x0, x1);
-                            pk[e / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                    for (int e = 0; e < 32; e += 16) {
+                        if (mine(c + e / 16)) {
+#pragma unroll
+                            for (int i = e; i < e + 16; i += 2) {
+                                const float2 x = unpack2(fma2(pack2(s[c * 16 + i], s[c * 16 + i + 1]), c2, mc2));
+                                const float x0 = ex2(x.x), x1 = ex2(x.y);
+                                sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], pack2(x0, x1));
+                                const __half2 hh = __floats2half2_rn(x0, x1);
+                                pk[i / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = e; i < e + 16; i += 2) pk[i / 2] = 0;
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) pk[e] = 0;
                     }
-                    tmem_st16(t_s(t) + lanes + c * 16, pk);
+                    tmem_st16(ts + c * 8, pk);
                 }
                 const float2 s01 = unpack2(add2(sum[0], sum[1]));
                 l += s01.x + s01.y;
@@ -527,10 +573,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(t));
+            if (lane == 0) mbar_arrive(p_full(t, buf));
             done++;
         }
-        if (ok && done > 0) ok = warp_wait(o_done(t), (done - 1) & 1);
+        if (ok && done > 0) ok = warp_wait(o_done(t, (done - 1) & 1), (done - 1) >> 1 & 1);
         tc_fence_after();
         if (!ok && lane == 0) atomicExch(p.err, 1);
         if constexpr (!SPLIT) {
@@ -540,10 +586,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 // time), 16-byte unit u of row i at u ^ (i mod 8) against bank
                 // conflicts: a store covers whole rows
                 constexpr int UNITS = DB * 8;
-                uint8_t *own = smem + t * cfg::TILE_BYTES + q4 * 32 * UNITS * 16;
-                const float inv = 1.0f / l;
+                uint8_t *own = smem + t * cfg::Q_BYTES + q4 * 32 * UNITS * 16;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const int64_t at = b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
-                bool bad = false;
+                // the largest magnitude's bits: above 65504's if it is beyond f16 or NaN
+                uint32_t top = 0;
 #pragma unroll 1
                 for (int x = 0; x < DB * 64; x += 32) {
                     float o[32];
@@ -552,8 +599,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                     tmem_ld32_end(o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
-                        o[e] = l == 0.0f ? 0.0f : o[e] * inv;
-                        bad = bad || (x + e < d.D && !(fabsf(o[e]) <= 65504.0f));
+                        o[e] = done > 0 && x + e < d.D ? o[e] * inv : 0.0f;
+                        top = max(top, __float_as_uint(o[e]) & 0x7fffffffu);
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
@@ -578,7 +625,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                         else copy_halves(o, reinterpret_cast<const __half *>(src), min(8, d.D - u * 8));
                     }
                 }
-                uint32_t redo = __ballot_sync(0xffffffffu, bad && row);
+                uint32_t redo = __ballot_sync(0xffffffffu, row && top > 0x477fe000u);
                 __syncwarp();
                 for (; redo; redo &= redo - 1) {
                     const int src = __ffs(redo) - 1;
@@ -811,8 +858,8 @@ cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st) {
     if (split) {
         int64_t keys = d.Tk;
         if (d.left >= 0 && d.right >= 0) keys = std::min<int64_t>(keys, (int64_t) p.tb + d.left + d.right + d.sinks);
-        const int64_t tiles = (keys + 127) / 128, ctas = bh * p.qtiles;
-        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>({8, sms / ctas, (tiles + 1) / 2}));
+        const int64_t tiles = (keys + 63) / 64, ctas = bh * p.qtiles;
+        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>({8, sms / ctas, (tiles + 3) / 4}));
     }
     const int64_t ctas = bh * p.qtiles * p.splits;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
@@ -820,7 +867,7 @@ cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st) {
     const int64_t qd[5] = {d.D, p.g, d.Tq, d.Hkv, d.B}, qs[5] = {1, d.qs[2], d.qs[1], d.qs[2] * p.g, d.qs[0]};
     const int64_t kd[4] = {d.D, d.Tk, d.Hkv, d.B};
     const int64_t ks[4] = {1, d.ks[1], d.ks[2], d.ks[0]}, vs[4] = {1, d.vs[1], d.vs[2], d.vs[0]};
-    const int qb[5] = {64, p.g, p.tb, 1, 1}, kb[4] = {64, 128, 1, 1};
+    const int qb[5] = {64, p.g, p.tb, 1, 1}, kb[4] = {64, 64, 1, 1};
     if (!encode_f16(&tmQ, d.q, 5, qd, qs, qb) || !encode_f16(&tmK, d.k, 4, kd, ks, kb) ||
         !encode_f16(&tmV, d.v, 4, kd, vs, kb))
         return cudaErrorInvalidValue;
