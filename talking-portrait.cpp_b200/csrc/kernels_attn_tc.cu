@@ -52,7 +52,7 @@ struct at_cfg {
     static constexpr int STAGE_BYTES = 2 * TILE_BYTES;   // a tile's V and a later one's K
     static constexpr int NQ = SPLIT ? 1 : 2;
     static constexpr int STAGES = DB == 2 ? (SPLIT ? 6 : 5) : 8;
-    static constexpr int THREADS = 320;                  // 8 softmax warps, TMA, MMA
+    static constexpr int THREADS = 352;                  // 8 softmax warps, TMA, an MMA warp for each warpgroup
     static constexpr int OLD = DB * 64 + 4;              // floats a row of the joined parts (bank shift)
     static constexpr int NBARS = 2 * STAGES + 4 + 4 + 4 + 4;
     static constexpr int DATA = NQ * Q_BYTES + STAGES * STAGE_BYTES;
@@ -213,7 +213,7 @@ __device__ __noinline__ void copy_halves(__half *y, const __half *x, int n) {
 }
 
 template <int DB, bool SPLIT>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(352, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ at_params p) {
     using cfg = at_cfg<DB, SPLIT>;
@@ -288,7 +288,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+            mbar_init(empty(s), SPLIT ? 1 : 2);  // the MMA warps that read the stage
         }
         for (int t = 0; t < 2; t++) {
             for (int x = 0; x < 2; x++) {
@@ -300,7 +300,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         mbar_init(q_full, 1);
         mbar_init(v_fixed(0), 1);
         mbar_init(v_fixed(1), 1);
-        mbar_init(fin, 1);
+        mbar_init(fin, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -322,7 +322,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     constexpr int AHEAD = SPLIT ? 4 : 2;
 
     if (warp == 8) {
-        int cnt = 0, slot = 0, ph = 0, fixes = 0;  // stage loads so far, the next one's slot and its phase
+        int cnt = 0, slot = 0, ph = 0;  // stages so far, the next one's slot and its phase
         auto load = [&](const CUtensorMap *tm0, int j0, const CUtensorMap *tm1, int j1) {  // j1 < nt, or one tile
             if (cnt >= ST && !warp_wait(empty(slot), ph ^ 1)) return false;
             if (elect_one()) {
@@ -355,8 +355,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                                 x * 64, 0, tok0 + (SPLIT ? 0 : r * p.tb), hk, b);
         }
         __syncwarp();
-        for (int j = 0; ok && j < min(AHEAD, nt); j += 2) {
-            ok = load(&tmK, j, &tmK, j + 1);
+        for (int e = 0; ok && e < AHEAD / 2; e++) {
+            if (e < nt) ok = load(&tmK, e, &tmK, e + AHEAD / 2);
             next();
         }
         for (int j = 0; ok && j < nt; j++) {
@@ -373,91 +373,97 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(v_fixed(fixes));
-                fixes++;
+                if (lane == 0) mbar_arrive(v_fixed(j < jwin ? 0 : 1));
             }
             next();
         }
-        // the copies in flight land before the CTA goes on
+        // the copies in flight land before the CTA goes on (the first stages are
+        // empty where there are fewer tiles than warpgroups)
         for (int i = max(0, cnt - ST); i < cnt; i++)
-            if (!warp_wait(full(i % ST), (i / ST) & 1)) ok = false;
+            if ((i >= AHEAD / 2 || i < nt) && !warp_wait(full(i % ST), (i / ST) & 1)) ok = false;
         if (nt > 0 && !warp_wait(q_full, 0)) ok = false;
         if (!ok && lane == 0) atomicExch(p.err, 1);
-    } else if (warp == 9) {
+    } else if (warp >= 9) {
+        // the MMAs of warpgroup t: the whole warp goes through the loop, so that
+        // what it computes stays in uniform registers, and one lane issues.
+        // (Two warps: what one does between its MMAs, the other's hide.)
+        const int t = warp - 9;
         if (nt > 0) {
-            // the whole warp goes through the loop, so that what it computes
-            // stays in uniform registers, and one lane issues the MMAs.
             // D f32 (bit 4), f16 operands; M >> 4 at bit 24, N >> 3 at bit 17; B along N (bit 16) for V
             const uint32_t id_base = (1u << 4) | (8u << 24);
             const int ksteps = (d.D + 15) / 16;
             const uint32_t id_pv = id_base | (1u << 16) | ((uint32_t) (ksteps * 2) << 17);
-            int slot = 0, ph = 0, fixes = 0;
-            auto next = [&] {
-                if (++slot == ST) {
-                    slot = 0;
+            int slot = 0, ph = 0, issued = 0, done = 0;
+            auto skip = [&](int n) {  // n < ST stages on
+                slot += n;
+                if (slot >= ST) {
+                    slot -= ST;
                     ph ^= 1;
                 }
             };
-            int issued[2] = {0, 0}, done[2] = {0, 0};
-            const uint64_t aq = smem_desc(sq, 1024, 2);
-            auto qk = [&](int t, int j, uint32_t k_tile) {
-                const int x = issued[t]++ & 1;
-                const uint64_t a = aq + (SPLIT ? 0 : t * (cfg::Q_BYTES / 16)), bb = smem_desc(k_tile, 1024, 2);
-                const uint32_t id = id_base | ((uint32_t) (tile_w(j) >> 3) << 17);
-                if (elect_one()) {
+            const uint64_t aq = smem_desc(sq + (SPLIT ? 0 : t * cfg::Q_BYTES), 1024, 2);
+            // (by the elected lane) S of buffer x = Q K^T of a tile of w keys
+            auto qk = [&](int x, int w, uint32_t k_tile) {
+                const uint64_t bb = smem_desc(k_tile, 1024, 2);
+                const uint32_t id = id_base | ((uint32_t) (w >> 3) << 17);
 #pragma unroll
-                    for (int k = 0; k < DB * 4; k++)
-                        if (k < ksteps)
-                            umma_f16(t_s(t, x), a + (k >> 2) * 1024 + (k & 3) * 2, bb + (k >> 2) * (KT * 8) + (k & 3) * 2, id,
-                                     k > 0);
-                    umma_commit(s_full(t, x));
-                }
-                __syncwarp();
+                for (int k = 0; k < DB * 4; k++)
+                    if (k < ksteps)
+                        umma_f16(t_s(t, x), aq + (k >> 2) * 1024 + (k & 3) * 2, bb + (k >> 2) * (KT * 8) + (k & 3) * 2, id,
+                                 k > 0);
+                umma_commit(s_full(t, x));
             };
             ok = warp_wait(q_full, 0);
-            for (int j = 0; ok && j < min(AHEAD, nt); j += 2) {
+            // the first two tiles' scores: SPLIT tiles t and t + 2 in stage t, else 0 and 1 in the only one
+            const int first = SPLIT ? t : 0;
+            if (SPLIT) skip(t);
+            if (ok && first < nt) {
                 ok = warp_wait(full(slot), ph);
-                if (!ok) break;
-                tc_fence_after();
-                for (int e = 0; e < 2; e++)
-                    for (int t = 0; t < 2; t++)
-                        if (j + e < nt && active(t, j + e)) qk(t, j + e, stage(slot) + e * cfg::TILE_BYTES);
-                if (elect_one()) umma_commit(empty(slot));
-                __syncwarp();
-                next();
+                if (ok) {
+                    tc_fence_after();
+                    for (int e = 0; e < 2; e++) {
+                        const int j = first + e * (AHEAD / 2);
+                        if (j < nt && active(t, j)) {
+                            if (elect_one()) qk(issued & 1, tile_w(j), stage(slot) + e * cfg::TILE_BYTES);
+                            __syncwarp();
+                            issued++;
+                        }
+                    }
+                    if (elect_one()) umma_commit(empty(slot));
+                    __syncwarp();
+                }
             }
-            for (int j = 0; ok && j < nt; j++) {
-                ok = warp_wait(full(slot), ph);
-                const int w = tile_w(j);
-                if (ok && tile_keys(j) < w) ok = warp_wait(v_fixed(fixes++), 0);
+            skip(SPLIT ? 2 : 1);
+            for (int j = first; ok && j < nt; j += SPLIT ? 2 : 1) {
+                // everything a step needs, then its MMAs without a pause: O += P V
+                // of tile j and the scores of tile j + AHEAD
+                const int keys = tile_keys(j), w = (keys + 15) & ~15, ja = j + AHEAD, wa = ja < nt ? tile_w(ja) : 0;
+                const bool pv = active(t, j), sc = wa > 0 && active(t, ja);
+                const int x = done & 1;
+                ok = pv ? warp_wait2(full(slot), ph, p_full(t, x), done >> 1 & 1) : warp_wait(full(slot), ph);
+                if (ok && keys < w) ok = warp_wait(v_fixed(j < jwin ? 0 : 1), 0);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t v = smem_desc_mn(stage(slot), KT * 128, 1024);
+                if (elect_one()) {
+                    if (pv) {
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    if (active(t, j)) {
-                        const int x = done[t] & 1;
-                        ok = warp_wait(p_full(t, x), done[t] >> 1 & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 0; k < KT / 16; k++)
-                                if (k < w / 16)
-                                    umma_f16_ts(t_o(t), t_s(t, x) + k * 8, v + k * 128, id_pv, done[t] > 0 || k > 0);
-                            umma_commit(o_done(t, x));
-                        }
-                        __syncwarp();
-                        done[t]++;
+                        for (int k = 0; k < KT / 16; k++)
+                            if (k < w / 16)
+                                umma_f16_ts(t_o(t), t_s(t, x) + k * 8, v + k * 128, id_pv, done > 0 || k > 0);
+                        umma_commit(o_done(t, x));
                     }
-                    if (j + AHEAD < nt && active(t, j + AHEAD)) qk(t, j + AHEAD, stage(slot) + cfg::TILE_BYTES);
+                    if (sc) qk(issued & 1, wa, stage(slot) + cfg::TILE_BYTES);
+                    umma_commit(empty(slot));
                 }
-                if (elect_one()) umma_commit(empty(slot));
                 __syncwarp();
-                next();
+                done += pv;
+                issued += sc;
+                skip(SPLIT ? 2 : 1);
             }
             // the MMAs in flight end before TMEM is freed
             if (elect_one()) umma_commit(fin);
+            __syncwarp();
             if (!warp_wait(fin, 0)) ok = false;
             if (!ok && lane == 0) atomicExch(p.err, 1);
         }

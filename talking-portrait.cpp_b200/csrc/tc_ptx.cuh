@@ -99,6 +99,12 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
+// both of two barriers' phases (their latencies overlap)
+__device__ __forceinline__ bool warp_wait2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1) {
+    const bool r0 = mbar_try(bar0, parity0), r1 = mbar_try(bar1, parity1);
+    if (__all_sync(0xffffffffu, r0 && r1)) return true;
+    return warp_wait(bar0, parity0) && warp_wait(bar1, parity1);
+}
 
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
