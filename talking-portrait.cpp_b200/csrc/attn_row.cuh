@@ -1,5 +1,5 @@
-// One query row of windowed attention on the CUDA cores, by one warp: the
-// general form (any stride, alignment and type), and what a tensor-core row
+// What both forms of windowed attention share: the keys that rows see, and
+// one query row by one warp, reading nothing but its visible keys, which a row
 // that came out not finite is computed again with.
 #pragma once
 #include <cuda_fp16.h>
@@ -17,6 +17,19 @@ template <>
 __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// the keys that a set of rows sees: [0, first) and [lo, hi), lo >= first
+struct key_range {
+    int first, lo, hi;
+};
+// of the rows at positions p0 .. p1
+__device__ __forceinline__ key_range keys_of(const attn_desc &d, int L, int64_t p0, int64_t p1) {
+    key_range k;
+    k.hi = d.right < 0 ? L : (int) max((int64_t) 0, min((int64_t) L, p1 + d.right + 1));
+    k.lo = d.left < 0 ? 0 : (int) min((int64_t) k.hi, max((int64_t) 0, p0 - d.left));
+    k.first = min(d.sinks, k.lo);
+    return k;
+}
 
 // row i of head h of sequence b, which has n rows and L keys; lane e holds
 // columns e, e + 32, ... of the row (D <= 32 EPL)
@@ -64,6 +77,19 @@ __device__ __noinline__ void attn_row(const attn_desc &p, int b, int h, int i, i
         const int d = lane + 32 * e;
         if (d < p.D) out[d] = from_f<T>(l == 0.0f ? 0.0f : o[e] * inv);
     }
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// *x of CTA `rank` of the cluster (its own shared memory where there is no cluster)
+__device__ __forceinline__ float ld_part(const float *x, int rank, int ctas) {
+    if (ctas == 1) return *x;
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t) __cvta_generic_to_shared(x)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
 }
 
 }  // namespace

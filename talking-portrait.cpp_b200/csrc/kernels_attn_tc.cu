@@ -180,19 +180,6 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
     return v;
 }
 
-// the keys that a set of rows sees: [0, first) and [lo, hi), lo >= first
-struct key_range {
-    int first, lo, hi;
-};
-// of the rows at positions p0 .. p1
-__device__ __forceinline__ key_range keys_of(const attn_desc &d, int L, int64_t p0, int64_t p1) {
-    key_range k;
-    k.hi = d.right < 0 ? L : (int) max((int64_t) 0, min((int64_t) L, p1 + d.right + 1));
-    k.lo = d.left < 0 ? 0 : (int) min((int64_t) k.hi, max((int64_t) 0, p0 - d.left));
-    k.first = min(d.sinks, k.lo);
-    return k;
-}
-
 // bit c set: column base + c lies in [a, b), c < 32
 __device__ __forceinline__ uint32_t bits32(int a, int b, int base) {
     const int lo = min(max(a - base, 0), 32), hi = min(max(b - base, 0), 32);
