@@ -207,8 +207,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     constexpr int ST = cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    // SPLIT, once the products are in: (m, sum) of every part's rows, and its O
+    // SPLIT, once the products are in: (m, sum) of every part's rows, and its O; the rows' places in `out`
     float2 *s_ml = (float2 *) smem;
+    int64_t *s_out = (int64_t *) (smem + 2048);
     float *parts = (float *) (smem + cfg::NQ * cfg::Q_BYTES);
     uint64_t *bars = (uint64_t *) (smem + cfg::DATA);
     uint32_t *tmem_slot = (uint32_t *) (bars + cfg::NBARS);
@@ -668,13 +669,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                 l = sl;
             }
             named_sync(1, 256);
-            if (row && part == 0) s_ml[r] = make_float2(m, l);
+            if (row && part == 0) {
+                s_ml[r] = make_float2(m, l);
+                s_out[r] = b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2];
+            }
+            named_sync(1, 256);
         }
     }
     if constexpr (SPLIT) {
-        constexpr int C4 = DB * 16;  // 4-column pieces a row
-        const int items = min(p.tb, toks) * p.g * C4, np = 2 * p.reps, per = 128 / p.reps;
-        auto sum_parts = [&](int rr, int x) {
+        // a warp takes a row (two of one box) at a time, four columns a lane
+        constexpr int C4 = DB * 16, RPW = 32 / C4;
+        const int nrow = min(p.tb, toks) * p.g, np = 2 * p.reps, per = 128 / p.reps, x = lane % C4 * 4;
+        auto sum_parts = [&](int rr) {
             float4 o = *reinterpret_cast<const float4 *>(parts + rr * cfg::OLD + x);
             for (int k = 1; k < np; k++) {
                 const float4 v = *reinterpret_cast<const float4 *>(parts + (k * per + rr) * cfg::OLD + x);
@@ -685,32 +691,44 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             }
             return o;
         };
-        if (p.splits > 1) {
+        // stores a row's four columns; whether one of them is beyond f16 or NaN
+        auto put = [&](int rr, float4 o) {
+            if (x >= d.D) return false;
+            __half *out = (__half *) d.out + s_out[rr] + x;
+            const __half2 hh[2] = {__floats2half2_rn(o.x, o.y), __floats2half2_rn(o.z, o.w)};
+            if (p.o_vec && x + 4 <= d.D) *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(hh);
+            else copy_halves(out, reinterpret_cast<const __half *>(hh), min(4, d.D - x));
+            // (columns from D on are zeros, or what is left in TMEM: looked at up to D only)
+            const uint32_t a = __float_as_uint(o.x) & 0x7fffffffu, e = __float_as_uint(o.y) & 0x7fffffffu;
+            const uint32_t c = __float_as_uint(o.z) & 0x7fffffffu, f = __float_as_uint(o.w) & 0x7fffffffu;
+            return max(max(a, x + 1 < d.D ? e : 0u), max(x + 2 < d.D ? c : 0u, x + 3 < d.D ? f : 0u)) > 0x477fe000u;
+        };
+        uint32_t bad = 0;  // bit i: of this lane's i-th row
+        if (p.splits == 1) {
+            if (warp < 8) {
+                int i = 0;
+#pragma unroll 4
+                for (int rr = warp * RPW + lane / C4; rr < nrow; rr += 8 * RPW, i++) bad |= (uint32_t) put(rr, sum_parts(rr)) << i;
+            }
+        } else {
             if (warp < 8)
-                for (int i = threadIdx.x; i < items; i += 256) {
-                    const int rr = i / C4, x = i % C4 * 4;
-                    *reinterpret_cast<float4 *>(parts + rr * cfg::OLD + x) = sum_parts(rr, x);
-                }
-            asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-        }
-        if (warp < 8) {
-            const uint32_t a_ml = smem_u32(s_ml), a_o = smem_u32(parts);
+                for (int rr = warp * RPW + lane / C4; rr < nrow; rr += 8 * RPW)
+                    *reinterpret_cast<float4 *>(parts + rr * cfg::OLD + x) = sum_parts(rr);
+            cluster_sync_all();
+            if (warp < 8) {
+                const uint32_t a_ml = smem_u32(s_ml), a_o = smem_u32(parts) + x * 4;
+                int i = 0;
 #pragma unroll 1
-            for (int base = rank * 256 + warp * 32; base < items; base += p.splits * 256) {
-                const int i = base + lane, rr = min(i, items - 1) / C4, x = i % C4 * 4;
-                float4 o;
-                if (p.splits == 1) {
-                    o = sum_parts(rr, x);
-                } else {
+                for (int rr = (rank * 8 + warp) * RPW + lane / C4; rr < nrow; rr += p.splits * 8 * RPW, i++) {
                     float M = -INFINITY, sl = 0.0f;
-                    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     float2 ml[8];
                     float4 v[8];
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         if (k < p.splits) {
                             ml[k] = ld_cluster2(cluster_addr(a_ml + rr * 8, k));
-                            v[k] = ld_cluster4(cluster_addr(a_o + (rr * cfg::OLD + x) * 4, k));
+                            v[k] = ld_cluster4(cluster_addr(a_o + rr * cfg::OLD * 4, k));
                             M = fmaxf(M, ml[k].x);
                         }
 #pragma unroll
@@ -723,33 +741,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                             o.z = fmaf(f, v[k].z, o.z);
                             o.w = fmaf(f, v[k].w, o.w);
                         }
-                    const float inv = 1.0f / sl;
-                    o = sl == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                   : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                }
-                const int tok = tok0 + rr / p.g, h = hk * p.g + rr % p.g;
-                __half *out = (__half *) d.out + b * d.os[0] + (int64_t) tok * d.os[1] + h * d.os[2] + x;
-                bool bad = false;
-                if (i < items && x < d.D) {
-                    __half2 hh[2] = {__floats2half2_rn(o.x, o.y), __floats2half2_rn(o.z, o.w)};
-                    if (p.o_vec && x + 4 <= d.D) *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(hh);
-                    else copy_halves(out, reinterpret_cast<const __half *>(hh), min(4, d.D - x));
-                    bad = !(fabsf(o.x) <= 65504.0f) || (x + 1 < d.D && !(fabsf(o.y) <= 65504.0f)) ||
-                          (x + 2 < d.D && !(fabsf(o.z) <= 65504.0f)) || (x + 3 < d.D && !(fabsf(o.w) <= 65504.0f));
-                }
-                uint32_t redo = __ballot_sync(0xffffffffu, bad);
-                while (redo) {
-                    const int src = __ffs(redo) - 1;
-                    // C4 lanes (all of the warp, or half) hold a row
-                    redo &= C4 == 32 ? 0u : src < 16 ? 0xffff0000u : 0u;
-                    __syncwarp();
-                    attn_row<__half, 4>(d, b, __shfl_sync(0xffffffffu, h, src), __shfl_sync(0xffffffffu, tok, src), n, L,
-                                        lane);
+                    const float inv = sl == 0.0f ? 0.0f : 1.0f / sl;
+                    bad |= (uint32_t) put(rr, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)) << i;
                 }
             }
         }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, bad != 0))
+            for (int i = 0; i < 32; i++)
+                for (int e = 0; e < RPW; e++) {
+                    const uint32_t of = __ballot_sync(0xffffffffu, bad >> i & 1) & (RPW == 1 ? 0xffffffffu : 0xffffu << 16 * e);
+                    if (!of) continue;
+                    const int rr = ((p.splits == 1 ? 0 : rank * 8) + warp) * RPW + e + i * (p.splits * 8 * RPW);
+                    attn_row<__half, 4>(d, b, hk * p.g + rr % p.g, tok0 + rr / p.g, n, L, lane);
+                }
         // no CTA leaves while others read its parts
-        if (p.splits > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        if (p.splits > 1) cluster_sync_all();
     }
     tc_fence_before();
     __syncthreads();
