@@ -655,7 +655,7 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     if (tiles > INT32_MAX) return fail("too many tiles");
     p.tiles = (int) tiles;
     p.tiles_n = (int) ((nblk + nb - 1) / nb);
-    const int splits = nb == 2 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>({8, sm_count() / tiles, kblocks / 2}));
+    const int splits = nb == 2 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>({cluster_cap(tiles), sm_count() / tiles, kblocks / 2}));
     p.kb_per_split = (kblocks + splits - 1) / splits;
     p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
     CUtensorMap tmX, tmW;
