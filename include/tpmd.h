@@ -339,7 +339,7 @@ int tpk_gemm(const void *X, int64_t ldx, const void *W, int64_t ldw, float *Y, i
  * rows = 1 (activations) or 128 (weights):
  *   s[m / rows][k / 128] = max(max |x| over the block / 448, 2^-126)
  *   q[m][k] = x[m][k] / s rounded to the nearest e4m3 value (ties to even),
- * every step in IEEE float32. Blocks at the ends hold what is left; a block
+ * in float32; the sign of a zero is not kept. Blocks at the ends hold what is left; a block
  * of zeros has the smallest scale. A NaN element quantises to NaN and does
  * not count in its block's maximum; an infinite one makes the scale infinite
  * (the other elements 0, itself NaN). q: one byte an element, row stride ldq

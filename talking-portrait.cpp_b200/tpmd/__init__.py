@@ -450,16 +450,24 @@ def gemm(X, W, Y, M, N, K, ldx=None, ldw=None, ldy=None, batch=1, x_row_b=0, x_c
     return Y
 
 
-def _rows2(t, what):
-    """(data pointer, row stride) of a matrix whose rows are contiguous"""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise TpmdError(f"{what}: a matrix with contiguous rows is needed")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+_dtypes = None
 
 
-def _expect(ok, what):
-    if not ok:
-        raise TpmdError(what)
+def _f8_dtypes():
+    """(float8_e4m3fn, float32, float16, int32), torch imported once"""
+    global _dtypes
+    if _dtypes is None:
+        import torch
+        _dtypes = (torch.float8_e4m3fn, torch.float32, torch.float16, torch.int32)
+    return _dtypes
+
+
+def _rows(shape, stride):
+    """The row stride of a matrix whose rows are contiguous, else None (the
+    calls below take microseconds: their checks touch each tensor little)"""
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        return None
+    return stride[0] if shape[0] > 1 else max(shape[1], stride[0])
 
 
 def quant_f8(x, q, s, rows=1, stream=0):
@@ -467,15 +475,20 @@ def quant_f8(x, q, s, rows=1, stream=0):
     with a scale per block of rows x 128 elements (see tpk_quant_f8 in
     include/tpmd.h): q [M, K] torch.float8_e4m3fn, s [ceil(M / rows),
     ceil(K / 128)] f32. rows = 1 for activations, 128 for weights."""
-    import torch
-    _expect(rows in (1, 128), "quant_f8: rows must be 1 or 128")
-    _expect(x.dtype in (torch.float16, torch.float32), "quant_f8: x must be float16 or float32")
-    _expect(q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32, "quant_f8: q must be float8_e4m3fn, s float32")
-    _expect(x.dim() == 2 and q.shape == x.shape and tuple(s.shape) == (-(-x.shape[0] // rows), -(-x.shape[1] // 128)),
-            "quant_f8: q must have x's shape, s one element per block")
-    (xp, ldx), (qp, ldq), (sp, lds) = _rows2(x, "quant_f8 x"), _rows2(q, "quant_f8 q"), _rows2(s, "quant_f8 s")
-    _tpk_check(load_library().tpk_quant_f8(xp, int(x.dtype == torch.float16), ldx, x.shape[0], x.shape[1], rows, qp,
-                                           ldq, sp, lds, stream))
+    f8, f32, f16, _ = _f8_dtypes()
+    dt, shape = x.dtype, x.shape
+    if rows != 1 and rows != 128:
+        raise TpmdError("quant_f8: rows must be 1 or 128")
+    if (dt is not f32 and dt is not f16) or q.dtype is not f8 or s.dtype is not f32:
+        raise TpmdError("quant_f8: x must be float16 or float32, q float8_e4m3fn, s float32")
+    if len(shape) != 2 or q.shape != shape or s.shape != (-(-shape[0] // rows), -(-shape[1] // 128)):
+        raise TpmdError("quant_f8: q must have x's shape [M, K], s one element per block")
+    ldx, ldq, lds = _rows(shape, x.stride()), _rows(shape, q.stride()), _rows(s.shape, s.stride())
+    if ldx is None or ldq is None or lds is None:
+        raise TpmdError("quant_f8: the rows of x, q and s must be contiguous")
+    if load_library().tpk_quant_f8(x.data_ptr(), 1 if dt is f16 else 0, ldx, shape[0], shape[1], rows, q.data_ptr(),
+                                   ldq, s.data_ptr(), lds, stream) != 0:
+        _tpk_check(-1)
     return q, s
 
 
@@ -484,28 +497,39 @@ def gemm_f8(X, sx, W, sw, Y, sy=None, bias=None, act=0, stream=0):
     with sx (rows = 1), W [N, K] with sw (rows = 128) (see tpk_gemm_f8 in
     include/tpmd.h). Y [M, N] float32, float16, or float8_e4m3fn with its
     scales in sy [M, ceil(N / 128)]."""
-    import torch
-    f8 = torch.float8_e4m3fn
-    _expect(X.dtype == f8 and W.dtype == f8 and sx.dtype == torch.float32 and sw.dtype == torch.float32,
-            "gemm_f8: X and W must be float8_e4m3fn, their scales float32")
-    _expect(Y.dtype in (torch.float32, torch.float16, f8), "gemm_f8: Y must be float32, float16 or float8_e4m3fn")
-    _expect((sy is not None) == (Y.dtype == f8), "gemm_f8: sy goes with a float8_e4m3fn Y, and only with it")
-    _expect(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1], "gemm_f8: X [M, K] and W [N, K] must share K")
-    (M, K), N = X.shape, W.shape[0]
-    kb, nb = -(-K // 128), -(-N // 128)
-    _expect(tuple(Y.shape) == (M, N) and tuple(sx.shape) == (M, kb) and tuple(sw.shape) == (nb, kb),
-            "gemm_f8: Y must be [M, N], sx [M, ceil(K / 128)], sw [ceil(N / 128), ceil(K / 128)]")
-    _expect(sy is None or (sy.dtype == torch.float32 and tuple(sy.shape) == (M, nb)),
-            "gemm_f8: sy must be float32 [M, ceil(N / 128)]")
-    _expect(bias is None or (bias.dtype == torch.float32 and tuple(bias.shape) == (N,) and bias.is_contiguous()),
-            "gemm_f8: bias must be contiguous float32 [N]")
-    (xp, ldx), (sxp, ldsx), (wp, ldw) = _rows2(X, "gemm_f8 X"), _rows2(sx, "gemm_f8 sx"), _rows2(W, "gemm_f8 W")
-    (swp, ldsw), (yp, ldy) = _rows2(sw, "gemm_f8 sw"), _rows2(Y, "gemm_f8 Y")
-    syp, ldsy = _rows2(sy, "gemm_f8 sy") if sy is not None else (None, 0)
-    yd = DTYPE_F8 if sy is not None else DTYPE_F16 if Y.dtype == torch.float16 else DTYPE_F32
-    _tpk_check(load_library().tpk_gemm_f8(xp, ldx, sxp, ldsx, wp, ldw, swp, ldsw, yp, ldy, yd, syp, ldsy, M, N, K,
-                                          bias.data_ptr() if bias is not None else None, act, stream))
+    f8, f32, f16, _ = _f8_dtypes()
+    if X.dtype is not f8 or W.dtype is not f8 or sx.dtype is not f32 or sw.dtype is not f32:
+        raise TpmdError("gemm_f8: X and W must be float8_e4m3fn, their scales float32")
+    yt = Y.dtype
+    if yt is not f32 and yt is not f16 and yt is not f8:
+        raise TpmdError("gemm_f8: Y must be float32, float16 or float8_e4m3fn")
+    if (sy is not None) != (yt is f8):
+        raise TpmdError("gemm_f8: sy goes with a float8_e4m3fn Y, and only with it")
+    xs, ws = X.shape, W.shape
+    if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[1]:
+        raise TpmdError("gemm_f8: X [M, K] and W [N, K] must share K")
+    M, K = xs
+    N, kb, nb = ws[0], -(-K // 128), -(-ws[0] // 128)
+    if Y.shape != (M, N) or sx.shape != (M, kb) or sw.shape != (nb, kb):
+        raise TpmdError("gemm_f8: Y must be [M, N], sx [M, ceil(K / 128)], sw [ceil(N / 128), ceil(K / 128)]")
+    if bias is not None and (bias.dtype is not f32 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise TpmdError("gemm_f8: bias must be contiguous float32 [N]")
+    lds = [_rows(t.shape, t.stride()) for t in (X, sx, W, sw, Y)]
+    syp, ldsy, yd = None, 0, 1 if yt is f16 else 0
+    if sy is not None:
+        if sy.dtype is not f32 or sy.shape != (M, nb):
+            raise TpmdError("gemm_f8: sy must be float32 [M, ceil(N / 128)]")
+        syp, ldsy, yd = sy.data_ptr(), _rows(sy.shape, sy.stride()), DTYPE_F8
+    if None in lds or ldsy is None:
+        raise TpmdError("gemm_f8: the rows of X, W, Y and the scales must be contiguous")
+    if load_library().tpk_gemm_f8(X.data_ptr(), lds[0], sx.data_ptr(), lds[1], W.data_ptr(), lds[2], sw.data_ptr(),
+                                  lds[3], Y.data_ptr(), lds[4], yd, syp, ldsy, M, N, K,
+                                  None if bias is None else bias.data_ptr(), act, stream) != 0:
+        _tpk_check(-1)
     return Y
+
+
+_strides12 = C.c_int64 * 12
 
 
 def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv_len=None, stream=0):
@@ -514,23 +538,27 @@ def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv
     v [B, Tk, Hkv, D] torch CUDA f32 or f16, any strides with a contiguous
     last dimension; q_len, kv_len int32 [B] or None; left, right < 0: no
     limit on that side; scale None: 1 / sqrt(D)."""
-    import torch
-    _expect(q.dtype in (torch.float16, torch.float32) and k.dtype == q.dtype and v.dtype == q.dtype and
-            out.dtype == q.dtype, "attn_window: q, k, v and out must share float16 or float32")
-    _expect(q.dim() == 4 and k.dim() == 4 and out.shape == q.shape and v.shape == k.shape and
-            k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3],
-            "attn_window: q and out [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")
-    (B, Tq, Hq, D), (_, Tk, Hkv, _) = q.shape, k.shape
-    for t in (q, k, v, out):
-        _expect(D == 1 or t.stride(3) == 1, "attn_window: the last dimension must be contiguous")
+    _, f32, f16, i32 = _f8_dtypes()
+    dt = q.dtype
+    if (dt is not f32 and dt is not f16) or k.dtype is not dt or v.dtype is not dt or out.dtype is not dt:
+        raise TpmdError("attn_window: q, k, v and out must share float16 or float32")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or out.shape != qs or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
+        raise TpmdError("attn_window: q and out [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")
+    (B, Tq, Hq, D), Tk, Hkv = qs, ks[1], ks[2]
+    a, b, c, o = q.stride(), k.stride(), v.stride(), out.stride()
+    if D > 1 and not (a[3] == b[3] == c[3] == o[3] == 1):
+        raise TpmdError("attn_window: the last dimension must be contiguous")
     for t in (q_len, kv_len):
-        _expect(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous()),
-                "attn_window: q_len and kv_len must be contiguous int32 [B]")
-    st = (C.c_int64 * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
-    _tpk_check(load_library().tpk_attn_window(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, int(q.dtype == torch.float16), B, Tq, Tk, Hq,
-        Hkv, D, q_len.data_ptr() if q_len is not None else None, kv_len.data_ptr() if kv_len is not None else None,
-        left, right, sinks, D ** -0.5 if scale is None else scale, stream))
+        if t is not None and (t.dtype is not i32 or t.shape != (B,) or not t.is_contiguous()):
+            raise TpmdError("attn_window: q_len and kv_len must be contiguous int32 [B]")
+    st = _strides12(a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2], o[0], o[1], o[2])
+    if load_library().tpk_attn_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st,
+                                      1 if dt is f16 else 0, B, Tq, Tk, Hq, Hkv, D,
+                                      None if q_len is None else q_len.data_ptr(),
+                                      None if kv_len is None else kv_len.data_ptr(), left, right, sinks,
+                                      D ** -0.5 if scale is None else scale, stream) != 0:
+        _tpk_check(-1)
     return out
 
 
