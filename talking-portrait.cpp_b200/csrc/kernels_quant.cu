@@ -40,17 +40,48 @@ __device__ __forceinline__ vec_of<T, VEC> load_row(const T *r, int64_t c, int64_
 __device__ __forceinline__ float amax_of(const vec_of<float, 4> &x) {
     return fmaxf(fmaxf(fabsf(x.v[0]), fabsf(x.v[1])), fmaxf(fabsf(x.v[2]), fabsf(x.v[3])));
 }
-__device__ __forceinline__ float amax_of(const vec_of<__half, 8> &x) {
+__device__ __forceinline__ __half2 amax2_of(const vec_of<__half, 8> &x) {
     const __half2 *h = reinterpret_cast<const __half2 *>(x.v);
-    const __half2 a = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+    return __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+}
+__device__ __forceinline__ float amax_of(const vec_of<__half, 8> &x) {
+    const __half2 a = amax2_of(x);
     return fmaxf(__low2float(a), __high2float(a));
 }
-template <typename T, int VEC, bool ALIGNED>
-__device__ __forceinline__ void store_row(uint8_t *r, int64_t c, int64_t K, f8_scale s, const vec_of<T, VEC> &x) {
+// the maxima over the LANES lanes that hold a block, of U blocks
+template <int U, int LANES>
+__device__ __forceinline__ void amax_lanes(const vec_of<float, 4> (&v)[U], float (&top)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        top[u] = amax_of(v[u]);
+#pragma unroll
+        for (int w = LANES / 2; w > 0; w >>= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], w));
+    }
+}
+// (f16: two blocks' maxima in one register)
+template <int U, int LANES>
+__device__ __forceinline__ void amax_lanes(const vec_of<__half, 8> (&v)[U], float (&top)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u += 2) {
+        const __half2 a = amax2_of(v[u]), b = u + 1 < U ? amax2_of(v[u + 1 < U ? u + 1 : u]) : a;
+        __half2 t = __hmax2(__lows2half2(a, b), __highs2half2(a, b));
+#pragma unroll
+        for (int w = LANES / 2; w > 0; w >>= 1) t = __hmax2(t, __shfl_xor_sync(0xffffffffu, t, w));
+        top[u] = __low2float(t);
+        if (u + 1 < U) top[u + 1] = __high2float(t);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ vec_of<uint8_t, VEC> quant_vec(const vec_of<T, VEC> &x, f8_scale s) {
     vec_of<uint8_t, VEC> t;
 #pragma unroll
     for (int e = 0; e < VEC; e += 4)
         *reinterpret_cast<uint32_t *>(t.v + e) = f8_quant4(to_f(x.v[e]), to_f(x.v[e + 1]), to_f(x.v[e + 2]), to_f(x.v[e + 3]), s);
+    return t;
+}
+template <typename T, int VEC, bool ALIGNED>
+__device__ __forceinline__ void store_row(uint8_t *r, int64_t c, int64_t K, f8_scale s, const vec_of<T, VEC> &x) {
+    const vec_of<uint8_t, VEC> t = quant_vec(x, s);
     if (ALIGNED && c + VEC <= K) {
         *reinterpret_cast<vec_of<uint8_t, VEC> *>(r + c) = t;
     } else {
@@ -80,19 +111,34 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x
             if (++m >= M) break;
         }
         vec_of<T, VEC> v[U];
+        float top[U];
+        constexpr int STEP = 32 / LANES * 128;  // columns a load of a warp
+        const int64_t c = ((int64_t) g * GROUP + sub) * 128 + lane * VEC;
+        if (ALIGNED && (int64_t) (g + 1) * GROUP * 128 <= K) {  // whole blocks: no column to look at
+            const T *xp = x + m * ldx + c;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            v[u] = load_row<T, VEC, ALIGNED>(x + m * ldx, ((int64_t) g * GROUP + u * (32 / LANES) + sub) * 128 + lane * VEC, K);
+            for (int u = 0; u < U; u++) v[u] = *reinterpret_cast<const vec_of<T, VEC> *>(xp + u * STEP);
+            amax_lanes<U, LANES>(v, top);
+            uint8_t *qp = q + m * ldq + c;
+            float *sp = s + m * lds + g * GROUP + sub;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int b = g * GROUP + u * (32 / LANES) + sub;
-            float a = amax_of(v[u]);
+            for (int u = 0; u < U; u++) {
+                const f8_scale sc = f8_scale_of(top[u]);
+                *reinterpret_cast<vec_of<uint8_t, VEC> *>(qp + u * STEP) = quant_vec(v[u], sc);
+                if (lane == 0) sp[u * (STEP / 128)] = sc.s;
+            }
+        } else {
 #pragma unroll
-            for (int w = LANES / 2; w > 0; w >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, w));
-            const f8_scale sc = f8_scale_of(a);
-            if (b < kb) {
-                store_row<T, VEC, ALIGNED>(q + m * ldq, (int64_t) b * 128 + lane * VEC, K, sc, v[u]);
-                if (lane == 0) s[m * lds + b] = sc.s;
+            for (int u = 0; u < U; u++) v[u] = load_row<T, VEC, ALIGNED>(x + m * ldx, c + u * STEP, K);
+            amax_lanes<U, LANES>(v, top);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int b = g * GROUP + u * (32 / LANES) + sub;
+                const f8_scale sc = f8_scale_of(top[u]);
+                if (b < kb) {
+                    store_row<T, VEC, ALIGNED>(q + m * ldq, c + u * STEP, K, sc, v[u]);
+                    if (lane == 0) s[m * lds + b] = sc.s;
+                }
             }
         }
     }

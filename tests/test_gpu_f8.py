@@ -94,8 +94,9 @@ def test_quant_strides_and_alignment(dtype, rows):
         assert bool((sraw[:, :2] == -1).all()) and bool((sraw[:, 2 - (-K // 128):] == -1).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("rows", [1, 128])
-def test_quant_special_values(rows):
+def test_quant_special_values(rows, dtype):
     """zeros, the smallest and largest numbers, infinities, NaN, ties"""
     x = torch.zeros(130, 640)
     x[0, 0:128] = 1e-45
@@ -105,6 +106,7 @@ def test_quant_special_values(rows):
     x[3, 384] = float("nan")
     x[3, 385] = 2.0
     x[4, 512:528] = torch.tensor([448.0, 1.0625, 1.1875, 17.0, 19.0, -1.0625, 2 ** -10, 3 * 2.0 ** -10] * 2)
+    x = x.to(dtype)
     q, _ = padded(130, 640)
     s = torch.zeros(-(-130 // rows), 5, device="cuda")
     tpmd.quant_f8(x.cuda(), q, s, rows=rows)
