@@ -52,6 +52,13 @@ int tpfm_set_tensor(tpfm_ctx *ctx, const char *name, const float *data, int64_t 
  * its float.fmt.* keys must equal this handle's config. */
 int tpfm_load_gguf(tpfm_ctx *ctx, const char *path);
 
+/* Attention sinks: the first `sinks` frames of a chunk's sequence (the
+ * context frames come first) stay visible to every frame after them, beside
+ * its own window. 0 (the default) is the reference's banded attention. Takes
+ * effect with the next forward or chunk. Windows of any width run; those of
+ * more than 15 keys, and sinks, on tpk_attn_window's kernels. */
+int tpfm_set_sinks(tpfm_ctx *ctx, int sinks);
+
 /* Upload the weights; requires every tensor. */
 int tpfm_prepare(tpfm_ctx *ctx);
 

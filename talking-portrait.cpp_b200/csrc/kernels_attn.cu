@@ -355,7 +355,9 @@ bool own_rows(const int64_t *stride, int64_t n0, int64_t n1, int64_t n2, int64_t
 
 }  // namespace
 
-cudaError_t launch_attn_simt(const attn_desc &d, cudaStream_t st) {
+cudaError_t launch_attn(const attn_desc &d, cudaStream_t st) {
+    if (d.D < 1 || d.D > 256) return cudaErrorInvalidValue;
+    if (attn_tc_supported(d)) return launch_attn_tc(d, st);
     return d.f16 ? run_simt<__half>(d, st) : run_simt<float>(d, st);
 }
 
@@ -406,7 +408,7 @@ extern "C" int tpk_attn_window(const void *q, const void *k, const void *v, void
     const void *ptrs[] = {q, out, q_len, kv_len, Tk > 0 ? k : nullptr, Tk > 0 ? v : nullptr};
     tpk_device_scope dev(ptrs, 6);
     if (!dev.ok()) return fail(dev.why);
-    const cudaError_t e = attn_tc_supported(d) ? launch_attn_tc(d, (cudaStream_t) stream) : launch_attn_simt(d, (cudaStream_t) stream);
+    const cudaError_t e = launch_attn(d, (cudaStream_t) stream);
     if (e == cudaErrorInvalidValue) return fail("too many rows, or the launch was refused");
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;

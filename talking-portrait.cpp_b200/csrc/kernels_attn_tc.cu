@@ -842,7 +842,7 @@ cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st) {
     p.c = d.scale * 1.4426950408889634f;
     p.o_vec = !((uintptr_t) d.out & 15) && (d.B == 1 || d.os[0] % 8 == 0) && (d.Tq == 1 || d.os[1] % 8 == 0) &&
               (d.Hq == 1 || d.os[2] % 8 == 0);
-    p.err = tpk_err_word();
+    p.err = d.err ? d.err : tpk_err_word();
     if (!p.err) return cudaErrorUnknown;
     const int64_t bh = (int64_t) d.B * d.Hkv;
     const int sms = sm_count(), tb = 128 / p.g;

@@ -57,6 +57,7 @@ struct tpfm_ctx {
     tpfm_config c{};
     int T = 0, M = 0, CD = 0, CDp = 0, FF = 0, H = 0;  // CDp: CD padded to 8 (GEMM row strides)
     int nmod = 0;  // adaLN columns of all blocks + the final layer
+    int sinks = 0;  // first frames that every later frame attends to (tpfm_set_sinks)
     std::string err;
     std::map<std::string, int64_t> spec;
     std::map<std::string, std::vector<float>> host;
@@ -180,6 +181,37 @@ bool t_embed(tpfm_ctx *c, int s, float *te) {
                  "t embed");
 }
 
+// attention over more than the band kernel holds: wider windows, first frames
+// that stay visible, wide heads (f16 mode: on f16 q, k and v, which the qkv
+// GEMM has written)
+bool wide_attention(tpfm_ctx *c) {
+    const int64_t T = c->T, H = c->H, hd = c->H / c->c.n_heads;
+    const size_t es = c->f16 ? 2 : 4;
+    attn_desc d{};
+    d.q = c->qkv;
+    d.k = (const char *) c->qkv + H * es;
+    d.v = (const char *) c->qkv + 2 * H * es;
+    d.out = c->att;
+    const int64_t in[3] = {T * 3 * H, 3 * H, hd}, out[3] = {T * H, H, hd};
+    for (int i = 0; i < 3; i++) {
+        d.qs[i] = d.ks[i] = d.vs[i] = in[i];
+        d.os[i] = out[i];
+    }
+    d.f16 = c->f16;
+    d.B = 3;
+    d.Tq = d.Tk = c->T;
+    d.Hq = d.Hkv = c->c.n_heads;
+    d.D = (int) hd;
+    d.left = d.right = std::min(c->c.attn_window, c->T);
+    d.sinks = c->sinks;
+    d.scale = 1.0f / sqrtf((float) hd);
+    d.err = c->gerr;
+    return c->ck(launch_attn(d, c->stream), "attention");
+}
+bool band_attention(const tpfm_ctx *c) {
+    return c->sinks == 0 && 2 * c->c.attn_window + 1 <= 16 && c->H / c->c.n_heads <= 128;
+}
+
 // one forward on the device buffers: x60 (f32) and the chunk's clin are set;
 // tf row `s`; output in vout (no bias). in_chunk: a sampler step, whose
 // timestep embedding was computed at prepare and whose x60 f16 copy the
@@ -221,8 +253,11 @@ bool forward_device(tpfm_ctx *c, int s, bool in_chunk = false) {
         const float *md2 = c->mod + (size_t) (l + 1) * 6 * H;
         const float *bmod2 = last ? c->F("decoder.adaLN_modulation.1.bias")
                                   : c->F("blocks." + std::to_string(l + 1) + ".adaLN_modulation.1.bias");
-        if (!c->gemm(c->h, M, H, b + "attn.qkv.weight", 3 * H, c->qkv, c->F(b + "attn.qkv.bias")) ||
-            !K(fmt_attn(h16, c->qkv, T, H, c->c.n_heads, c->c.attn_window, c->att, st), "attention") ||
+        const bool band = band_attention(c);
+        if (!c->gemm_w(c->h, M, H, H, c->Wt(b + "attn.qkv.weight"), c->ldk.at(b + "attn.qkv.weight"), 3 * H, c->qkv,
+                       "attn.qkv", c->F(b + "attn.qkv.bias"), 0, h16 && !band ? (__half *) c->qkv : nullptr) ||
+            !(band ? K(fmt_attn(h16, c->qkv, T, H, c->c.n_heads, c->c.attn_window, c->att, st), "attention")
+                   : wide_attention(c)) ||
             !c->gemm(c->att, M, H, b + "attn.proj.weight", H, c->o, c->F(b + "attn.proj.bias")) ||
             !K(fmt_res_norm(h16, c->x, c->o, md, bmod, NM, 2 * H, M, H, eps, md, bmod,
                             3 * H, 4 * H, c->h, st),
@@ -273,7 +308,7 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
         return nullptr;
     }
     if (cfg->dim_h <= 0 || cfg->n_heads <= 0 || cfg->dim_h % cfg->n_heads || cfg->depth <= 0 || cfg->nfe < 2 ||
-        cfg->chunk_frames <= 0 || cfg->prev_frames < 0 || cfg->attn_window < 0 || 2 * cfg->attn_window + 1 > 16 ||
+        cfg->chunk_frames <= 0 || cfg->prev_frames < 0 || cfg->attn_window < 0 ||
         cfg->t_freq_dim < 2 || cfg->t_freq_dim % 2 || cfg->dim_w <= 0 || cfg->dim_a < 0 || cfg->dim_e < 0 ||
         cfg->mlp_ratio <= 0.0f || cfg->dim_h % 8 || cfg->dim_w % 8 || (int) (cfg->dim_h * cfg->mlp_ratio) % 8) {
         g_create_err = "tpfm_create: invalid config";
@@ -420,6 +455,19 @@ int tpfm_load_gguf(tpfm_ctx *c, const char *path) {
     if (tpmd_gguf_read(path, "float-fmt", 0, take_fmt_tensor, c, e, sizeof e) != 0) {
         if (std::string(e).find("rejected by the consumer") == std::string::npos) c->fail(e);
         return -1;
+    }
+    return 0;
+}
+
+int tpfm_set_sinks(tpfm_ctx *c, int sinks) {
+    if (!c) return -1;
+    if (sinks < 0 || sinks > c->T) return c->fail("tpfm_set_sinks: sinks must lie in [0, chunk_frames + prev_frames]"), -1;
+    if (sinks == c->sinks) return 0;
+    c->sinks = sinks;
+    if (c->graph) {  // captured with the old attention
+        if (!c->ck(cudaSetDevice(c->device), "cudaSetDevice")) return -1;
+        cudaGraphExecDestroy(c->graph);
+        c->graph = nullptr;
     }
     return 0;
 }

@@ -194,9 +194,11 @@ struct attn_desc {
     const int32_t *q_len, *kv_len;
     int left, right, sinks;
     float scale;
+    int *err = nullptr;  // set when a bounded wait expires (nullptr: tpk_device_status's word)
 };
-cudaError_t launch_attn_simt(const attn_desc &d, cudaStream_t st);
-// the tensor-core form: f16, D <= 128, what TMA can address
+// on the tensor cores where the inputs allow it (f16, D <= 128, what TMA can
+// address), else on the CUDA cores; D <= 256
+cudaError_t launch_attn(const attn_desc &d, cudaStream_t st);
 bool attn_tc_supported(const attn_desc &d);
 cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st);
 

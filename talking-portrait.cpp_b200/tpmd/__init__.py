@@ -53,7 +53,7 @@ EXPORTS = ("tpmd_abi_version", "tpmd_create", "tpmd_create_error", "tpmd_destroy
            "tpmd_group_set_feats", "tpmd_group_set_feats_device", "tpmd_shard_range", "tpmd_group_decode",
            "tpmd_group_max", "tpmd_group_selftest_nccl", "tpmd_decode_rgb24", "tpmd_group_decode_rgb24",
            "tpk_chw_to_rgb24", "tpk_gemm", "tpmd_decode_schedule",
-           "tpk_quant_f8", "tpk_gemm_f8", "tpk_attn_window", "tpk_device_status")
+           "tpfm_set_sinks", "tpk_quant_f8", "tpk_gemm_f8", "tpk_attn_window", "tpk_device_status")
 
 _lib = None
 
@@ -157,6 +157,7 @@ def load_library(path: str = LIB_PATH):
     L.tpfm_set_tensor.argtypes = [v, cp, v, i64]
     L.tpfm_load_gguf.argtypes = [v, cp]
     L.tpfm_prepare.argtypes = [v]
+    L.tpfm_set_sinks.argtypes = [v, C.c_int]
     L.tpfm_forward.argtypes = [v, v, v, C.c_float, v]
     L.tpfm_sample_chunk.argtypes = [v, v, v, v, v, v, C.c_int, v]
     L.tpae_default_config.argtypes = [C.POINTER(AudConfig)]
@@ -659,6 +660,10 @@ class FmtSampler:
 
     def prepare(self):
         self._check(self._L.tpfm_prepare(self._h))
+
+    def set_sinks(self, sinks: int):
+        """the first frames that every later frame attends to (0: none)"""
+        self._check(self._L.tpfm_set_sinks(self._h, int(sinks)))
 
     def forward(self, x60, cond, t: float) -> np.ndarray:
         c = self.cfg
