@@ -273,6 +273,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         return t == 0 ? j < to0 || j >= jwin : toks1 > 0 && (j >= from1 && j < to1 || j >= jwin);
     };
 
+    if (threadIdx.x == 32) {
+        prefetch_map(&tmQ);
+        prefetch_map(&tmK);
+        prefetch_map(&tmV);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) {
             mbar_init(full(s), 1);

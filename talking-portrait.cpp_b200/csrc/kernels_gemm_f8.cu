@@ -114,18 +114,24 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t tmem, uint32_t cols) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-__device__ __forceinline__ float act_one(float v, int act) {
-    if (act == 1) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
-    if (act == 2) return __fdividef(v, 1.0f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-    if (act == 3) return fmaxf(v, 0.2f * v);
+// of four values; erf by a call, so that the epilogues stay within the
+// instruction caches
+__device__ __noinline__ float4 gelu_erf4(float4 v) {
+    constexpr float R = 0.70710678118654752f;
+    return make_float4(0.5f * v.x * (1.0f + erff(v.x * R)), 0.5f * v.y * (1.0f + erff(v.y * R)),
+                       0.5f * v.z * (1.0f + erff(v.z * R)), 0.5f * v.w * (1.0f + erff(v.w * R)));
+}
+// 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
+__device__ __forceinline__ float gelu_tanh(float v) {
+    return __fdividef(v, 1.0f + __expf(v * fmaf(-0.0713548162726f, v * v, -1.5957691216057308f)));
+}
+__device__ __forceinline__ float4 act4(float4 v, int act) {
+    if (act == 1) return gelu_erf4(v);
+    if (act == 2) return make_float4(gelu_tanh(v.x), gelu_tanh(v.y), gelu_tanh(v.z), gelu_tanh(v.w));
+    if (act == 3)
+        return make_float4(fmaxf(v.x, 0.2f * v.x), fmaxf(v.y, 0.2f * v.y), fmaxf(v.z, 0.2f * v.z), fmaxf(v.w, 0.2f * v.w));
     return v;
 }
-// of four values; a call, so that the epilogues stay within the instruction caches
-__device__ __noinline__ float4 act4_call(float4 v, int act) {
-    return make_float4(act_one(v.x, act), act_one(v.y, act), act_one(v.z, act), act_one(v.w, act));
-}
-__device__ __forceinline__ float4 act4(float4 v, int act) { return act == 0 ? v : act4_call(v, act); }
 
 // NB: blocks of 128 columns a tile
 template <int NB>
@@ -264,6 +270,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     const int cta = NB == 1 ? blockIdx.x / p.splits : blockIdx.x / 2, ctas = NB == 1 ? gridDim.x / p.splits : gridDim.x / 2;
     const int kb0 = split * p.kb_per_split, nk = min(p.kblocks - kb0, p.kb_per_split);  // nk >= 1 (host)
 
+    if (threadIdx.x == 32) {
+        prefetch_map(&tmX);
+        prefetch_map(&tmW);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) {
             mbar_init(full(s), 1);
@@ -480,8 +490,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     if (NB == 1) {
         // each CTA of the cluster adds its share of the rows over all
         // splits (always in the same order), a warp a row
-        __syncthreads();
+        __syncwarp();
         if (p.splits > 1) cluster_sync();
+        else __syncthreads();
         const int n0 = cta % p.tiles_n * 128, m0 = cta / p.tiles_n * cfg::BM, n = n0 + lane * 4;
         const uint32_t part = smem_u32(smem) + lane * 16;
         float bias[4];
@@ -492,55 +503,56 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         const int rows = min(cfg::BM, p.M - m0);
 #pragma unroll 1
         for (int r0 = (split * NW + warp) * RB; r0 < rows; r0 += p.splits * NW * RB) {
-            if (p.splits > 1) {
-                float4 v[RB];
+            float4 v[RB];
 #pragma unroll
-                for (int j = 0; j < RB; j++) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int j = 0; j < RB; j++) v[j] = make_float4(bias[0], bias[1], bias[2], bias[3]);
 #pragma unroll 1
-                for (int k0 = 0; k0 < p.splits; k0 += 2) {
-                    float4 f[2][RB];
+            for (int k0 = 0; k0 < p.splits; k0 += 2) {
+                float4 f[2][RB];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        // every CTA starts with its own part: no two read one CTA's at a time
-                        int from = split + k0 + k;
-                        if (from >= p.splits) from -= p.splits;
+                for (int k = 0; k < 2; k++) {
+                    // every CTA starts with its own part: no two read one CTA's at a time
+                    int from = split + k0 + k;
+                    if (from >= p.splits) from -= p.splits;
 #pragma unroll
-                        for (int j = 0; j < RB; j++)
-                            f[k][j] = k0 + k < p.splits ? ld_rank4(part + (r0 + j) * cfg::PART_LD * 4, from)
-                                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int j = 0; j < RB; j++) {
+                        if (k0 + k >= p.splits) f[k][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        else if (p.splits > 1) f[k][j] = ld_rank4(part + (r0 + j) * cfg::PART_LD * 4, from);
+                        else f[k][j] = *reinterpret_cast<const float4 *>((const float *) smem + (r0 + j) * cfg::PART_LD + lane * 4);
                     }
-#pragma unroll
-                    for (int k = 0; k < 2; k++)
-#pragma unroll
-                        for (int j = 0; j < RB; j++) {
-                            v[j].x += f[k][j].x;
-                            v[j].y += f[k][j].y;
-                            v[j].z += f[k][j].z;
-                            v[j].w += f[k][j].w;
-                        }
                 }
-                // (this CTA's copy of its own rows: nobody else reads it)
 #pragma unroll
-                for (int j = 0; j < RB; j++)
-                    *reinterpret_cast<float4 *>((float *) smem + (r0 + j) * cfg::PART_LD + lane * 4) = v[j];
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int j = 0; j < RB; j++) {
+                        v[j].x += f[k][j].x;
+                        v[j].y += f[k][j].y;
+                        v[j].z += f[k][j].z;
+                        v[j].w += f[k][j].w;
+                    }
             }
-#pragma unroll 1
-            for (int r = r0; r < min(r0 + RB, rows); r++) {
-                const float4 f = *reinterpret_cast<const float4 *>((const float *) smem + r * cfg::PART_LD + lane * 4);
-                const float4 t = act4(make_float4(f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]), p.act);
-                const float y[4] = {t.x, t.y, t.z, t.w};
+            float top[RB];
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                v[j] = act4(v[j], p.act);
+                top[j] = fmaxf(fmaxf(n < p.N ? fabsf(v[j].x) : 0.0f, n + 1 < p.N ? fabsf(v[j].y) : 0.0f),
+                               fmaxf(n + 2 < p.N ? fabsf(v[j].z) : 0.0f, n + 3 < p.N ? fabsf(v[j].w) : 0.0f));
+            }
+            if constexpr (YT == TPMD_DTYPE_F8)
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+                    for (int j = 0; j < RB; j++) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], w));
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                if (r0 + j >= rows) break;
                 f8_scale s = {1.0f, 1.0f};
                 if constexpr (YT == TPMD_DTYPE_F8) {
-                    float top = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < p.N) top = fmaxf(top, fabsf(y[e]));
-#pragma unroll
-                    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                    s = f8_scale_of(top);
-                    if (lane == 0) p.sy[(int64_t) (m0 + r) * p.ldsy + n0 / 128] = s.s;
+                    s = f8_scale_of(top[j]);
+                    if (lane == 0) p.sy[(int64_t) (m0 + r0 + j) * p.ldsy + n0 / 128] = s.s;
                 }
-                if (n < p.N) store4<YT>(p, m0 + r, n, y, s);
+                const float y[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                if (n < p.N) store4<YT>(p, m0 + r0 + j, n, y, s);
             }
         }
         if (p.splits > 1) cluster_sync();  // no CTA leaves while others read its partial

@@ -56,6 +56,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     return mbar_wait_for(bar, parity, 2000000000ull);
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *tm) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t) tm) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int c0,
                                             int c1, int c2, int c3) {
     asm volatile(
