@@ -362,7 +362,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             for (int tile = cta; ok && tile < p.tiles; tile += ctas)
                 for (int i = 0; i < nk; i++, c++) {
                     const int s = c % ST, a = c % NA;
-                    ok = warp_wait(full(s), (c / ST) & 1) && (c < NA || warp_wait(tempty(a), ((c / NA) - 1) & 1));
+                    ok = c < NA ? warp_wait(full(s), (c / ST) & 1)
+                                : warp_wait2(full(s), (c / ST) & 1, tempty(a), ((c / NA) - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t ad = smem_desc(A(s), 1024, 2), bd = smem_desc(B(s), 1024, 2);
@@ -394,11 +395,18 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             float acc[CW];
 #pragma unroll
             for (int e = 0; e < CW; e++) acc[e] = 0.0f;
-            for (int i = 0; i < nk; i++, c++) {
-                const int a = c % NA, f = c % cfg::FR;
-                ok = warp_wait(ffull(f), (c / cfg::FR) & 1);
-                const float scale = fsx[f * cfg::BM + q * 32 + lane] * fsw[f * NB + blk];
-                ok = warp_wait(tfull(a), (c / NA) & 1) && ok;
+            // (the next block's factor is fetched once a block has been read: it
+            // waits with the products then, not before them)
+            float scale = 0.0f;
+            auto factor = [&](int at) {
+                const int f = at % cfg::FR;
+                ok = warp_wait(ffull(f), (at / cfg::FR) & 1);
+                scale = fsx[f * cfg::BM + q * 32 + lane] * fsw[f * NB + blk];
+            };
+            factor(c);
+            for (int i = 0; ok && i < nk; i++, c++) {
+                const int a = c % NA;
+                ok = warp_wait(tfull(a), (c / NA) & 1);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
@@ -411,6 +419,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_first<NB>(tempty(a));
+                if (i + 1 < nk) factor(c + 1);
             }
             if (NB == 1) {  // the (partial) tile into the stages (one tile a CTA, its products are in)
                 if (!ok) break;
@@ -422,20 +431,25 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             }
             if constexpr (NB == 2) {
                 if (!ok) break;
-                // bias and activation in place (the same columns in every lane)
+                // bias and activation in place (the same columns in every lane;
+                // one test of the activation, not one for every four columns)
+                if (p.bias) {
 #pragma unroll
-                for (int e = 0; e < CW; e += 4) {
-                    float bias[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) bias[j] = p.bias ? __ldg(p.bias + min(n0 + e + j, p.N - 1)) : 0.0f;
-                    const float4 f = act4(make_float4(acc[e] + bias[0], acc[e + 1] + bias[1], acc[e + 2] + bias[2],
-                                                      acc[e + 3] + bias[3]),
-                                          p.act);
-                    acc[e] = f.x;
-                    acc[e + 1] = f.y;
-                    acc[e + 2] = f.z;
-                    acc[e + 3] = f.w;
+                    for (int e = 0; e < CW; e++) acc[e] += __ldg(p.bias + min(n0 + e, p.N - 1));
                 }
+                auto activate = [&](auto f) {
+#pragma unroll
+                    for (int e = 0; e < CW; e += 4) {
+                        const float4 v = f(make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]));
+                        acc[e] = v.x;
+                        acc[e + 1] = v.y;
+                        acc[e + 2] = v.z;
+                        acc[e + 3] = v.w;
+                    }
+                };
+                if (p.act == 1) activate([](float4 v) { return gelu_erf4(v); });
+                else if (p.act == 2) activate([](float4 v) { return act4(v, 2); });
+                else if (p.act == 3) activate([](float4 v) { return act4(v, 3); });
                 f8_scale k = {1.0f, 1.0f};
                 if constexpr (YT == TPMD_DTYPE_F8) {
                     float top = 0.0f;
@@ -450,6 +464,11 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 // a store covers eight rows
                 constexpr int ES = YT == TPMD_DTYPE_F32 ? 4 : YT == TPMD_DTYPE_F16 ? 2 : 1, PER = 16 / ES;
                 const int sub = lane / 4, unit = lane % 4;
+                uint8_t *y = (uint8_t *) p.Y + ((int64_t) (m0 + sub) * p.ldy + n0 + unit * PER) * ES;
+                const int64_t step = 8 * p.ldy * ES;
+                const uint8_t *src = piece + sub * 64 + (unit ^ (sub >> 1 & 3)) * 16;  // (row + 8: the same unit)
+                uint8_t *own = piece + lane * 64;
+                const bool whole = p.y_vec && m0 + 32 <= p.M && n0 + CW <= p.N;
 #pragma unroll
                 for (int x = 0; x < CW; x += 4 * PER) {
 #pragma unroll
@@ -468,18 +487,20 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                                            f8_quant4(v[8], v[9], v[10], v[11], k),
                                            f8_quant4(v[12], v[13], v[14], v[15], k));
                         }
-                        *reinterpret_cast<uint4 *>(piece + lane * 64 + (u ^ (lane >> 1 & 3)) * 16) = w;
+                        *reinterpret_cast<uint4 *>(own + (u ^ (lane >> 1 & 3)) * 16) = w;
                     }
                     __syncwarp();
-                    const int n = n0 + x + unit * PER;
+                    if (whole) {
+                        uint4 t[4];
 #pragma unroll
-                    for (int r = 0; r < 32; r += 8) {
-                        const int row = r + sub;
-                        const uint4 *src = reinterpret_cast<const uint4 *>(piece + row * 64 + (unit ^ (row >> 1 & 3)) * 16);
-                        uint8_t *y = (uint8_t *) p.Y + ((int64_t) (m0 + row) * p.ldy + n) * ES;
-                        if (m0 + row >= p.M || n >= p.N) continue;
-                        if (p.y_vec && n + PER <= p.N) *reinterpret_cast<uint4 *>(y) = *src;
-                        else copy_elements<ES>(y, reinterpret_cast<const uint8_t *>(src), min(PER, p.N - n));
+                        for (int r = 0; r < 4; r++) t[r] = *reinterpret_cast<const uint4 *>(src + r * 512);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) *reinterpret_cast<uint4 *>(y + r * step + x * ES) = t[r];
+                    } else {
+                        const int left = min(PER, p.N - n0 - x - unit * PER);
+#pragma unroll 1
+                        for (int r = 0; r < 4; r++)
+                            if (m0 + sub + r * 8 < p.M && left > 0) copy_elements<ES>(y + r * step + x * ES, src + r * 512, left);
                     }
                     __syncwarp();
                 }
