@@ -395,19 +395,26 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             float acc[CW];
 #pragma unroll
             for (int e = 0; e < CW; e++) acc[e] = 0.0f;
-            // (the next block's factor is fetched once a block has been read: it
-            // waits with the products then, not before them)
-            float scale = 0.0f;
-            auto factor = [&](int at) {
-                const int f = at % cfg::FR;
-                ok = warp_wait(ffull(f), (at / cfg::FR) & 1);
-                scale = fsx[f * cfg::BM + q * 32 + lane] * fsw[f * NB + blk];
-            };
-            factor(c);
-            for (int i = 0; ok && i < nk; i++, c++) {
+            // four blocks' factors at a time, once the last of them is there (the
+            // TMA warp is that far ahead: the fifth block after the one being
+            // read waits for the products of that one only)
+            static_assert(ST >= 4, "the TMA warp may run four blocks ahead");
+            float f4[4];
+            for (int i = 0; i < nk; i++, c++) {
                 const int a = c % NA;
-                ok = warp_wait(tfull(a), (c / NA) & 1);
+                if (i % 4 == 0) {
+                    const int last = c + min(3, nk - 1 - i);
+                    ok = warp_wait2(ffull(last % cfg::FR), (last / cfg::FR) & 1, tfull(a), (c / NA) & 1);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int f = min(c + e, last) % cfg::FR;
+                        f4[e] = fsx[f * cfg::BM + q * 32 + lane] * fsw[f * NB + blk];
+                    }
+                } else {
+                    ok = warp_wait(tfull(a), (c / NA) & 1);
+                }
                 if (!ok) break;
+                const float scale = i % 4 == 0 ? f4[0] : i % 4 == 1 ? f4[1] : i % 4 == 2 ? f4[2] : f4[3];
                 tc_fence_after();
 #pragma unroll
                 for (int x = 0; x < CW; x += 32) {
@@ -419,7 +426,6 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_first<NB>(tempty(a));
-                if (i + 1 < nk) factor(c + 1);
             }
             if (NB == 1) {  // the (partial) tile into the stages (one tile a CTA, its products are in)
                 if (!ok) break;
