@@ -6,9 +6,11 @@
 // GEMM, where it is written in the GEMM's input type TIN (float or __half).
 // The block linears add their bias in the GEMM epilogue (fc1 also GELU);
 // the kernel consuming the other GEMMs' output adds their bias.
+#include "f8.cuh"
 #include "tpmd_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tpmd {
 namespace {
@@ -232,7 +234,8 @@ __global__ void __launch_bounds__(256) res_norm_kernel(float *__restrict__ x, co
 // res_norm_kernel with one warp per row for H = 128 NV: each lane holds NV
 // float4 groups (columns 4 lane + 128 j); every load of the row (x, o, both
 // modulations) goes out before the first use, the sums are warp shuffles in
-// a fixed order, no block barrier
+// a fixed order, no block barrier. TIN = uint8_t: h is quantised to e4m3, one
+// scale for each 128 columns (a group j of the warp's lanes) in hs [M][NV]
 template <typename TIN, int NV>
 __global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ x, const float *__restrict__ o,
                                                             const float *__restrict__ mod,
@@ -240,7 +243,8 @@ __global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ 
                                                             int gate_off, int M, float eps,
                                                             const float *__restrict__ mod2,
                                                             const float *__restrict__ bmod2, int shift_off,
-                                                            int scale_off, TIN *__restrict__ h) {
+                                                            int scale_off, TIN *__restrict__ h,
+                                                            float *__restrict__ hs) {
     pdl_wait();
     pdl_trigger();
     constexpr int H = 128 * NV;
@@ -302,8 +306,17 @@ __global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ 
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = v[e] * sc[e] + v[e] + sh[e];
         TIN *hp = h + (int64_t) m * H + 4 * q;
+        if constexpr (std::is_same<TIN, uint8_t>::value) {
+            float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
-        for (int e = 0; e < 4; e++) hp[e] = cvt<TIN>(v[e]);
+            for (int w = 16; w > 0; w >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, w));
+            const f8_scale k = f8_scale_of(a);
+            *reinterpret_cast<uint32_t *>(hp) = f8_quant4(v[0], v[1], v[2], v[3], k);
+            if (lane == 0) hs[(int64_t) m * NV + j] = k.s;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) hp[e] = cvt<TIN>(v[e]);
+        }
     }
 }
 
@@ -389,19 +402,24 @@ cudaError_t fmt_attn(bool f16, const float *qkv, int T, int H, int nh, int windo
 }
 cudaError_t fmt_res_norm(bool f16, float *x, const float *o, const float *mod, const float *bmod,
                          int mod_stride, int gate_off, int M, int H, float eps, const float *mod2, const float *bmod2,
-                         int shift_off, int scale_off, void *h, cudaStream_t st) {
+                         int shift_off, int scale_off, void *h, cudaStream_t st, float *hs) {
     if (H > RN_PER_THREAD * 256) return cudaErrorInvalidValue;
     const bool al = !(((uintptr_t) x | (uintptr_t) o | (uintptr_t) mod | (uintptr_t) bmod |
                        (uintptr_t) mod2 | (uintptr_t) bmod2) & 15) &&
                     mod_stride % 4 == 0 && gate_off % 4 == 0 && shift_off % 4 == 0 && scale_off % 4 == 0;
     if (H == 1024 && al) {  // the sampler's width: a warp per row
         const dim3 g((M * 32 + 255) / 256);
+        float *none = nullptr;
+        if (hs)
+            return launch_pdl(res_norm_warp_kernel<uint8_t, 8>, g, dim3(256), 0, st, x, o, mod, bmod, mod_stride,
+                              gate_off, M, eps, mod2, bmod2, shift_off, scale_off, (uint8_t *) h, hs);
         if (f16)
             return launch_pdl(res_norm_warp_kernel<__half, 8>, g, dim3(256), 0, st, x, o, mod, bmod, mod_stride,
-                              gate_off, M, eps, mod2, bmod2, shift_off, scale_off, (__half *) h);
+                              gate_off, M, eps, mod2, bmod2, shift_off, scale_off, (__half *) h, none);
         return launch_pdl(res_norm_warp_kernel<float, 8>, g, dim3(256), 0, st, x, o, mod, bmod, mod_stride, gate_off,
-                          M, eps, mod2, bmod2, shift_off, scale_off, (float *) h);
+                          M, eps, mod2, bmod2, shift_off, scale_off, (float *) h, none);
     }
+    if (hs) return cudaErrorInvalidValue;
     if (f16)
         return launch_pdl(res_norm_kernel<__half>, dim3(M), dim3(256), 0, st, x, o, mod, bmod, mod_stride,
                           gate_off, H, eps, mod2, bmod2, shift_off, scale_off, (__half *) h);

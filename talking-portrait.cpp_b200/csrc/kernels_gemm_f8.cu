@@ -300,6 +300,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         // rows' sx a lane, loaded four blocks ahead. Block c's slot was last read
         // for block c - FR, and its stage is free only when the products of
         // block c - ST are done, which began after block c - ST - NA was read.
+        // (a programmatic dependent starts while the kernel before it runs: all
+        // that this one reads of it, and writes, comes after this wait)
+        pdl_wait();
+        pdl_trigger();
         int c = 0;
         for (int tile = cta; ok && tile < p.tiles; tile += ctas) {
             const int n0 = tile % p.tiles_n * cfg::BN, m0 = (tile / p.tiles_n * NB + rank) * cfg::BM;
@@ -602,7 +606,7 @@ bool encode_bytes(CUtensorMap *tm, const void *base, int64_t cols, int64_t rows,
 }
 
 template <int YT, int NB>
-cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
+cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st, bool pdl) {
     using cfg = f8_cfg<NB>;
     static std::mutex mu;
     static uint64_t attr_set = 0;  // one bit per device
@@ -622,22 +626,76 @@ cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_para
     lc.blockDim = dim3(cfg::THREADS, 1, 1);
     lc.dynamicSmemBytes = cfg::SMEM;
     lc.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned) (NB == 1 ? p.splits : 2);
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    int na = 0;
+    if (NB == 2 || p.splits > 1) {
+        at[na].id = cudaLaunchAttributeClusterDimension;
+        at[na].val.clusterDim.x = (unsigned) (NB == 1 ? p.splits : 2);
+        at[na].val.clusterDim.y = 1;
+        at[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (pdl) {
+        at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
     lc.attrs = at;
-    lc.numAttrs = NB == 2 || p.splits > 1 ? 1 : 0;
+    lc.numAttrs = na;
     const cudaError_t e = cudaLaunchKernelEx(&lc, gemm_f8_kernel<YT, NB>, tmX, tmW, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 template <int YT>
-cudaError_t run_f8(int nb, const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
-    return nb == 2 ? run_f8<YT, 2>(tmX, tmW, p, st) : run_f8<YT, 1>(tmX, tmW, p, st);
+cudaError_t run_f8(int nb, const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st, bool pdl) {
+    return nb == 2 ? run_f8<YT, 2>(tmX, tmW, p, st, pdl) : run_f8<YT, 1>(tmX, tmW, p, st, pdl);
 }
 
 }  // namespace
+
+cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
+    f8_params p{};
+    const int kblocks = (d.K + 127) / 128;
+    p.M = d.M;
+    p.N = d.N;
+    p.K = d.K;
+    p.kblocks = kblocks;
+    p.sx = d.sx;
+    p.sw = d.sw;
+    p.bias = d.bias;
+    p.ldsx = d.ldsx;
+    p.ldsw = d.ldsw;
+    p.Y = d.Y;
+    p.ldy = d.ldy;
+    p.sy = d.sy;
+    p.ldsy = d.ldsy;
+    p.act = d.act;
+    p.err = d.err ? d.err : tpk_err_word();
+    if (!p.err) return cudaErrorUnknown;
+    const int es = d.y_dtype == TPMD_DTYPE_F32 ? 4 : d.y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
+    const int64_t nblk = (d.N + 127) / 128;
+    // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128,
+    // their k blocks shared out over a cluster while SMs are left and each CTA
+    // keeps two blocks
+    const int nb = ((int64_t) d.M + 255) / 256 * ((nblk + 1) / 2) >= sm_count() / 2 ? 2 : 1;
+    const int unit = nb == 2 ? 16 : 4 * es;
+    p.y_vec = !((uintptr_t) d.Y & (unit - 1)) && (d.M == 1 || d.ldy * es % unit == 0);
+    const int64_t tiles = ((int64_t) d.M + nb * 128 - 1) / (nb * 128) * ((nblk + nb - 1) / nb);
+    if (tiles > INT32_MAX / 8) return cudaErrorInvalidValue;
+    p.tiles = (int) tiles;
+    p.tiles_n = (int) ((nblk + nb - 1) / nb);
+    const int splits =
+        nb == 2 ? 1
+                : (int) std::max<int64_t>(1, std::min<int64_t>({cluster_cap(tiles), sm_count() / tiles, kblocks / 2}));
+    p.kb_per_split = (kblocks + splits - 1) / splits;
+    p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
+    CUtensorMap tmX, tmW;
+    if (!encode_bytes(&tmX, d.X, d.K, d.M, d.ldx, 128) || !encode_bytes(&tmW, d.W, d.K, d.N, d.ldw, 128))
+        return cudaErrorInvalidValue;
+    return d.y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(nb, tmX, tmW, p, st, d.pdl)
+           : d.y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(nb, tmX, tmW, p, st, d.pdl)
+                                         : run_f8<TPMD_DTYPE_F8>(nb, tmX, tmW, p, st, d.pdl);
+}
+
 }  // namespace tpmd
 
 extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t ldsx, const void *W, int64_t ldw,
@@ -666,46 +724,29 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     const void *ptrs[] = {X, sx, W, sw, Y, sy, bias};
     tpk_device_scope dev(ptrs, 7);
     if (!dev.ok()) return fail(dev.why);
-    f8_params p{};
-    p.M = M;
-    p.N = N;
-    p.K = K;
-    p.kblocks = kblocks;
-    p.sx = sx;
-    p.sw = sw;
-    p.bias = bias;
-    p.ldsx = ldsx;
-    p.ldsw = ldsw;
-    p.Y = Y;
-    p.ldy = ldy;
-    p.sy = sy;
-    p.ldsy = ldsy;
-    p.act = act;
-    const int es = y_dtype == TPMD_DTYPE_F32 ? 4 : y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
-    p.err = tpk_err_word();
-    const int64_t nblk = (N + 127) / 128;
-    // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128,
-    // their k blocks shared out over a cluster of up to 8 CTAs while SMs are
-    // left and each keeps two blocks
-    const int nb = (M + 255) / 256 * ((nblk + 1) / 2) >= sm_count() / 2 ? 2 : 1;
-    const int unit = nb == 2 ? 16 : 4 * es;
-    p.y_vec = !((uintptr_t) Y & (unit - 1)) && (M == 1 || ldy * es % unit == 0);
-    const int64_t tiles = (M + nb * 128 - 1) / (nb * 128) * ((nblk + nb - 1) / nb);
-    if (tiles > INT32_MAX) return fail("too many tiles");
-    p.tiles = (int) tiles;
-    p.tiles_n = (int) ((nblk + nb - 1) / nb);
-    const int splits = nb == 2 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>({cluster_cap(tiles), sm_count() / tiles, kblocks / 2}));
-    p.kb_per_split = (kblocks + splits - 1) / splits;
-    p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
-    CUtensorMap tmX, tmW;
-    if (!p.err || !encode_bytes(&tmX, X, K, M, ldx, 128) || !encode_bytes(&tmW, W, K, N, ldw, 128)) {
+    gemm_f8_desc d;
+    d.X = X;
+    d.ldx = ldx;
+    d.sx = sx;
+    d.ldsx = ldsx;
+    d.W = W;
+    d.ldw = ldw;
+    d.sw = sw;
+    d.ldsw = ldsw;
+    d.Y = Y;
+    d.ldy = ldy;
+    d.y_dtype = y_dtype;
+    d.sy = sy;
+    d.ldsy = ldsy;
+    d.M = M;
+    d.N = N;
+    d.K = K;
+    d.bias = bias;
+    d.act = act;
+    const cudaError_t e = gemm_f8(d, (cudaStream_t) stream);
+    if (e != cudaSuccess) {
         cudaGetLastError();
-        return fail("set-up failed");
+        return fail(e == cudaErrorInvalidValue ? "too many tiles, or the launch was refused" : cudaGetErrorString(e));
     }
-    cudaStream_t st = (cudaStream_t) stream;
-    const cudaError_t e = y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(nb, tmX, tmW, p, st)
-                          : y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(nb, tmX, tmW, p, st)
-                                                      : run_f8<TPMD_DTYPE_F8>(nb, tmX, tmW, p, st);
-    if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;
 }

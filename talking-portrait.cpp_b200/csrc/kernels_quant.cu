@@ -97,6 +97,8 @@ template <typename T, int VEC, bool ALIGNED, int U>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t M, int64_t K,
                                                          int kb, uint8_t *__restrict__ q, int64_t ldq,
                                                          float *__restrict__ s, int64_t lds) {
+    pdl_wait();
+    pdl_trigger();
     constexpr int LANES = 128 / VEC, GROUP = U * 32 / LANES;
     const int per_row = (kb + GROUP - 1) / GROUP, lane = threadIdx.x % LANES, sub = threadIdx.x % 32 / LANES;
     const int64_t warps = (int64_t) gridDim.x * 8, w0 = (int64_t) blockIdx.x * 8 + threadIdx.x / 32;
@@ -177,29 +179,46 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__
 
 template <typename T, int VEC, bool ALIGNED>
 cudaError_t run_quant(const void *x, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
-                      int64_t lds, cudaStream_t st) {
+                      int64_t lds, cudaStream_t st, bool pdl) {
     const int64_t kb = (K + 127) / 128;
     if (rows == 1) {
         // loads in flight a lane: four where the blocks fill the SMs' warps all
         // the same, else one (180 x 1024 f32: 2.0 us, with four 3.1)
         auto go = [&](auto kernel, int group) {
             const int64_t ctas = (M * ((kb + group - 1) / group) + 7) / 8;
-            kernel<<<(unsigned) std::min<int64_t>(ctas, 148 * 8), 256, 0, st>>>((const T *) x, ldx, M, K, (int) kb,
-                                                                              (uint8_t *) q, ldq, s, lds);
+            const dim3 grid((unsigned) std::min<int64_t>(ctas, 148 * 8));
+            if (pdl)
+                return launch_pdl(kernel, grid, dim3(256), 0, st, (const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s,
+                                  lds);
+            kernel<<<grid, 256, 0, st>>>((const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s, lds);
+            return cudaGetLastError();
         };
         constexpr int PER = VEC / 4;  // blocks a load of a warp
-        if (M * ((kb + 4 * PER - 1) / (4 * PER)) >= 148 * 64) go(quant_rows_kernel<T, VEC, ALIGNED, 4>, 4 * PER);
-        else go(quant_rows_kernel<T, VEC, ALIGNED, 1>, PER);
-    } else {
-        const int64_t ctas = (M + 127) / 128 * kb;
-        if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-        quant_blocks_kernel<T, VEC, ALIGNED><<<(unsigned) ctas, 256, 0, st>>>(
-            (const T *) x, ldx, M, K, kb, (uint8_t *) q, ldq, s, lds);
+        if (M * ((kb + 4 * PER - 1) / (4 * PER)) >= 148 * 64) return go(quant_rows_kernel<T, VEC, ALIGNED, 4>, 4 * PER);
+        return go(quant_rows_kernel<T, VEC, ALIGNED, 1>, PER);
     }
+    const int64_t ctas = (M + 127) / 128 * kb;
+    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+    quant_blocks_kernel<T, VEC, ALIGNED><<<(unsigned) ctas, 256, 0, st>>>((const T *) x, ldx, M, K, kb, (uint8_t *) q, ldq,
+                                                                         s, lds);
     return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t quant_f8(const void *x, bool f16, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
+                     int64_t lds, cudaStream_t st, bool pdl) {
+    const int es = f16 ? 2 : 4, vec = 16 / es;
+    // whole 16-byte loads and 4- or 8-byte stores where every row starts aligned for them
+    const bool al = !((uintptr_t) x & 15) && !((uintptr_t) q & (vec - 1)) &&
+                    (M == 1 || (ldx * es % 16 == 0 && ldq % vec == 0));
+    if (f16)
+        return al ? run_quant<__half, 8, true>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl)
+                  : run_quant<__half, 8, false>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl);
+    return al ? run_quant<float, 4, true>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl)
+              : run_quant<float, 4, false>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl);
+}
+
 }  // namespace tpmd
 
 extern "C" int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, int64_t K, int rows, void *q,
@@ -217,19 +236,7 @@ extern "C" int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, in
     const void *ptrs[] = {x, q, s};
     tpk_device_scope dev(ptrs, 3);
     if (!dev.ok()) return fail(dev.why);
-    const bool f16 = dtype == TPMD_DTYPE_F16;
-    const int es = f16 ? 2 : 4, vec = 16 / es;
-    // whole 16-byte loads and 4- or 8-byte stores where every row starts aligned for them
-    const bool al = !((uintptr_t) x & 15) && !((uintptr_t) q & (vec - 1)) &&
-                    (M == 1 || (ldx * es % 16 == 0 && ldq % vec == 0));
-    cudaStream_t st = (cudaStream_t) stream;
-    cudaError_t e;
-    if (f16)
-        e = al ? run_quant<__half, 8, true>(x, ldx, M, K, rows, q, ldq, s, lds, st)
-               : run_quant<__half, 8, false>(x, ldx, M, K, rows, q, ldq, s, lds, st);
-    else
-        e = al ? run_quant<float, 4, true>(x, ldx, M, K, rows, q, ldq, s, lds, st)
-               : run_quant<float, 4, false>(x, ldx, M, K, rows, q, ldq, s, lds, st);
+    const cudaError_t e = quant_f8(x, dtype == TPMD_DTYPE_F16, ldx, M, K, rows, q, ldq, s, lds, (cudaStream_t) stream, false);
     if (e == cudaErrorInvalidValue) return fail("too many blocks");
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;

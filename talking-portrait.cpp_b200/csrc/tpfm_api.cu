@@ -35,7 +35,8 @@ cudaError_t fmt_norm_mod(bool f16, float *x, int M, int H, float eps, const floa
 cudaError_t fmt_attn(bool f16, const float *qkv, int T, int H, int nh, int window, void *out, cudaStream_t st);
 cudaError_t fmt_res_norm(bool f16, float *x, const float *o, const float *mod, const float *bmod,
                          int mod_stride, int gate_off, int M, int H, float eps, const float *mod2, const float *bmod2,
-                         int shift_off, int scale_off, void *h, cudaStream_t st);
+                         int shift_off, int scale_off, void *h, cudaStream_t st,
+                         float *hs = nullptr);  // hs: h quantised to 8 bits, its scales in hs (H = 1024)
 cudaError_t fmt_cfg_euler(const float *vout, const float *bv, int T, int P, int D, float a_cfg, float e_cfg,
                           float dt, float *x, float *x60, __half *x60h, cudaStream_t st);
 cudaError_t fmt_add_bias(const float *a, const float *b, int M, int N, float *y, cudaStream_t st);
@@ -54,6 +55,7 @@ float ode_t(int i, int nfe) { return (float) ((double) i / (double) (nfe - 1)); 
 struct tpfm_ctx {
     int device = 0;
     bool f16 = false;
+    bool f8 = false;  // block and adaLN linears in 8 bits (and f16 set: the others in f16)
     tpfm_config c{};
     int T = 0, M = 0, CD = 0, CDp = 0, FF = 0, H = 0;  // CDp: CD padded to 8 (GEMM row strides)
     int nmod = 0;  // adaLN columns of all blocks + the final layer
@@ -63,8 +65,14 @@ struct tpfm_ctx {
     std::map<std::string, std::vector<float>> host;
     std::map<std::string, size_t> off32, off16;
     std::map<std::string, int> kdim, ldk;  // linear weights: K, and the row stride (K padded to 8)
+    std::map<std::string, size_t> off8, offs8;  // 8-bit weights: bytes, and their scales [ceil(N/128)][ceil(K/128)]
     float *w32 = nullptr;
     __half *w16 = nullptr;
+    uint8_t *w8 = nullptr;
+    float *ws8 = nullptr;
+    // 8-bit mode: a linear's quantised input rows and scales, the MLP's hidden rows and scales
+    uint8_t *x8 = nullptr, *m8 = nullptr;
+    float *xs8 = nullptr, *ms8 = nullptr;
     bool wready = false;
     cudaStream_t stream = nullptr;
     void *act = nullptr;
@@ -115,6 +123,37 @@ struct tpfm_ctx {
     bool gemm(const void *X, int Mr, int K, const std::string &wname, int N, float *Y, const float *bias = nullptr) {
         return gemm_w(X, Mr, K, K, Wt(wname), ldk.at(wname), N, Y, wname.c_str(), bias);
     }
+    // rows of K halves (the block's activations) into x8 / xs8
+    bool quant8(const void *X, int K, const char *what) {
+        return ck(quant_f8(X, true, K, M, K, 1, x8, K, xs8, (K + 127) / 128, stream, true), what);
+    }
+    // an 8-bit linear over all rows: Y (f32, or f16 when half_y), or quantised into m8 / ms8 when Y is null
+    bool gemm8(const uint8_t *X, const float *xs, int K, const std::string &wname, int N, void *Y, bool half_y,
+               const float *bias, int act) {
+        const int kb = (K + 127) / 128;
+        gemm_f8_desc d;
+        d.X = X;
+        d.ldx = K;
+        d.sx = xs;
+        d.ldsx = kb;
+        d.W = w8 + off8.at(wname);
+        d.ldw = K;
+        d.sw = ws8 + offs8.at(wname);
+        d.ldsw = kb;
+        d.Y = Y ? Y : m8;
+        d.ldy = N;
+        d.y_dtype = !Y ? TPMD_DTYPE_F8 : half_y ? TPMD_DTYPE_F16 : TPMD_DTYPE_F32;
+        d.sy = Y ? nullptr : ms8;
+        d.ldsy = (N + 127) / 128;
+        d.M = M;
+        d.N = N;
+        d.K = K;
+        d.bias = bias;
+        d.act = act;
+        d.err = gerr;
+        d.pdl = true;
+        return ck(gemm_f8(d, stream), wname.c_str());
+    }
     // after a synchronize: a GEMM whose pipeline wait expired
     bool gemm_status() {
         int flag = 0;
@@ -132,6 +171,8 @@ struct tpfm_ctx {
         if (act) cudaFree(act);
         if (w32) cudaFree(w32);
         if (w16) cudaFree(w16);
+        if (w8) cudaFree(w8);
+        if (ws8) cudaFree(ws8);
         if (stream) cudaStreamDestroy(stream);
     }
 };
@@ -167,6 +208,13 @@ void build_spec(tpfm_ctx *c) {
 bool is_gemm_weight(const std::string &n) {
     const size_t k = n.size();
     return k > 7 && n.compare(k - 7, 7, ".weight") == 0 && n.rfind("t_embedder.", 0) != 0;
+}
+
+// 8-bit mode: the weights kept in 8 bits (the block linears; the adaLN
+// modulations as one matrix, under the first one's name)
+bool is_f8_weight(const std::string &n) {
+    return is_gemm_weight(n) && (n.find(".attn.") != std::string::npos || n.find(".mlp.") != std::string::npos ||
+                                 n.find("adaLN_modulation") != std::string::npos);
 }
 
 // the timestep MLP of tf row `s` into te (two GEMVs)
@@ -234,7 +282,9 @@ bool forward_device(tpfm_ctx *c, int s, bool in_chunk = false) {
     }
     const int NM = c->nmod;
     if (!c->gemm(x60_in, T, c->c.dim_w, "x_embedder.proj.weight", H, c->x1) ||
-        !c->gemm_w(c->sc, M, H, H, c->adaln_w(), H, NM, c->mod, "adaLN modulation"))
+        !(c->f8 ? c->quant8(c->sc, H, "cond f8") && c->gemm8(c->x8, c->xs8, H, "blocks.0.adaLN_modulation.1.weight", NM,
+                                                            c->mod, false, nullptr, 0)
+                : c->gemm_w(c->sc, M, H, H, c->adaln_w(), H, NM, c->mod, "adaLN modulation")))
         return false;
     // each gated residual runs fused with the layer norm after it; the first
     // block's attention norm forms the embedded rows (x1 + bias + pos, three
@@ -244,6 +294,9 @@ bool forward_device(tpfm_ctx *c, int s, bool in_chunk = false) {
                         c->x1, c->F("x_embedder.proj.bias"), c->F("pos_embed"), T),
            "embed + norm"))
         return false;
+    // 8-bit mode: the norms quantise their rows themselves at the sampler's width
+    const bool f8 = c->f8, norm8 = f8 && H == 1024;
+    if (f8 && !c->quant8(c->h, H, "norm f8")) return false;
     for (int l = 0; l < c->c.depth; l++) {
         const std::string b = "blocks." + std::to_string(l) + ".";
         const float *bmod = c->F(b + "adaLN_modulation.1.bias");
@@ -254,6 +307,27 @@ bool forward_device(tpfm_ctx *c, int s, bool in_chunk = false) {
         const float *bmod2 = last ? c->F("decoder.adaLN_modulation.1.bias")
                                   : c->F("blocks." + std::to_string(l + 1) + ".adaLN_modulation.1.bias");
         const bool band = band_attention(c);
+        if (f8) {
+            const bool half_qkv = !band;
+            if (!c->gemm8(c->x8, c->xs8, H, b + "attn.qkv.weight", 3 * H, c->qkv, half_qkv, c->F(b + "attn.qkv.bias"), 0) ||
+                !(band ? K(fmt_attn(true, c->qkv, T, H, c->c.n_heads, c->c.attn_window, c->att, st), "attention")
+                       : wide_attention(c)) ||
+                !c->quant8(c->att, H, "attention f8") ||
+                !c->gemm8(c->x8, c->xs8, H, b + "attn.proj.weight", H, c->o, false, c->F(b + "attn.proj.bias"), 0) ||
+                !K(fmt_res_norm(true, c->x, c->o, md, bmod, NM, 2 * H, M, H, eps, md, bmod, 3 * H, 4 * H,
+                                norm8 ? (void *) c->x8 : c->h, st, norm8 ? c->xs8 : nullptr),
+                   "residual + norm") ||
+                (!norm8 && !c->quant8(c->h, H, "norm f8")) ||
+                !c->gemm8(c->x8, c->xs8, H, b + "mlp.fc1.weight", FF, nullptr, false, c->F(b + "mlp.fc1.bias"), 2) ||
+                !c->gemm8(c->m8, c->ms8, FF, b + "mlp.fc2.weight", H, c->o, false, c->F(b + "mlp.fc2.bias"), 0) ||
+                // (the final layer's linear takes f16)
+                !K(fmt_res_norm(true, c->x, c->o, md, bmod, NM, 5 * H, M, H, eps, md2, bmod2, 0, H,
+                                norm8 && !last ? (void *) c->x8 : c->h, st, norm8 && !last ? c->xs8 : nullptr),
+                   "residual + norm") ||
+                (!norm8 && !last && !c->quant8(c->h, H, "norm f8")))
+                return false;
+            continue;
+        }
         if (!c->gemm_w(c->h, M, H, H, c->Wt(b + "attn.qkv.weight"), c->ldk.at(b + "attn.qkv.weight"), 3 * H, c->qkv,
                        "attn.qkv", c->F(b + "attn.qkv.bias"), 0, h16 && !band ? (__half *) c->qkv : nullptr) ||
             !(band ? K(fmt_attn(h16, c->qkv, T, H, c->c.n_heads, c->c.attn_window, c->att, st), "attention")
@@ -303,7 +377,7 @@ void tpfm_default_config(tpfm_config *cfg) {
 
 tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
     int n = 0;
-    if (!cfg || (dtype != TPMD_DTYPE_F32 && dtype != TPMD_DTYPE_F16)) {
+    if (!cfg || (dtype != TPMD_DTYPE_F32 && dtype != TPMD_DTYPE_F16 && dtype != TPMD_DTYPE_F8)) {
         g_create_err = "tpfm_create: bad argument";
         return nullptr;
     }
@@ -312,6 +386,10 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
         cfg->t_freq_dim < 2 || cfg->t_freq_dim % 2 || cfg->dim_w <= 0 || cfg->dim_a < 0 || cfg->dim_e < 0 ||
         cfg->mlp_ratio <= 0.0f || cfg->dim_h % 8 || cfg->dim_w % 8 || (int) (cfg->dim_h * cfg->mlp_ratio) % 8) {
         g_create_err = "tpfm_create: invalid config";
+        return nullptr;
+    }
+    if (dtype == TPMD_DTYPE_F8 && (cfg->dim_h % 16 || (int) (cfg->dim_h * cfg->mlp_ratio) % 16)) {
+        g_create_err = "tpfm_create: 8-bit linears need dim_h and the MLP width in multiples of 16";
         return nullptr;
     }
     if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n) {
@@ -327,7 +405,8 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
     }
     tpfm_ctx *c = new tpfm_ctx();
     c->device = device;
-    c->f16 = dtype == TPMD_DTYPE_F16;
+    c->f8 = dtype == TPMD_DTYPE_F8;
+    c->f16 = dtype == TPMD_DTYPE_F16 || c->f8;
     c->c = *cfg;
     c->H = cfg->dim_h;
     c->T = cfg->chunk_frames + cfg->prev_frames;
@@ -344,7 +423,9 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
                       M * 3 * H * 4, M * H * 4, M * D * 4, M * D * 4,
                       (size_t) cfg->chunk_frames * D * 4, (size_t) (cfg->nfe) * cfg->t_freq_dim * 4,
                       (size_t) cfg->nfe * H * 4,
-                      M * H * es, M * H * es, M * H * es, M * FF * es, M * CD * es, T * D * es};
+                      M * H * es, M * H * es, M * H * es, M * FF * es, M * CD * es, T * D * es,
+                      c->f8 ? M * H : 0, c->f8 ? M * FF : 0, c->f8 ? M * ((H + 127) / 128) * 4 : 0,
+                      c->f8 ? M * ((FF + 127) / 128) * 4 : 0};
     const int ns = sizeof(sizes) / sizeof(sizes[0]);
     size_t offs[32], total = 0;
     for (int i = 0; i < ns; i++) {
@@ -370,6 +451,10 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
     for (float **p : fl) *p = (float *) (b + offs[i++]);
     void **vp[] = {&c->sc, &c->h, &c->att, &c->m1, &c->cond_in, &c->x60_in};
     for (void **p : vp) *p = b + offs[i++];
+    c->x8 = (uint8_t *) (b + offs[i++]);
+    c->m8 = (uint8_t *) (b + offs[i++]);
+    c->xs8 = (float *) (b + offs[i++]);
+    c->ms8 = (float *) (b + offs[i++]);
     // the t-embedding frequencies of every Euler step (host, as the reference)
     const int half = cfg->t_freq_dim / 2;
     std::vector<float> tf((size_t) cfg->nfe * cfg->t_freq_dim);
@@ -497,13 +582,37 @@ int tpfm_prepare(tpfm_ctx *c) {
         const size_t sz = stored(n);
         c->off32[n] = n32;
         n32 += sz;
-        if (c->f16 && is_gemm_weight(n)) {
+        if (c->f16 && is_gemm_weight(n) && !(c->f8 && is_f8_weight(n))) {
             c->off16[n] = n16;
             n16 += sz;
         }
         if (i + 1 >= n_adaln) {  // 256-byte aligned starts after the adaLN group
             n32 = (n32 + 63) & ~(size_t) 63;
             n16 = (n16 + 127) & ~(size_t) 127;
+        }
+    }
+    // 8-bit weights, each from a 128-byte boundary: rows, columns and first float
+    struct mat8 {
+        std::string name;
+        int64_t N, K;
+        size_t src;
+    };
+    std::vector<mat8> mats;
+    size_t n8 = 0, ns8 = 0;
+    c->off8.clear();
+    c->offs8.clear();
+    if (c->f8) {
+        mats.push_back({order[0], c->nmod, c->H, c->off32[order[0]]});
+        for (size_t i = n_adaln; i < order.size(); i++)
+            if (is_f8_weight(order[i])) {
+                const int64_t K = c->kdim.at(order[i]);
+                mats.push_back({order[i], c->spec.at(order[i]) / K, K, c->off32[order[i]]});
+            }
+        for (const mat8 &m : mats) {
+            c->off8[m.name] = n8;
+            c->offs8[m.name] = ns8;
+            n8 += ((size_t) (m.N * m.K) + 127) & ~(size_t) 127;
+            ns8 += (size_t) ((m.N + 127) / 128 * ((m.K + 127) / 128));
         }
     }
     std::vector<float> img(n32, 0.0f);
@@ -520,8 +629,12 @@ int tpfm_prepare(tpfm_ctx *c) {
     if (!c->ck(cudaSetDevice(c->device), "cudaSetDevice")) return -1;
     if (c->w32) cudaFree(c->w32);
     if (c->w16) cudaFree(c->w16);
+    if (c->w8) cudaFree(c->w8);
+    if (c->ws8) cudaFree(c->ws8);
     c->w32 = nullptr;
     c->w16 = nullptr;
+    c->w8 = nullptr;
+    c->ws8 = nullptr;
     if (c->graph) {
         cudaGraphExecDestroy(c->graph);
         c->graph = nullptr;
@@ -537,6 +650,17 @@ int tpfm_prepare(tpfm_ctx *c) {
                        "f16 weights"))
                 return -1;
         if (!c->ck(cudaStreamSynchronize(c->stream), "f16 weights")) return -1;
+    }
+    if (c->f8) {
+        if (!c->ck(cudaMalloc(&c->w8, n8), "cudaMalloc(fmt 8-bit weights)") ||
+            !c->ck(cudaMalloc(&c->ws8, ns8 * 4), "cudaMalloc(fmt weight scales)"))
+            return -1;
+        for (const mat8 &m : mats)
+            if (!c->ck(quant_f8(c->w32 + m.src, false, m.K, m.N, m.K, 128, c->w8 + c->off8[m.name], m.K,
+                                c->ws8 + c->offs8[m.name], (m.K + 127) / 128, c->stream, false),
+                       "8-bit weights"))
+                return -1;
+        if (!c->ck(cudaStreamSynchronize(c->stream), "8-bit weights")) return -1;
     }
     // the sampler's timestep embeddings depend only on the weights
     for (int s = 0; s + 1 < c->c.nfe; s++)

@@ -183,6 +183,33 @@ struct tpk_device_scope {
 // (nullptr and a CUDA error pending when it cannot be had)
 int *tpk_err_word();
 
+// tpk_quant_f8 without its checks (include/tpmd.h). pdl: launched as a
+// programmatic dependent (rows = 1 only)
+cudaError_t quant_f8(const void *x, bool f16, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
+                     int64_t lds, cudaStream_t st, bool pdl);
+// tpk_gemm_f8 without its checks
+struct gemm_f8_desc {
+    const void *X = nullptr;
+    int64_t ldx = 0;
+    const float *sx = nullptr;
+    int64_t ldsx = 0;
+    const void *W = nullptr;
+    int64_t ldw = 0;
+    const float *sw = nullptr;
+    int64_t ldsw = 0;
+    void *Y = nullptr;
+    int64_t ldy = 0;
+    int y_dtype = 0;  // TPMD_DTYPE_*
+    float *sy = nullptr;
+    int64_t ldsy = 0;
+    int M = 0, N = 0, K = 0;
+    const float *bias = nullptr;
+    int act = 0;
+    int *err = nullptr;  // set when a bounded wait expires (nullptr: tpk_device_status's word)
+    bool pdl = false;    // launched as a programmatic dependent
+};
+cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st);
+
 // Sliding-window attention (tpk_attn_window): lens clamped, left and right
 // within [0, 2^30]; strides {batch, token, head} in elements
 struct attn_desc {
