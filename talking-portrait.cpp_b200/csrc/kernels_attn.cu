@@ -281,8 +281,7 @@ cudaError_t run_tile(tile_params &p, cudaStream_t st) {
         keys = std::min<int64_t>(keys, cfg::BM / p.g + 2 + (int64_t) d.left + d.right + d.sinks);
     if (qtiles > INT32_MAX || bh * qtiles > INT32_MAX / 8) return cudaErrorInvalidValue;
     p.qtiles = (int) qtiles;
-    // a second CTA fits each SM: parts down to two tiles of keys
-    p.splits = (int) std::max<int64_t>(1, std::min<int64_t>({8, 2 * sm_count() / (bh * qtiles), (keys + 63) / 64}));
+    p.splits = cluster_size(bh * qtiles, (keys + 63) / 64);  // parts down to two tiles of keys
     static std::mutex mu;
     static uint64_t attr_set = 0;  // one bit per device
     int dev = 0;

@@ -864,7 +864,7 @@ cudaError_t launch_attn_tc(const attn_desc &d, cudaStream_t st) {
         int64_t keys = d.Tk;
         if (d.left >= 0 && d.right >= 0) keys = std::min<int64_t>(keys, (int64_t) p.tb + d.left + d.right + d.sinks);
         const int64_t tiles = (keys + 63) / 64, ctas = bh * p.qtiles;
-        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>({cluster_cap(ctas), sms / ctas, (tiles + 3) / 4}));
+        p.splits = cluster_size(ctas, (tiles + 3) / 4);
     }
     const int64_t ctas = bh * p.qtiles * p.splits;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;

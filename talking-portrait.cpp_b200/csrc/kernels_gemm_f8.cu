@@ -683,9 +683,7 @@ cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
     if (tiles > INT32_MAX / 8) return cudaErrorInvalidValue;
     p.tiles = (int) tiles;
     p.tiles_n = (int) ((nblk + nb - 1) / nb);
-    const int splits =
-        nb == 2 ? 1
-                : (int) std::max<int64_t>(1, std::min<int64_t>({cluster_cap(tiles), sm_count() / tiles, kblocks / 2}));
+    const int splits = nb == 2 ? 1 : cluster_size(tiles, kblocks / 2);
     p.kb_per_split = (kblocks + splits - 1) / splits;
     p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
     CUtensorMap tmX, tmW;

@@ -187,11 +187,17 @@ inline int sm_count() {
     return n;
 }
 
-// the largest cluster that `n` of them are launched with, for kernels with one
-// CTA an SM: a cluster lies within a GPC (16 to 18 SMs), so eight clusters of
-// eight always find room together, and as many of four as SMs; 16 clusters of
-// eight waited for one another (180x1024x4096 in 8 bits: 17.9 us, of four 9.9)
-inline int64_t cluster_cap(int64_t n) { return n <= 8 ? 8 : 4; }
+// CTAs a cluster when n clusters share work out, at most `most`, for kernels
+// with one CTA an SM: all n have to run at once. A cluster lies within a GPC
+// (16 to 18 SMs), so pairs use every SM, clusters of four 128 or so, and one
+// of eight a GPC is safe; sizes that do not divide a GPC's SMs leave some
+// idle. (In 8 bits, 180x1024x4096: 16 clusters of eight 17.9 us, of four 9.9;
+// 180x3072x1024: 48 of three 13.6 us, of two 8.4.)
+inline int cluster_size(int64_t n, int64_t most) {
+    if (most >= 8 && n <= 8) return 8;
+    if (most >= 4 && n <= 32) return 4;
+    return most >= 2 && 2 * n <= sm_count() ? 2 : 1;
+}
 
 }  // namespace
 }  // namespace tpmd
