@@ -168,6 +168,7 @@ struct f8_params {
     float *sy;
     int64_t ldsy;
     int act;
+    bool w_pre;  // W's first tiles load before the programmatic-dependence wait
     bool y_vec;  // Y takes stores of four elements (NB = 2: of 16 bytes)
     int *err;
 };
@@ -205,42 +206,19 @@ __device__ __noinline__ void copy_elements(uint8_t *y, const uint8_t *x, int n) 
         else y[i] = x[i];
     }
 }
-// four values of a row to Y columns n .. n + 3 (F8: quantised by s)
+// four values of a row to Y columns n .. n + 3 where these end, or start off a
+// vector's boundary (F8: quantised by s)
 template <int YT>
-__device__ __forceinline__ void store4(const f8_params &p, int64_t m, int n, const float (&v)[4], f8_scale s) {
-    if constexpr (YT == TPMD_DTYPE_F8) {
-        uint8_t *y = (uint8_t *) p.Y + m * p.ldy + n;
-        const uint32_t q = f8_quant4(v[0], v[1], v[2], v[3], s);
-        if (p.y_vec && n + 4 <= p.N) {
-            *reinterpret_cast<uint32_t *>(y) = q;
-        } else {
-#pragma unroll 1
-            for (int e = 0; e < 4; e++)
-                if (n + e < p.N) y[e] = (uint8_t) (q >> 8 * e);
+__device__ __noinline__ void store4(const f8_params &p, int64_t m, int n, float4 f, f8_scale s) {
+    const float v[4] = {f.x, f.y, f.z, f.w};
+    const uint32_t q = YT == TPMD_DTYPE_F8 ? f8_quant4(f.x, f.y, f.z, f.w, s) : 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < p.N) {
+            if constexpr (YT == TPMD_DTYPE_F8) ((uint8_t *) p.Y)[m * p.ldy + n + e] = (uint8_t) (q >> 8 * e);
+            else if constexpr (YT == TPMD_DTYPE_F16) ((__half *) p.Y)[m * p.ldy + n + e] = __float2half_rn(v[e]);
+            else ((float *) p.Y)[m * p.ldy + n + e] = v[e];
         }
-    } else if constexpr (YT == TPMD_DTYPE_F16) {
-        __half *y = (__half *) p.Y + m * p.ldy + n;
-        if (p.y_vec && n + 4 <= p.N) {
-            const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-            uint2 w;
-            w.x = *reinterpret_cast<const uint32_t *>(&a);
-            w.y = *reinterpret_cast<const uint32_t *>(&b);
-            *reinterpret_cast<uint2 *>(y) = w;
-        } else {
-#pragma unroll 1
-            for (int e = 0; e < 4; e++)
-                if (n + e < p.N) y[e] = __float2half_rn(e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]);
-        }
-    } else {
-        float *y = (float *) p.Y + m * p.ldy + n;
-        if (p.y_vec && n + 4 <= p.N) {
-            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll 1
-            for (int e = 0; e < 4; e++)
-                if (n + e < p.N) y[e] = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
-        }
-    }
 }
 
 // YT: TPMD_DTYPE_* of Y
@@ -249,7 +227,7 @@ __global__ void __launch_bounds__(f8_cfg<NB>::THREADS, 1)
 gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                const __grid_constant__ f8_params p) {
     using cfg = f8_cfg<NB>;
-    constexpr int ST = cfg::STAGES, NA = cfg::NACC;
+    constexpr int ST = cfg::STAGES, NA = cfg::NACC, ES = YT == TPMD_DTYPE_F32 ? 4 : YT == TPMD_DTYPE_F16 ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
     uint8_t *pieces = smem + ST * cfg::STAGE_BYTES;
@@ -302,6 +280,14 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         // block c - ST are done, which began after block c - ST - NA was read.
         // (a programmatic dependent starts while the kernel before it runs: all
         // that this one reads of it, and writes, comes after this wait)
+        // (but W, which a dependent's predecessor does not write)
+        const int pre = NB == 1 && p.w_pre ? min(nk, ST) : 0;
+        if (pre && elect_one())
+            for (int i = 0; i < pre; i++) {
+                mbar_expect_tx(full(i), cfg::STAGE_BYTES);
+                load_tile<NB>(B(i), &tmW, full(i), (kb0 + i) * cfg::KB, cta % p.tiles_n * cfg::BN);
+            }
+        __syncwarp();
         pdl_wait();
         pdl_trigger();
         int c = 0;
@@ -340,9 +326,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     }
                     if (lane == 0) {
                         // the bytes of both CTAs of a pair count on its first one's barrier
-                        if (rank == 0) mbar_expect_tx(full(s), cfg::STAGE_BYTES * NB);
+                        if (rank == 0 && c >= pre) mbar_expect_tx(full(s), cfg::STAGE_BYTES * NB);
                         load_tile<NB>(A(s), &tmX, full(s), (kb0 + i0 + e) * cfg::KB, m0);
-                        load_tile<NB>(B(s), &tmW, full(s), (kb0 + i0 + e) * cfg::KB, n0 + rank * 128);
+                        if (c >= pre) load_tile<NB>(B(s), &tmW, full(s), (kb0 + i0 + e) * cfg::KB, n0 + rank * 128);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; r++) fsx[f * cfg::BM + lane + 32 * r] = x[e][r];
@@ -465,14 +451,14 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     float top = 0.0f;
 #pragma unroll
                     for (int e = 0; e < CW; e++)
-                        if (n0 + e < p.N) top = fmaxf(top, fabsf(acc[e]));
+                        top = fmaxf(top, fabsf(acc[e]));  // (columns behind the last one: zeros or NaN)
                     k = f8_scale_of(top);
                     if (m0 + lane < p.M && n0 < p.N) p.sy[(int64_t) (m0 + lane) * p.ldsy + nb] = k.s;
                 }
                 // 64 bytes of each row at a time through shared memory, 16-byte
                 // unit u of row r at u ^ (r / 2 mod 4) against bank conflicts:
                 // a store covers eight rows
-                constexpr int ES = YT == TPMD_DTYPE_F32 ? 4 : YT == TPMD_DTYPE_F16 ? 2 : 1, PER = 16 / ES;
+                constexpr int PER = 16 / ES;
                 const int sub = lane / 4, unit = lane % 4;
                 uint8_t *y = (uint8_t *) p.Y + ((int64_t) (m0 + sub) * p.ldy + n0 + unit * PER) * ES;
                 const int64_t step = 8 * p.ldy * ES;
@@ -529,61 +515,83 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         float bias[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
-        // four rows a warp at a time, their loads in flight together
+        // four rows a warp at a time, three other CTAs' loads in flight together.
+        // (Columns behind the last one are zeros or NaN: they do not count in a
+        // row's maximum.)
         constexpr int RB = 4, NW = cfg::THREADS / 32;
         const int rows = min(cfg::BM, p.M - m0);
+        const bool vec4 = p.y_vec && n + 4 <= p.N;
 #pragma unroll 1
         for (int r0 = (split * NW + warp) * RB; r0 < rows; r0 += p.splits * NW * RB) {
             float4 v[RB];
 #pragma unroll
-            for (int j = 0; j < RB; j++) v[j] = make_float4(bias[0], bias[1], bias[2], bias[3]);
+            for (int j = 0; j < RB; j++) {
+                v[j] = *reinterpret_cast<const float4 *>((const float *) smem + (r0 + j) * cfg::PART_LD + lane * 4);
+                v[j] = make_float4(v[j].x + bias[0], v[j].y + bias[1], v[j].z + bias[2], v[j].w + bias[3]);
+            }
 #pragma unroll 1
-            for (int k0 = 0; k0 < p.splits; k0 += 2) {
-                float4 f[2][RB];
+            for (int k0 = 1; k0 < p.splits; k0 += 3) {
+                float4 f[3][RB];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    // every CTA starts with its own part: no two read one CTA's at a time
+                for (int k = 0; k < 3; k++) {
+                    // every CTA starts with the one after it: no two read one CTA's at a time
                     int from = split + k0 + k;
                     if (from >= p.splits) from -= p.splits;
 #pragma unroll
-                    for (int j = 0; j < RB; j++) {
-                        if (k0 + k >= p.splits) f[k][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        else if (p.splits > 1) f[k][j] = ld_rank4(part + (r0 + j) * cfg::PART_LD * 4, from);
-                        else f[k][j] = *reinterpret_cast<const float4 *>((const float *) smem + (r0 + j) * cfg::PART_LD + lane * 4);
-                    }
+                    for (int j = 0; j < RB; j++)
+                        if (k0 + k < p.splits) f[k][j] = ld_rank4(part + (r0 + j) * cfg::PART_LD * 4, from);
                 }
 #pragma unroll
-                for (int k = 0; k < 2; k++)
+                for (int k = 0; k < 3; k++)
 #pragma unroll
-                    for (int j = 0; j < RB; j++) {
-                        v[j].x += f[k][j].x;
-                        v[j].y += f[k][j].y;
-                        v[j].z += f[k][j].z;
-                        v[j].w += f[k][j].w;
-                    }
+                    for (int j = 0; j < RB; j++)
+                        if (k0 + k < p.splits) {
+                            v[j].x += f[k][j].x;
+                            v[j].y += f[k][j].y;
+                            v[j].z += f[k][j].z;
+                            v[j].w += f[k][j].w;
+                        }
+            }
+            if (p.act == 2) {
+#pragma unroll
+                for (int j = 0; j < RB; j++) v[j] = act4(v[j], 2);
+            } else if (p.act) {
+#pragma unroll
+                for (int j = 0; j < RB; j++) v[j] = act4(v[j], p.act);
             }
             float top[RB];
+            if constexpr (YT == TPMD_DTYPE_F8) {
 #pragma unroll
-            for (int j = 0; j < RB; j++) {
-                v[j] = act4(v[j], p.act);
-                top[j] = fmaxf(fmaxf(n < p.N ? fabsf(v[j].x) : 0.0f, n + 1 < p.N ? fabsf(v[j].y) : 0.0f),
-                               fmaxf(n + 2 < p.N ? fabsf(v[j].z) : 0.0f, n + 3 < p.N ? fabsf(v[j].w) : 0.0f));
-            }
-            if constexpr (YT == TPMD_DTYPE_F8)
+                for (int j = 0; j < RB; j++)
+                    top[j] = fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
 #pragma unroll
                 for (int w = 16; w > 0; w >>= 1)
 #pragma unroll
                     for (int j = 0; j < RB; j++) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], w));
+            }
+            const int64_t m = m0 + r0;
+            uint8_t *y = (uint8_t *) p.Y + (m * p.ldy + n) * ES;
+            const int64_t step = p.ldy * ES;
 #pragma unroll
             for (int j = 0; j < RB; j++) {
                 if (r0 + j >= rows) break;
                 f8_scale s = {1.0f, 1.0f};
                 if constexpr (YT == TPMD_DTYPE_F8) {
                     s = f8_scale_of(top[j]);
-                    if (lane == 0) p.sy[(int64_t) (m0 + r0 + j) * p.ldsy + n0 / 128] = s.s;
+                    if (lane == 0) p.sy[(m + j) * p.ldsy + n0 / 128] = s.s;
                 }
-                const float y[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-                if (n < p.N) store4<YT>(p, m0 + r0 + j, n, y, s);
+                if (vec4) {
+                    if constexpr (YT == TPMD_DTYPE_F8) {
+                        *reinterpret_cast<uint32_t *>(y + j * step) = f8_quant4(v[j].x, v[j].y, v[j].z, v[j].w, s);
+                    } else if constexpr (YT == TPMD_DTYPE_F16) {
+                        const __half2 h[2] = {__floats2half2_rn(v[j].x, v[j].y), __floats2half2_rn(v[j].z, v[j].w)};
+                        *reinterpret_cast<uint2 *>(y + j * step) = *reinterpret_cast<const uint2 *>(h);
+                    } else {
+                        *reinterpret_cast<float4 *>(y + j * step) = v[j];
+                    }
+                } else if (n < p.N) {
+                    store4<YT>(p, m + j, n, v[j], s);
+                }
             }
         }
         if (p.splits > 1) cluster_sync();  // no CTA leaves while others read its partial
@@ -669,6 +677,7 @@ cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
     p.sy = d.sy;
     p.ldsy = d.ldsy;
     p.act = d.act;
+    p.w_pre = d.pdl;
     p.err = d.err ? d.err : tpk_err_word();
     if (!p.err) return cudaErrorUnknown;
     const int es = d.y_dtype == TPMD_DTYPE_F32 ? 4 : d.y_dtype == TPMD_DTYPE_F16 ? 2 : 1;

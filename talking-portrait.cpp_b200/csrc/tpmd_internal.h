@@ -206,7 +206,7 @@ struct gemm_f8_desc {
     const float *bias = nullptr;
     int act = 0;
     int *err = nullptr;  // set when a bounded wait expires (nullptr: tpk_device_status's word)
-    bool pdl = false;    // launched as a programmatic dependent
+    bool pdl = false;    // launched as a programmatic dependent; W is not written by the kernels before it
 };
 cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st);
 
