@@ -36,8 +36,8 @@ typedef struct tpfm_ctx tpfm_ctx;
 
 /* dtype: TPMD_DTYPE_F32 (float32 GEMMs, no TF32), TPMD_DTYPE_F16 (f16
  * weights and GEMM inputs, float32 accumulation and everything else) or
- * TPMD_DTYPE_F8 (as F16, but the block linears and the adaLN modulations in
- * 8-bit floating point, tpk_quant_f8 and tpk_gemm_f8: half the weights' memory;
+ * TPMD_DTYPE_F8 (as F16, but the qkv and MLP linears and the adaLN modulations
+ * in 8-bit floating point, tpk_quant_f8 and tpk_gemm_f8: half their memory;
  * dim_h and the MLP width multiples of 16).
  * NULL on failure, reason in tpfm_create_error(). */
 tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg);

@@ -305,17 +305,30 @@ __global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ 
         const float sh[4] = {tv[j].x + bt.x, tv[j].y + bt.y, tv[j].z + bt.z, tv[j].w + bt.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = v[e] * sc[e] + v[e] + sh[e];
-        TIN *hp = h + (int64_t) m * H + 4 * q;
         if constexpr (std::is_same<TIN, uint8_t>::value) {
-            float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, w));
-            const f8_scale k = f8_scale_of(a);
-            *reinterpret_cast<uint32_t *>(hp) = f8_quant4(v[0], v[1], v[2], v[3], k);
-            if (lane == 0) hs[(int64_t) m * NV + j] = k.s;
+            xv[j] = make_float4(v[0], v[1], v[2], v[3]);
         } else {
+            TIN *hp = h + (int64_t) m * H + 4 * q;
 #pragma unroll
             for (int e = 0; e < 4; e++) hp[e] = cvt<TIN>(v[e]);
+        }
+    }
+    if constexpr (std::is_same<TIN, uint8_t>::value) {
+        // the groups' maxima, all of a step's shuffles in flight together
+        float a[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            a[j] = fmaxf(fmaxf(fabsf(xv[j].x), fabsf(xv[j].y)), fmaxf(fabsf(xv[j].z), fabsf(xv[j].w)));
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+            for (int j = 0; j < NV; j++) a[j] = fmaxf(a[j], __shfl_xor_sync(0xffffffffu, a[j], w));
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const f8_scale k = f8_scale_of(a[j]);
+            *reinterpret_cast<uint32_t *>(h + (int64_t) m * H + 4 * (lane + 32 * j)) =
+                f8_quant4(xv[j].x, xv[j].y, xv[j].z, xv[j].w, k);
+            if (lane == 0) hs[(int64_t) m * NV + j] = k.s;
         }
     }
 }

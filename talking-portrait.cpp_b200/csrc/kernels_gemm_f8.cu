@@ -464,7 +464,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 const int64_t step = 8 * p.ldy * ES;
                 const uint8_t *src = piece + sub * 64 + (unit ^ (sub >> 1 & 3)) * 16;  // (row + 8: the same unit)
                 uint8_t *own = piece + lane * 64;
-                const bool whole = p.y_vec && m0 + 32 <= p.M && n0 + CW <= p.N;
+                const bool whole = p.y_vec && n0 + CW <= p.N;
+                const int rows_left = p.M - m0 - sub;
 #pragma unroll
                 for (int x = 0; x < CW; x += 4 * PER) {
 #pragma unroll
@@ -491,12 +492,13 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 #pragma unroll
                         for (int r = 0; r < 4; r++) t[r] = *reinterpret_cast<const uint4 *>(src + r * 512);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) *reinterpret_cast<uint4 *>(y + r * step + x * ES) = t[r];
+                        for (int r = 0; r < 4; r++)
+                            if (r * 8 < rows_left) *reinterpret_cast<uint4 *>(y + r * step + x * ES) = t[r];
                     } else {
                         const int left = min(PER, p.N - n0 - x - unit * PER);
 #pragma unroll 1
                         for (int r = 0; r < 4; r++)
-                            if (m0 + sub + r * 8 < p.M && left > 0) copy_elements<ES>(y + r * step + x * ES, src + r * 512, left);
+                            if (r * 8 < rows_left && left > 0) copy_elements<ES>(y + r * step + x * ES, src + r * 512, left);
                     }
                     __syncwarp();
                 }

@@ -55,7 +55,7 @@ float ode_t(int i, int nfe) { return (float) ((double) i / (double) (nfe - 1)); 
 struct tpfm_ctx {
     int device = 0;
     bool f16 = false;
-    bool f8 = false;  // block and adaLN linears in 8 bits (and f16 set: the others in f16)
+    bool f8 = false;  // qkv, MLP and adaLN linears in 8 bits (and f16 set: the others in f16)
     tpfm_config c{};
     int T = 0, M = 0, CD = 0, CDp = 0, FF = 0, H = 0;  // CDp: CD padded to 8 (GEMM row strides)
     int nmod = 0;  // adaLN columns of all blocks + the final layer
@@ -210,10 +210,13 @@ bool is_gemm_weight(const std::string &n) {
     return k > 7 && n.compare(k - 7, 7, ".weight") == 0 && n.rfind("t_embedder.", 0) != 0;
 }
 
-// 8-bit mode: the weights kept in 8 bits (the block linears; the adaLN
-// modulations as one matrix, under the first one's name)
+// 8-bit mode: the weights kept in 8 bits, those of the linears whose input
+// the kernel before them quantises on its way (qkv and the MLP; the
+// attention's output stays f16 for proj: a launch to quantise it costs more
+// than the 8-bit product gains), and the adaLN modulations, as one matrix
+// under the first one's name
 bool is_f8_weight(const std::string &n) {
-    return is_gemm_weight(n) && (n.find(".attn.") != std::string::npos || n.find(".mlp.") != std::string::npos ||
+    return is_gemm_weight(n) && (n.find(".attn.qkv.") != std::string::npos || n.find(".mlp.") != std::string::npos ||
                                  n.find("adaLN_modulation") != std::string::npos);
 }
 
@@ -312,8 +315,7 @@ bool forward_device(tpfm_ctx *c, int s, bool in_chunk = false) {
             if (!c->gemm8(c->x8, c->xs8, H, b + "attn.qkv.weight", 3 * H, c->qkv, half_qkv, c->F(b + "attn.qkv.bias"), 0) ||
                 !(band ? K(fmt_attn(true, c->qkv, T, H, c->c.n_heads, c->c.attn_window, c->att, st), "attention")
                        : wide_attention(c)) ||
-                !c->quant8(c->att, H, "attention f8") ||
-                !c->gemm8(c->x8, c->xs8, H, b + "attn.proj.weight", H, c->o, false, c->F(b + "attn.proj.bias"), 0) ||
+                !c->gemm(c->att, M, H, b + "attn.proj.weight", H, c->o, c->F(b + "attn.proj.bias")) ||
                 !K(fmt_res_norm(true, c->x, c->o, md, bmod, NM, 2 * H, M, H, eps, md, bmod, 3 * H, 4 * H,
                                 norm8 ? (void *) c->x8 : c->h, st, norm8 ? c->xs8 : nullptr),
                    "residual + norm") ||
