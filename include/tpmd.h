@@ -353,7 +353,7 @@ int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, int64_t K, in
  *   Y[m][n] = act(sum_b sx[m][b] sw[n/128][b] (sum_{k in block b} X[m][k] W[n][k]) + bias[n])
  * m < M, n < N, k < K, blocks of 128 along k; the sums are f32 and each
  * block's sum is scaled and added in f32. Scales may be any float32 values. act as in
- * tpk_gemm (0 to 3); bias may be NULL. y_dtype: TPMD_DTYPE_F32, F16, or F8:
+ * tpk_gemm (0 to 3); bias may be NULL; M, N, K up to 2^30. y_dtype: TPMD_DTYPE_F32, F16, or F8:
  * Y is then quantised as by tpk_quant_f8 with rows = 1, its scales in sy
  * [M][ceil(N/128)] (row stride ldsy), which is NULL otherwise. X and W: 16-byte
  * aligned with row strides of multiples of 16 bytes; everything else any

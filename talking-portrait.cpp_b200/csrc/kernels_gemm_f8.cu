@@ -714,7 +714,7 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     auto fail = [](const char *m) { return tpk_fail(std::string("tpk_gemm_f8: ") + m); };
     if (y_dtype != TPMD_DTYPE_F32 && y_dtype != TPMD_DTYPE_F16 && y_dtype != TPMD_DTYPE_F8) return fail("y_dtype");
     if (act < 0 || act > 3) return fail("act");
-    if (M < 0 || N < 0 || K <= 0) return fail("bad shape");
+    if (M < 0 || N < 0 || K <= 0 || M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return fail("bad shape");
     if ((y_dtype == TPMD_DTYPE_F8) != (sy != nullptr) && M > 0 && N > 0) return fail("sy goes with an F8 Y, and only with it");
     if (M == 0 || N == 0) return 0;
     if (!X || !sx || !W || !sw || !Y) return fail("null pointer");

@@ -42,7 +42,7 @@ def _gemm(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(yd=3), "y_dtype"), (dict(act=4), "act"), (dict(act=-1), "act"), (dict(M=-1), "shape"), (dict(K=0), "shape"),
-    (dict(K=-5), "shape"), (dict(yd=2), "sy goes"), (dict(sy=P), "sy goes"), (dict(X=None), "null"),
+    (dict(K=-5), "shape"), (dict(M=(1 << 30) + 1), "shape"), (dict(N=(1 << 30) + 1, ldy=1 << 31), "shape"), (dict(yd=2), "sy goes"), (dict(sy=P), "sy goes"), (dict(X=None), "null"),
     (dict(W=None), "null"), (dict(sx=None), "null"), (dict(sw=None), "null"), (dict(Y=None), "null"),
     (dict(X=P + 8), "16-byte"), (dict(W=P + 1), "16-byte"), (dict(ldx=136), "16-byte"), (dict(ldw=129), "16-byte"),
     (dict(ldx=112), "row stride"), (dict(ldy=63), "row stride"), (dict(K=256, ldx=256, ldw=256), "row stride"),
