@@ -79,6 +79,8 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
     float *sq = (float *) smem4, *skv = sq + cfg::BM * LD, *sp = skv + 4 * cfg::KV;
     float2 *s_ml = (float2 *) (sp + cfg::BM * cfg::PLD);
     const attn_desc &d = p.d;
+    pdl_wait();
+    pdl_trigger();
     const int tid = threadIdx.x, kx = tid % 8, rg = tid / 8;
     int idx = blockIdx.x;
     const int rank = idx % p.splits;
@@ -300,13 +302,15 @@ cudaError_t run_tile(tile_params &p, cudaStream_t st) {
     lc.blockDim = dim3(128, 1, 1);
     lc.dynamicSmemBytes = cfg::SMEM;
     lc.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned) p.splits;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned) p.splits;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
     lc.attrs = at;
-    lc.numAttrs = p.splits > 1 ? 1 : 0;
+    lc.numAttrs = p.splits > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&lc, attn_tile_kernel<T, DC, RPT>, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }

@@ -230,6 +230,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const attn_desc &d = p.d;
+    pdl_wait();
+    pdl_trigger();
     // block -> (cluster rank,) batch and key head, query tile (the last ones,
     // which see most keys, first)
     int idx = blockIdx.x;
@@ -811,13 +813,15 @@ cudaError_t run_tc(const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtenso
     lc.blockDim = dim3(cfg::THREADS, 1, 1);
     lc.dynamicSmemBytes = cfg::SMEM;
     lc.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned) p.splits;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned) p.splits;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
     lc.attrs = at;
-    lc.numAttrs = p.splits > 1 ? 1 : 0;
+    lc.numAttrs = p.splits > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&lc, attn_tc_kernel<DB, SPLIT>, tmQ, tmK, tmV, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }

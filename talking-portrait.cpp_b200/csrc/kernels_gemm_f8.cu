@@ -280,7 +280,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         // block c - ST are done, which began after block c - ST - NA was read.
         // (a programmatic dependent starts while the kernel before it runs: all
         // that this one reads of it, and writes, comes after this wait)
-        // (but W, which a dependent's predecessor does not write)
+        // (but W, where that kernel does not write it)
         const int pre = NB == 1 && p.w_pre ? min(nk, ST) : 0;
         if (pre && elect_one())
             for (int i = 0; i < pre; i++) {
@@ -616,7 +616,7 @@ bool encode_bytes(CUtensorMap *tm, const void *base, int64_t cols, int64_t rows,
 }
 
 template <int YT, int NB>
-cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st, bool pdl) {
+cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
     using cfg = f8_cfg<NB>;
     static std::mutex mu;
     static uint64_t attr_set = 0;  // one bit per device
@@ -645,19 +645,17 @@ cudaError_t run_f8(const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_para
         at[na].val.clusterDim.z = 1;
         na++;
     }
-    if (pdl) {
-        at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[na].val.programmaticStreamSerializationAllowed = 1;
-        na++;
-    }
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na].val.programmaticStreamSerializationAllowed = 1;
+    na++;
     lc.attrs = at;
     lc.numAttrs = na;
     const cudaError_t e = cudaLaunchKernelEx(&lc, gemm_f8_kernel<YT, NB>, tmX, tmW, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 template <int YT>
-cudaError_t run_f8(int nb, const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st, bool pdl) {
-    return nb == 2 ? run_f8<YT, 2>(tmX, tmW, p, st, pdl) : run_f8<YT, 1>(tmX, tmW, p, st, pdl);
+cudaError_t run_f8(int nb, const CUtensorMap &tmX, const CUtensorMap &tmW, const f8_params &p, cudaStream_t st) {
+    return nb == 2 ? run_f8<YT, 2>(tmX, tmW, p, st) : run_f8<YT, 1>(tmX, tmW, p, st);
 }
 
 }  // namespace
@@ -679,7 +677,7 @@ cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
     p.sy = d.sy;
     p.ldsy = d.ldsy;
     p.act = d.act;
-    p.w_pre = d.pdl;
+    p.w_pre = d.w_const;
     p.err = d.err ? d.err : tpk_err_word();
     if (!p.err) return cudaErrorUnknown;
     const int es = d.y_dtype == TPMD_DTYPE_F32 ? 4 : d.y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
@@ -700,9 +698,9 @@ cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
     CUtensorMap tmX, tmW;
     if (!encode_bytes(&tmX, d.X, d.K, d.M, d.ldx, 128) || !encode_bytes(&tmW, d.W, d.K, d.N, d.ldw, 128))
         return cudaErrorInvalidValue;
-    return d.y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(nb, tmX, tmW, p, st, d.pdl)
-           : d.y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(nb, tmX, tmW, p, st, d.pdl)
-                                         : run_f8<TPMD_DTYPE_F8>(nb, tmX, tmW, p, st, d.pdl);
+    return d.y_dtype == TPMD_DTYPE_F32   ? run_f8<TPMD_DTYPE_F32>(nb, tmX, tmW, p, st)
+           : d.y_dtype == TPMD_DTYPE_F16 ? run_f8<TPMD_DTYPE_F16>(nb, tmX, tmW, p, st)
+                                         : run_f8<TPMD_DTYPE_F8>(nb, tmX, tmW, p, st);
 }
 
 }  // namespace tpmd

@@ -151,6 +151,8 @@ template <typename T, int VEC, bool ALIGNED>
 __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__ x, int64_t ldx, int64_t M, int64_t K,
                                                            int64_t kb, uint8_t *__restrict__ q, int64_t ldq,
                                                            float *__restrict__ s, int64_t lds) {
+    pdl_wait();
+    pdl_trigger();
     constexpr int LANES = 128 / VEC, ROWS = 256 / LANES, N = 128 / ROWS;
     __shared__ float red[8];
     const int64_t mb = blockIdx.x / kb, b = blockIdx.x % kb;
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__
 
 template <typename T, int VEC, bool ALIGNED>
 cudaError_t run_quant(const void *x, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
-                      int64_t lds, cudaStream_t st, bool pdl) {
+                      int64_t lds, cudaStream_t st) {
     const int64_t kb = (K + 127) / 128;
     if (rows == 1) {
         // loads in flight a lane: four where the blocks fill the SMs' warps all
@@ -187,11 +189,8 @@ cudaError_t run_quant(const void *x, int64_t ldx, int64_t M, int64_t K, int rows
         auto go = [&](auto kernel, int group) {
             const int64_t ctas = (M * ((kb + group - 1) / group) + 7) / 8;
             const dim3 grid((unsigned) std::min<int64_t>(ctas, 148 * 8));
-            if (pdl)
-                return launch_pdl(kernel, grid, dim3(256), 0, st, (const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s,
-                                  lds);
-            kernel<<<grid, 256, 0, st>>>((const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s, lds);
-            return cudaGetLastError();
+            return launch_pdl(kernel, grid, dim3(256), 0, st, (const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s,
+                              lds);
         };
         constexpr int PER = VEC / 4;  // blocks a load of a warp
         if (M * ((kb + 4 * PER - 1) / (4 * PER)) >= 148 * 64) return go(quant_rows_kernel<T, VEC, ALIGNED, 4>, 4 * PER);
@@ -199,24 +198,23 @@ cudaError_t run_quant(const void *x, int64_t ldx, int64_t M, int64_t K, int rows
     }
     const int64_t ctas = (M + 127) / 128 * kb;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-    quant_blocks_kernel<T, VEC, ALIGNED><<<(unsigned) ctas, 256, 0, st>>>((const T *) x, ldx, M, K, kb, (uint8_t *) q, ldq,
-                                                                         s, lds);
-    return cudaGetLastError();
+    return launch_pdl(quant_blocks_kernel<T, VEC, ALIGNED>, dim3((unsigned) ctas), dim3(256), 0, st, (const T *) x, ldx, M,
+                      K, kb, (uint8_t *) q, ldq, s, lds);
 }
 
 }  // namespace
 
 cudaError_t quant_f8(const void *x, bool f16, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
-                     int64_t lds, cudaStream_t st, bool pdl) {
+                     int64_t lds, cudaStream_t st) {
     const int es = f16 ? 2 : 4, vec = 16 / es;
     // whole 16-byte loads and 4- or 8-byte stores where every row starts aligned for them
     const bool al = !((uintptr_t) x & 15) && !((uintptr_t) q & (vec - 1)) &&
                     (M == 1 || (ldx * es % 16 == 0 && ldq % vec == 0));
     if (f16)
-        return al ? run_quant<__half, 8, true>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl)
-                  : run_quant<__half, 8, false>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl);
-    return al ? run_quant<float, 4, true>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl)
-              : run_quant<float, 4, false>(x, ldx, M, K, rows, q, ldq, s, lds, st, pdl);
+        return al ? run_quant<__half, 8, true>(x, ldx, M, K, rows, q, ldq, s, lds, st)
+                  : run_quant<__half, 8, false>(x, ldx, M, K, rows, q, ldq, s, lds, st);
+    return al ? run_quant<float, 4, true>(x, ldx, M, K, rows, q, ldq, s, lds, st)
+              : run_quant<float, 4, false>(x, ldx, M, K, rows, q, ldq, s, lds, st);
 }
 
 }  // namespace tpmd
@@ -236,7 +234,7 @@ extern "C" int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, in
     const void *ptrs[] = {x, q, s};
     tpk_device_scope dev(ptrs, 3);
     if (!dev.ok()) return fail(dev.why);
-    const cudaError_t e = quant_f8(x, dtype == TPMD_DTYPE_F16, ldx, M, K, rows, q, ldq, s, lds, (cudaStream_t) stream, false);
+    const cudaError_t e = quant_f8(x, dtype == TPMD_DTYPE_F16, ldx, M, K, rows, q, ldq, s, lds, (cudaStream_t) stream);
     if (e == cudaErrorInvalidValue) return fail("too many blocks");
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;

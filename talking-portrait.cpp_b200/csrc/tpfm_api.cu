@@ -125,7 +125,7 @@ struct tpfm_ctx {
     }
     // rows of K halves (the block's activations) into x8 / xs8
     bool quant8(const void *X, int K, const char *what) {
-        return ck(quant_f8(X, true, K, M, K, 1, x8, K, xs8, (K + 127) / 128, stream, true), what);
+        return ck(quant_f8(X, true, K, M, K, 1, x8, K, xs8, (K + 127) / 128, stream), what);
     }
     // an 8-bit linear over all rows: Y (f32, or f16 when half_y), or quantised into m8 / ms8 when Y is null
     bool gemm8(const uint8_t *X, const float *xs, int K, const std::string &wname, int N, void *Y, bool half_y,
@@ -151,7 +151,7 @@ struct tpfm_ctx {
         d.bias = bias;
         d.act = act;
         d.err = gerr;
-        d.pdl = true;
+        d.w_const = true;
         return ck(gemm_f8(d, stream), wname.c_str());
     }
     // after a synchronize: a GEMM whose pipeline wait expired
@@ -659,7 +659,7 @@ int tpfm_prepare(tpfm_ctx *c) {
             return -1;
         for (const mat8 &m : mats)
             if (!c->ck(quant_f8(c->w32 + m.src, false, m.K, m.N, m.K, 128, c->w8 + c->off8[m.name], m.K,
-                                c->ws8 + c->offs8[m.name], (m.K + 127) / 128, c->stream, false),
+                                c->ws8 + c->offs8[m.name], (m.K + 127) / 128, c->stream),
                        "8-bit weights"))
                 return -1;
         if (!c->ck(cudaStreamSynchronize(c->stream), "8-bit weights")) return -1;

@@ -183,11 +183,10 @@ struct tpk_device_scope {
 // (nullptr and a CUDA error pending when it cannot be had)
 int *tpk_err_word();
 
-// tpk_quant_f8 without its checks (include/tpmd.h). pdl: launched as a
-// programmatic dependent (rows = 1 only)
+// tpk_quant_f8, tpk_gemm_f8 and tpk_attn_window without their checks
+// (include/tpmd.h); all launch their kernels as programmatic dependents
 cudaError_t quant_f8(const void *x, bool f16, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq, float *s,
-                     int64_t lds, cudaStream_t st, bool pdl);
-// tpk_gemm_f8 without its checks
+                     int64_t lds, cudaStream_t st);
 struct gemm_f8_desc {
     const void *X = nullptr;
     int64_t ldx = 0;
@@ -206,11 +205,11 @@ struct gemm_f8_desc {
     const float *bias = nullptr;
     int act = 0;
     int *err = nullptr;  // set when a bounded wait expires (nullptr: tpk_device_status's word)
-    bool pdl = false;    // launched as a programmatic dependent; W is not written by the kernels before it
+    bool w_const = false;  // W is not written by the kernels before it: its first tiles load before the wait for them
 };
 cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st);
 
-// Sliding-window attention (tpk_attn_window): lens clamped, left and right
+// lens clamped, left and right
 // within [0, 2^30]; strides {batch, token, head} in elements
 struct attn_desc {
     const void *q, *k, *v;
