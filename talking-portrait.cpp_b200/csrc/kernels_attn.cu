@@ -10,8 +10,8 @@
 //
 // A CTA has 16 RPT rows (tokens times the query heads of a group, so that
 // these share a key head's tiles) and goes through the keys that any of them
-// sees, 32 at a time, with a running maximum and sum: the window from its
-// first key on, then the sinks. K and V tiles come by cp.async, one ahead.
+// sees, 32 at a time, with a running maximum and sum: one list of the sinks
+// and the window behind them. K and V tiles come by cp.async, one ahead.
 // Thread (rg, kx) = (tid / 8, tid % 8) has rows rg + 16 j: their scores with
 // keys kx + 8 i, then columns 4 kx + 32 i of their outputs (register tiles
 // of 4 x 4 RPT: the FMAs need one 16-byte shared load for every eight).
@@ -94,7 +94,9 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
     if (rows <= 0) return;  // (the whole cluster alike)
     const int64_t base = (int64_t) L - n;
     const key_range kr = keys_of(d, L, base + r0 / p.g, base + (r0 + rows - 1) / p.g);
-    const int nwin = (kr.hi - kr.lo + KT - 1) / KT, nall = nwin + (kr.first + KT - 1) / KT;
+    // the keys that some row sees, in one list: the sinks, then the window
+    const int keys = kr.first + kr.hi - kr.lo, nall = (keys + KT - 1) / KT;
+    auto key_at = [&](int i) { return i < kr.first ? i : i - kr.first + kr.lo; };
     const int i0 = (int) ((int64_t) nall * rank / p.splits), i1 = (int) ((int64_t) nall * (rank + 1) / p.splits);
     const T *kbase = (const T *) d.k + b * d.ks[0] + hk * d.ks[2], *vbase = (const T *) d.v + b * d.vs[0] + hk * d.vs[2];
 
@@ -107,13 +109,13 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
         }
         *reinterpret_cast<float4 *>(sq + r * LD + x) = make_float4(f.x * p.c, f.y * p.c, f.z * p.c, f.w * p.c);
     }
-    // tile i of the keys into buffer i & 1; keys that no row sees are zeros
+    // tile i of the list into buffer i & 1, zeros behind its end
     auto load = [&](int i) {
-        const int kb = i < nwin ? kr.lo + i * KT : (i - nwin) * KT, end = i < nwin ? kr.hi : kr.first;
         float *k = skv + (i & 1) * 2 * cfg::KV, *v = k + cfg::KV;
         for (int e = tid; e < KT * DC * 8; e += 128) {
-            const int r = e / (DC * 8), x = e % (DC * 8) * 4, left = kb + r < end ? d.D - x : 0;
-            const T *ks = kbase + (int64_t) (kb + r) * d.ks[1] + x, *vs = vbase + (int64_t) (kb + r) * d.vs[1] + x;
+            const int r = e / (DC * 8), x = e % (DC * 8) * 4, left = i * KT + r < keys ? d.D - x : 0;
+            const int64_t key = key_at(i * KT + r);
+            const T *ks = kbase + key * d.ks[1] + x, *vs = vbase + key * d.vs[1] + x;
             if (sizeof(T) == 4 && p.kv_vec && (left >= 4 || left <= 0)) {
                 const int bytes = left > 0 ? 16 : 0;  // 0: zeros, nothing is read
                 if (!bytes) {
@@ -156,7 +158,7 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
         }
         __syncthreads();
         const float *k = skv + (i & 1) * 2 * cfg::KV, *v = k + cfg::KV;
-        const int kb = i < nwin ? kr.lo + i * KT : (i - nwin) * KT;
+        const int here = min(KT, keys - i * KT);  // keys of the tile
         float s[RPT][4];
 #pragma unroll
         for (int j = 0; j < RPT; j++)
@@ -176,14 +178,11 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
         }
 #pragma unroll
         for (int j = 0; j < RPT; j++) {
-            // window tiles: [lo, hi) and what lies below sinks; the sinks' tiles: [0, first) below hi
-            const int a0 = i < nwin ? kk[j].lo : 0, a1 = i < nwin ? kk[j].hi : min(kr.first, kk[j].hi);
-            const int a2 = i < nwin ? min(d.sinks, kk[j].hi) : 0;
             float mn = m[j];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int key = kb + kx + 8 * e;
-                if (!(key >= a0 && key < a1 || key < a2)) s[j][e] = -INFINITY;
+                const int at = kx + 8 * e, key = key_at(i * KT + at);
+                if (!(at < here && key < kk[j].hi && (key >= kk[j].lo || key < d.sinks))) s[j][e] = -INFINITY;
                 mn = fmaxf(mn, s[j][e]);
             }
 #pragma unroll
@@ -207,7 +206,7 @@ attn_tile_kernel(const __grid_constant__ tile_params p) {
         }
         __syncwarp();  // (a row's weights are written and read by one warp)
 #pragma unroll 2
-        for (int key = 0; key < KT; key += 4) {
+        for (int key = 0; key < here; key += 4) {  // (weights behind the list's end are zeros, and so are the values)
             float4 w[RPT];
 #pragma unroll
             for (int j = 0; j < RPT; j++)

@@ -192,7 +192,7 @@ inline int sm_count() {
 // (16 to 18 SMs), so pairs use every SM, clusters of four 128 or so, and one
 // of eight a GPC is safe; sizes that do not divide a GPC's SMs leave some
 // idle. (In 8 bits, 180x1024x4096: 16 clusters of eight 17.9 us, of four 9.9;
-// 180x3072x1024: 48 of three 13.6 us, of two 8.4.)
+// 48 clusters of three 13.6 us, of two 8.4.)
 inline int cluster_size(int64_t n, int64_t most) {
     if (most >= 8 && n <= 8) return 8;
     if (most >= 4 && n <= 32) return 4;
