@@ -384,6 +384,15 @@ int tpk_attn_window(const void *q, const void *k, const void *v, void *out, cons
                     int B, int Tq, int Tk, int Hq, int Hkv, int D, const int32_t *q_len, const int32_t *kv_len,
                     int left, int right, int sinks, float scale, void *stream);
 
+/* The three calls above with their arguments in one block, for callers whose
+ * foreign calls cost by the argument (through ctypes a call of 19 arguments
+ * takes longer than a small kernel): in the same order, 8 bytes each, pointers
+ * (0: NULL) and integers as int64_t, tpk_attn_window's twelve strides in their
+ * place and its scale as a double. The block is read before they return. */
+int tpk_quant_f8_packed(const int64_t args[11]);
+int tpk_gemm_f8_packed(const int64_t args[19]);
+int tpk_attn_window_packed(const int64_t args[30]);
+
 /* Synchronises `stream` (a stream of the current device), then reads and
  * clears the device's expired-wait word of tpk_gemm_f8 and tpk_attn_window.
  * 0 when no wait expired since the last query, else -1 with the message in

@@ -674,3 +674,19 @@ extern "C" int tpk_attn_window(const void *q, const void *k, const void *v, void
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;
 }
+
+extern "C" int tpk_attn_window_packed(const int64_t args[30]) {
+    tpmd::packed_args p{args};
+    const void *q = p.ptr(), *k = p.ptr(), *v = p.ptr();
+    void *out = p.ptr();
+    const int64_t *strides = p.a;
+    p.a += 12;
+    const int dtype = p.i32(), B = p.i32(), Tq = p.i32(), Tk = p.i32(), Hq = p.i32(), Hkv = p.i32(), D = p.i32();
+    const int32_t *q_len = (const int32_t *) p.ptr(), *kv_len = (const int32_t *) p.ptr();
+    const int left = p.i32(), right = p.i32(), sinks = p.i32();
+    const float scale = (float) p.f64();
+    void *stream = p.ptr();
+    if (!p.fits) return tpmd::tpk_fail("tpk_attn_window: an argument is out of its range");
+    return tpk_attn_window(q, k, v, out, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_len, kv_len, left, right, sinks,
+                           scale, stream);
+}

@@ -757,3 +757,26 @@ extern "C" int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t 
     }
     return 0;
 }
+
+extern "C" int tpk_gemm_f8_packed(const int64_t args[19]) {
+    tpmd::packed_args p{args};
+    const void *X = p.ptr();
+    const int64_t ldx = p.i64();
+    const float *sx = (const float *) p.ptr();
+    const int64_t ldsx = p.i64();
+    const void *W = p.ptr();
+    const int64_t ldw = p.i64();
+    const float *sw = (const float *) p.ptr();
+    const int64_t ldsw = p.i64();
+    void *Y = p.ptr();
+    const int64_t ldy = p.i64();
+    const int y_dtype = p.i32();
+    float *sy = (float *) p.ptr();
+    const int64_t ldsy = p.i64();
+    const int M = p.i32(), N = p.i32(), K = p.i32();
+    const float *bias = (const float *) p.ptr();
+    const int act = p.i32();
+    void *stream = p.ptr();
+    if (!p.fits) return tpmd::tpk_fail("tpk_gemm_f8: an argument is out of its range");
+    return tpk_gemm_f8(X, ldx, sx, ldsx, W, ldw, sw, ldsw, Y, ldy, y_dtype, sy, ldsy, M, N, K, bias, act, stream);
+}

@@ -239,3 +239,18 @@ extern "C" int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, in
     if (e != cudaSuccess) return fail(cudaGetErrorString(e));
     return 0;
 }
+
+extern "C" int tpk_quant_f8_packed(const int64_t args[11]) {
+    tpmd::packed_args p{args};
+    const void *x = p.ptr();
+    const int dtype = p.i32();
+    const int64_t ldx = p.i64(), M = p.i64(), K = p.i64();
+    const int rows = p.i32();
+    void *q = p.ptr();
+    const int64_t ldq = p.i64();
+    float *s = (float *) p.ptr();
+    const int64_t lds = p.i64();
+    void *stream = p.ptr();
+    if (!p.fits) return tpmd::tpk_fail("tpk_quant_f8: an argument is out of its range");
+    return tpk_quant_f8(x, dtype, ldx, M, K, rows, q, ldq, s, lds, stream);
+}

@@ -2,6 +2,7 @@
 // (tpmd_api.cpp) and its CUDA kernels. Not installed.
 #pragma once
 
+#include <cstring>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -178,6 +179,22 @@ struct tpk_device_scope {
 
   private:
     int prev_ = -1;
+};
+// the arguments of a packed call (include/tpmd.h), in order
+struct packed_args {
+    const int64_t *a;
+    bool fits = true;  // every int so far was one
+    void *ptr() { return (void *) (uintptr_t) *a++; }
+    int64_t i64() { return *a++; }
+    int i32() {
+        fits = fits && *a == (int) *a;
+        return (int) *a++;
+    }
+    double f64() {
+        double v;
+        memcpy(&v, a++, sizeof v);
+        return v;
+    }
 };
 // the current device's expired-wait word that tpk_device_status reads
 // (nullptr and a CUDA error pending when it cannot be had)

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -53,7 +54,8 @@ EXPORTS = ("tpmd_abi_version", "tpmd_create", "tpmd_create_error", "tpmd_destroy
            "tpmd_group_set_feats", "tpmd_group_set_feats_device", "tpmd_shard_range", "tpmd_group_decode",
            "tpmd_group_max", "tpmd_group_selftest_nccl", "tpmd_decode_rgb24", "tpmd_group_decode_rgb24",
            "tpk_chw_to_rgb24", "tpk_gemm", "tpmd_decode_schedule",
-           "tpfm_set_sinks", "tpk_quant_f8", "tpk_gemm_f8", "tpk_attn_window", "tpk_device_status")
+           "tpfm_set_sinks", "tpk_quant_f8", "tpk_gemm_f8", "tpk_attn_window", "tpk_quant_f8_packed",
+           "tpk_gemm_f8_packed", "tpk_attn_window_packed", "tpk_device_status")
 
 _lib = None
 
@@ -127,6 +129,8 @@ def load_library(path: str = LIB_PATH):
     L.tpk_gemm_f8.argtypes = [v, i64, v, i64, v, i64, v, i64, v, i64, C.c_int, v, i64, C.c_int, C.c_int, C.c_int, v,
                               C.c_int, v]
     L.tpk_attn_window.argtypes = [v, v, v, v, C.POINTER(i64)] + [C.c_int] * 7 + [v, v] + [C.c_int] * 3 + [C.c_float, v]
+    for f in (L.tpk_quant_f8_packed, L.tpk_gemm_f8_packed, L.tpk_attn_window_packed):
+        f.argtypes = [cp]
     L.tpk_device_status.argtypes = [v]
     L.tpmd_group_selftest_nccl.argtypes = [C.c_int, C.c_int, C.c_double, C.POINTER(C.c_int), C.c_char_p,
                                            C.c_size_t]
@@ -463,12 +467,22 @@ def _f8_dtypes():
     return _dtypes
 
 
-def _rows(shape, stride):
+def _row_stride(t):
     """The row stride of a matrix whose rows are contiguous, else None (the
     calls below take microseconds: their checks touch each tensor little)"""
-    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+    rows, cols = t.shape
+    if t.is_contiguous():
+        return cols
+    a, b = t.stride()
+    if b != 1 and cols > 1:
         return None
-    return stride[0] if shape[0] > 1 else max(shape[1], stride[0])
+    return a if rows > 1 else max(cols, a)
+
+
+# the arguments of the ops' packed forms (include/tpmd.h)
+_pack_quant = struct.Struct("11q").pack
+_pack_gemm = struct.Struct("19q").pack
+_pack_attn = struct.Struct("28qdq").pack
 
 
 def quant_f8(x, q, s, rows=1, stream=0):
@@ -484,11 +498,14 @@ def quant_f8(x, q, s, rows=1, stream=0):
         raise TpmdError("quant_f8: x must be float16 or float32, q float8_e4m3fn, s float32")
     if len(shape) != 2 or q.shape != shape or s.shape != (-(-shape[0] // rows), -(-shape[1] // 128)):
         raise TpmdError("quant_f8: q must have x's shape [M, K], s one element per block")
-    ldx, ldq, lds = _rows(shape, x.stride()), _rows(shape, q.stride()), _rows(s.shape, s.stride())
+    M, K = shape
+    ldx = K if x.is_contiguous() else _row_stride(x)
+    ldq = K if q.is_contiguous() else _row_stride(q)
+    lds = _row_stride(s)
     if ldx is None or ldq is None or lds is None:
         raise TpmdError("quant_f8: the rows of x, q and s must be contiguous")
-    if load_library().tpk_quant_f8(x.data_ptr(), 1 if dt is f16 else 0, ldx, shape[0], shape[1], rows, q.data_ptr(),
-                                   ldq, s.data_ptr(), lds, stream) != 0:
+    if load_library().tpk_quant_f8_packed(_pack_quant(
+            x.data_ptr(), 1 if dt is f16 else 0, ldx, M, K, rows, q.data_ptr(), ldq, s.data_ptr(), lds, stream or 0)) != 0:
         _tpk_check(-1)
     return q, s
 
@@ -515,22 +532,23 @@ def gemm_f8(X, sx, W, sw, Y, sy=None, bias=None, act=0, stream=0):
         raise TpmdError("gemm_f8: Y must be [M, N], sx [M, ceil(K / 128)], sw [ceil(N / 128), ceil(K / 128)]")
     if bias is not None and (bias.dtype is not f32 or bias.shape != (N,) or not bias.is_contiguous()):
         raise TpmdError("gemm_f8: bias must be contiguous float32 [N]")
-    lds = [_rows(t.shape, t.stride()) for t in (X, sx, W, sw, Y)]
-    syp, ldsy, yd = None, 0, 1 if yt is f16 else 0
+    ldx = K if X.is_contiguous() else _row_stride(X)
+    ldsx = kb if sx.is_contiguous() else _row_stride(sx)
+    ldw = K if W.is_contiguous() else _row_stride(W)
+    ldsw = kb if sw.is_contiguous() else _row_stride(sw)
+    ldy = N if Y.is_contiguous() else _row_stride(Y)
+    syp, ldsy, yd = 0, 0, 1 if yt is f16 else 0
     if sy is not None:
         if sy.dtype is not f32 or sy.shape != (M, nb):
             raise TpmdError("gemm_f8: sy must be float32 [M, ceil(N / 128)]")
-        syp, ldsy, yd = sy.data_ptr(), _rows(sy.shape, sy.stride()), DTYPE_F8
-    if None in lds or ldsy is None:
+        syp, ldsy, yd = sy.data_ptr(), _row_stride(sy), DTYPE_F8
+    if ldx is None or ldsx is None or ldw is None or ldsw is None or ldy is None or ldsy is None:
         raise TpmdError("gemm_f8: the rows of X, W, Y and the scales must be contiguous")
-    if load_library().tpk_gemm_f8(X.data_ptr(), lds[0], sx.data_ptr(), lds[1], W.data_ptr(), lds[2], sw.data_ptr(),
-                                  lds[3], Y.data_ptr(), lds[4], yd, syp, ldsy, M, N, K,
-                                  None if bias is None else bias.data_ptr(), act, stream) != 0:
+    if load_library().tpk_gemm_f8_packed(_pack_gemm(
+            X.data_ptr(), ldx, sx.data_ptr(), ldsx, W.data_ptr(), ldw, sw.data_ptr(), ldsw, Y.data_ptr(), ldy, yd, syp,
+            ldsy, M, N, K, 0 if bias is None else bias.data_ptr(), act, stream or 0)) != 0:
         _tpk_check(-1)
     return Y
-
-
-_strides12 = C.c_int64 * 12
 
 
 def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv_len=None, stream=0):
@@ -553,12 +571,11 @@ def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv
     for t in (q_len, kv_len):
         if t is not None and (t.dtype is not i32 or t.shape != (B,) or not t.is_contiguous()):
             raise TpmdError("attn_window: q_len and kv_len must be contiguous int32 [B]")
-    st = _strides12(a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2], o[0], o[1], o[2])
-    if load_library().tpk_attn_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st,
-                                      1 if dt is f16 else 0, B, Tq, Tk, Hq, Hkv, D,
-                                      None if q_len is None else q_len.data_ptr(),
-                                      None if kv_len is None else kv_len.data_ptr(), left, right, sinks,
-                                      D ** -0.5 if scale is None else scale, stream) != 0:
+    if load_library().tpk_attn_window_packed(_pack_attn(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1],
+            c[2], o[0], o[1], o[2], 1 if dt is f16 else 0, B, Tq, Tk, Hq, Hkv, D,
+            0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(), left, right, sinks,
+            D ** -0.5 if scale is None else scale, stream or 0)) != 0:
         _tpk_check(-1)
     return out
 

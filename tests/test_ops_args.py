@@ -4,6 +4,7 @@ the pointers are host addresses that no accepted call would read)."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import pytest
 import torch
@@ -110,3 +111,33 @@ def test_binding_refuses():
                 dict(q=torch.zeros(2, 3, 8, 4).transpose(2, 3))):
         with pytest.raises(tpmd.TpmdError):
             tpmd.attn_window(**{**a, **bad})
+
+
+def _words(args):
+    """Arguments as a packed call takes them: 8 bytes each, strides in their place"""
+    w = []
+    for a in args:
+        if isinstance(a, float):
+            w.append(struct.pack("d", a))
+        else:
+            w += [struct.pack("q", x or 0) for x in (a if isinstance(a, tuple) else (a,))]
+    return b"".join(w)
+
+
+@pytest.mark.parametrize("name,args,msg", [
+    ("quant_f8", (P, 0, 128, 4, 128, 64, P, 128, P, 1, None), "rows"),
+    ("quant_f8", (P, 0, 128, 4, 128, 1, P, 128, P + 1, 1, None), "element type"),
+    ("quant_f8", (P, 0, 128, 4, 128, 1, P, 127, P, 1, None), "row stride"),
+    ("quant_f8", (P, 0, 128, 4, 128, 1 << 32 | 1, P, 128, P, 1, None), "range"),
+    ("gemm_f8", (P, 128, P, 1, P, 128, P, 1, P, 64, 0, None, 0, 4, 64, 128, None, 4, None), "act"),
+    ("gemm_f8", (P, 128, P, 1, P, 128, P, 1, P, 64, 0, None, 0, 4, 64, 128, P + 1, 0, None), "element type"),
+    ("gemm_f8", (P, 128, P, 1, P, 128, P, 1, P, 64, 0, None, 0, 1 << 32 | 4, 64, 128, None, 0, None), "range"),
+    ("attn_window", (P, P, P, P, (512, 128, 64) * 4, 1, 1, 4, 4, 2, 2, 64, None, P + 1, 1, 0, 0, 0.125, None), "element type"),
+    ("attn_window", (P, P, P, P, (512, 128, 64) * 4, 1, 1, 4, 4, 2, 2, 64, None, None, 1, 0, -1, 0.125, None), "sinks"),
+    ("attn_window", (P, P, P, P, (512, 128, 64) * 4, 1, 1, 4, 4, 2, 2, 64, None, None, 1, 0, 0, float("inf"), None), "scale"),
+    ("attn_window", (P, P, P, P, (512, 128, 64) * 3 + (512, 64, 64), 1, 1, 4, 4, 2, 2, 64, None, None, 1, 0, 0, 0.125, None), "overlap"),
+    ("attn_window", (P, P, P, P, (512, 128, 64) * 4, 1, 1, 4, 4, 2, 2, 64, None, None, 1 << 31, 0, 0, 0.125, None), "range")])
+def test_packed_calls_refuse_alike(name, args, msg):
+    """Each word reaches the argument of its place: the last ones of a kind are the bad ones here"""
+    assert getattr(tpmd.load_library(), f"tpk_{name}_packed")(_words(args)) == -1
+    assert msg in _err() and f"tpk_{name}:" in _err()
