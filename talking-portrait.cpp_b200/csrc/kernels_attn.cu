@@ -9,26 +9,25 @@
 //   p = L - n + i
 //
 // Rows are tokens times the query heads of a group, so that these share a key
-// head's tiles; the keys that any row of a CTA sees are one list, the sinks
-// and the window behind them, in tiles with a running maximum and sum. K and
-// V tiles come by cp.async. Two kernels:
+// head's tiles. A CTA has up to 16; the keys that any of them sees are one
+// list, the sinks and the window behind them. Every warp has all the rows and
+// its own share of that list, in tiles of 8 keys with a running maximum and
+// sum, K and V by cp.async two tiles ahead, and waits for nothing but its
+// copies. Lane (rg, kx) = (lane / 8, lane % 8) holds columns 4 kx + 32 i of
+// rows rg + 4 j and of their outputs in registers: eight lanes sum a row's
+// scores over their columns, key kx's to lane kx, and each 16-byte shared
+// load of K or V feeds R rows. The warps' parts join in shared memory; where
+// CTAs do not fill the SMs a cluster of up to eight shares the list and joins
+// over distributed shared memory; always in the same order.
 //
-//  * attn_tile_kernel, many rows: 64 a CTA, tiles of 32 keys, one ahead.
-//    Thread (rg, kx) = (tid / 8, tid % 8) has rows rg + 16 j: their scores
-//    with keys kx + 8 i, then columns 4 kx + 32 i of their outputs (register
-//    tiles of 4 x 4 RPT). Bound by shared-memory reads and FMAs alike, half
-//    of either's rate with the eight warps that fit an SM: 30 TFLOP/s (4096
-//    tokens, 16 heads of 128 on 4, 1024 keys each, 1.02 ms).
-//  * attn_rows_kernel, few rows: up to 16 a CTA. Every warp has all rows and
-//    its own share of the keys, its own tiles (8 keys, K and V two ahead) and
-//    nothing to wait for but its copies; lane (rg, kx) as above with rows
-//    rg + 4 j. The warps' parts join in shared memory, and where CTAs do not
-//    fill the SMs a cluster of up to eight shares the keys and joins over
-//    distributed shared memory; always in the same order. Bound by the
-//    latency of shared-memory reads: 268 MB of cache in 73 us, 3.7 TB/s (16
-//    sequences of one token, 16 heads of 128 on 4, 4100 keys); the sampler's
-//    60 frames of 3 x 8 heads over 5 + 10 keys in 9.4 us, 2.5 of them a
-//    launch.
+// Measured: 16 sequences of one token over 4100 keys, 16 heads of 128 on 4:
+// 58 us, 4.6 TB/s (latency of the shared loads with eight warps an SM; tiles
+// of 64 rows with all threads in step took 241 us). 4096 tokens, 16 heads of
+// 128 on 4, 1024 keys each: 1.04 ms, 32 TFLOP/s (the same eight warps:
+// registers; tiles of 64 rows 0.91 ms, but 173 us against 117 at 3000 tokens
+// of 8 heads, 200 keys, where whole tiles of 64 do not share out evenly). The
+// sampler's 60 frames of 3 x 8 heads over 5 + 10 keys: 9.6 us, of which a
+// launch is 2.5.
 //
 // Values of keys that no row sees load as zeros; a row that comes out not
 // finite is computed again from its visible keys alone (a weight of zero
@@ -48,7 +47,7 @@
 namespace tpmd {
 namespace {
 
-struct tile_params {
+struct rows_params {
     attn_desc d;
     int g, qtiles, splits;
     float c;  // scale log2(e)
@@ -68,9 +67,6 @@ __device__ __forceinline__ float4 load4(const __half *x, int n, bool vec) {
     }
     return make_float4(n > 0 ? __half2float(x[0]) : 0.0f, n > 1 ? __half2float(x[1]) : 0.0f,
                        n > 2 ? __half2float(x[2]) : 0.0f, n > 3 ? __half2float(x[3]) : 0.0f);
-}
-__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
-    return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s))));
 }
 
 // the sum of n parts of a row, each relative to its own maximum, relative to
@@ -92,10 +88,10 @@ __device__ __forceinline__ float2 join_parts(int n, ML ml, V part, float (&v)[DC
 }
 // row (token, head of the group) `row` of the outputs from its sums
 template <typename T, int DC>
-__device__ __forceinline__ void store_row(const tile_params &p, int b, int hk, int64_t row, int n, int L, float sl,
+__device__ __forceinline__ void store_row(const rows_params &p, int b, int hk, int64_t row, int n, int L, float sl,
                                           const float (&v)[DC], int lane) {
     const attn_desc &d = p.d;
-    const int tok = (int) (row / p.g), h = hk * p.g + (int) (row % p.g);
+    const int tok = (int) ((uint32_t) row / (uint32_t) p.g), h = hk * p.g + (int) ((uint32_t) row - tok * (uint32_t) p.g);
     T *out = (T *) d.out + b * d.os[0] + tok * d.os[1] + h * d.os[2];
     bool bad = false;
 #pragma unroll
@@ -147,194 +143,29 @@ __device__ __forceinline__ void load_keys(const T *src, int64_t stride, int at, 
     }
 }
 
-template <int DC, int RPT>
-struct tile_cfg {
-    static constexpr int BM = 16 * RPT, KT = 32, DP = 32 * DC, LD = DP + 4, PLD = KT + 4;
-    static constexpr int KV = KT * LD;  // floats a K or V tile
-    static constexpr int SMEM = (BM * LD + 4 * KV + BM * PLD + BM) * 4;
-    static_assert(BM * LD <= 4 * KV, "the sums fit the tiles");
-    static_assert(SMEM <= 232448, "shared memory");
-};
-
-template <typename T, int DC, int RPT>
-__global__ void __launch_bounds__(128)
-attn_tile_kernel(const __grid_constant__ tile_params p) {
-    using cfg = tile_cfg<DC, RPT>;
-    constexpr int KT = cfg::KT, LD = cfg::LD;
-    extern __shared__ float4 smem4[];
-    float *sq = (float *) smem4, *skv = sq + cfg::BM * LD, *sp = skv + 4 * cfg::KV;
-    float *s_l = sp + cfg::BM * cfg::PLD;
-    const attn_desc &d = p.d;
-    pdl_wait();
-    pdl_trigger();
-    const int tid = threadIdx.x, kx = tid % 8, rg = tid / 8;
-    const int idx = blockIdx.x;
-    const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);  // (the last rows see most keys)
-    const int b = bh / d.Hkv, hk = bh % d.Hkv;
-    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
-    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
-    const int64_t r0 = (int64_t) qt * cfg::BM;  // rows: token g + head of the group
-    const int rows = (int) min((int64_t) cfg::BM, (int64_t) n * p.g - r0);
-    if (rows <= 0) return;
-    const int64_t base = (int64_t) L - n;
-    const key_range kr = keys_of(d, L, base + r0 / p.g, base + (r0 + rows - 1) / p.g);
-    // the keys that some row sees, in one list: the sinks, then the window
-    const int keys = kr.first + kr.hi - kr.lo, nall = (keys + KT - 1) / KT;
-    auto key_at = [&](int i) { return i < kr.first ? i : i - kr.first + kr.lo; };
-    const T *kbase = (const T *) d.k + b * d.ks[0] + hk * d.ks[2], *vbase = (const T *) d.v + b * d.vs[0] + hk * d.vs[2];
-
-    for (int i = tid; i < cfg::BM * DC * 8; i += 128) {
-        const int r = i / (DC * 8), x = i % (DC * 8) * 4;
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < rows) {
-            const int tok = (int) ((r0 + r) / p.g), h = hk * p.g + (int) ((r0 + r) % p.g);
-            f = load4((const T *) d.q + b * d.qs[0] + tok * d.qs[1] + h * d.qs[2] + x, d.D - x, p.q_vec);
-        }
-        *reinterpret_cast<float4 *>(sq + r * LD + x) = make_float4(f.x * p.c, f.y * p.c, f.z * p.c, f.w * p.c);
-    }
-    auto load = [&](int i) {  // tile i of the list into buffer i & 1
-        float *k = skv + (i & 1) * 2 * cfg::KV;
-        load_keys<T, DC, KT, LD, 128>(kbase, d.ks[1], i * KT, kr, keys, d.D, p.kv_vec, k, tid);
-        load_keys<T, DC, KT, LD, 128>(vbase, d.vs[1], i * KT, kr, keys, d.D, p.kv_vec, k + cfg::KV, tid);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    key_range kk[RPT];
-    float m[RPT], l[RPT];
-    float4 o[RPT][DC];
-#pragma unroll
-    for (int j = 0; j < RPT; j++) {
-        const int64_t pos = base + (r0 + min(rg + 16 * j, rows - 1)) / p.g;
-        kk[j] = keys_of(d, L, pos, pos);
-        m[j] = -INFINITY;
-        l[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DC; i++) o[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    if (nall) load(0);
-    for (int i = 0; i < nall; i++) {
-        if (i + 1 < nall) {
-            load(i + 1);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        __syncthreads();
-        const float *k = skv + (i & 1) * 2 * cfg::KV, *v = k + cfg::KV;
-        const int here = min(KT, keys - i * KT);  // keys of the tile
-        float s[RPT][4];
-#pragma unroll
-        for (int j = 0; j < RPT; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[j][e] = 0.0f;
-#pragma unroll 4
-        for (int x = 0; x < cfg::DP; x += 4) {
-            float4 kv[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) kv[e] = *reinterpret_cast<const float4 *>(k + (kx + 8 * e) * LD + x);
-#pragma unroll
-            for (int j = 0; j < RPT; j++) {
-                const float4 q = *reinterpret_cast<const float4 *>(sq + (rg + 16 * j) * LD + x);
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[j][e] = dot4(q, kv[e], s[j][e]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < RPT; j++) {
-            float mn = m[j];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int at = kx + 8 * e, key = key_at(i * KT + at);
-                if (!(at < here && key < kk[j].hi && (key >= kk[j].lo || key < d.sinks))) s[j][e] = -INFINITY;
-                mn = fmaxf(mn, s[j][e]);
-            }
-#pragma unroll
-            for (int w = 4; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
-            const float zero = mn == -INFINITY ? 0.0f : mn, f = exp2f(m[j] - zero);
-            m[j] = mn;
-            l[j] *= f;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float w = exp2f(s[j][e] - zero);
-                l[j] += w;
-                sp[(rg + 16 * j) * cfg::PLD + kx + 8 * e] = w;
-            }
-#pragma unroll
-            for (int e = 0; e < DC; e++) {
-                o[j][e].x *= f;
-                o[j][e].y *= f;
-                o[j][e].z *= f;
-                o[j][e].w *= f;
-            }
-        }
-        __syncwarp();  // (a row's weights are written and read by one warp)
-#pragma unroll 2
-        for (int key = 0; key < here; key += 4) {  // (weights behind the list's end are zeros, and so are the values)
-            float4 w[RPT];
-#pragma unroll
-            for (int j = 0; j < RPT; j++)
-                w[j] = *reinterpret_cast<const float4 *>(sp + (rg + 16 * j) * cfg::PLD + key);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int x = 0; x < DC; x++) {
-                    const float4 vv = *reinterpret_cast<const float4 *>(v + (key + e) * LD + 4 * kx + 32 * x);
-#pragma unroll
-                    for (int j = 0; j < RPT; j++) {
-                        const float f = e == 0 ? w[j].x : e == 1 ? w[j].y : e == 2 ? w[j].z : w[j].w;
-                        o[j][x].x = fmaf(f, vv.x, o[j][x].x);
-                        o[j][x].y = fmaf(f, vv.y, o[j][x].y);
-                        o[j][x].z = fmaf(f, vv.z, o[j][x].z);
-                        o[j][x].w = fmaf(f, vv.w, o[j][x].w);
-                    }
-                }
-        }
-        __syncthreads();  // (the tile's buffer is loaded again)
-    }
-    // sums to shared memory (in the tiles' place), then a row at a time to a warp
-#pragma unroll
-    for (int j = 0; j < RPT; j++) {
-#pragma unroll
-        for (int w = 4; w > 0; w >>= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], w);
-        const int r = rg + 16 * j;
-        if (kx == 0) s_l[r] = l[j];
-#pragma unroll
-        for (int x = 0; x < DC; x++) *reinterpret_cast<float4 *>(skv + r * LD + 4 * kx + 32 * x) = o[j][x];
-    }
-    __syncthreads();
-    const int lane = tid & 31, warp = tid >> 5;
-    for (int r = warp; r < rows; r += 4) {
-        float v[DC];
-#pragma unroll
-        for (int x = 0; x < DC; x++) v[x] = skv[r * LD + lane + 32 * x];
-        store_row<T, DC>(p, b, hk, r0 + r, n, L, s_l[r], v, lane);
-    }
-}
-
-template <int DC, int R, int W>
+template <int DC, int R, int WARPS>
 struct row_cfg {
-    static constexpr int WARPS = W, KT = 8, KPL = KT / 8;
-    static constexpr int BM = 4 * R, LD = 32 * DC + 4, PLD = KT + 4;
+    static constexpr int KT = 8, BM = 4 * R, LD = 32 * DC + 4, PLD = KT + 4;
     static constexpr int KV = KT * LD;                  // floats a K or V tile
     static constexpr int WARP = 4 * KV + BM * PLD;      // floats a warp: two tiles of each, weights
-    static constexpr int SMEM = (BM * LD + WARPS * WARP + 2 * WARPS * BM) * 4;
+    static constexpr int SMEM = (WARPS * WARP + 2 * WARPS * BM) * 4;
     static_assert(BM <= 4 * KT, "a part fits the tiles");
     static_assert(SMEM <= 232448, "shared memory");
 };
 
-// few rows: 4 R of them, all by each of the CTA's warps, which share the
-// keys out and run on their own until they join
+// 4 R rows, all by each of the CTA's warps, which share the keys out and run
+// on their own until they join
 template <typename T, int DC, int R, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
-attn_rows_kernel(const __grid_constant__ tile_params p) {
+attn_rows_kernel(const __grid_constant__ rows_params p) {
     using cfg = row_cfg<DC, R, WARPS>;
-    constexpr int KT = cfg::KT, LD = cfg::LD, KPL = cfg::KPL, BM = cfg::BM;
+    constexpr int KT = cfg::KT, LD = cfg::LD, BM = cfg::BM;
     extern __shared__ float4 smem4[];
     const attn_desc &d = p.d;
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kx = lane % 8, rg = lane / 8;
-    float *sq = (float *) smem4, *parts = sq + BM * LD, *skv = parts + warp * cfg::WARP, *sp = skv + 4 * cfg::KV;
+    float *parts = (float *) smem4, *skv = parts + warp * cfg::WARP, *sp = skv + 4 * cfg::KV;
     float2 *s_ml = (float2 *) (parts + WARPS * cfg::WARP);
     int idx = blockIdx.x;
     const int rank = idx % p.splits;
@@ -347,7 +178,7 @@ attn_rows_kernel(const __grid_constant__ tile_params p) {
     const int rows = (int) min((int64_t) BM, (int64_t) n * p.g - r0);
     if (rows <= 0) return;  // (the whole cluster alike)
     const int64_t base = (int64_t) L - n;
-    const key_range kr = keys_of(d, L, base + r0 / p.g, base + (r0 + rows - 1) / p.g);
+    const key_range kr = keys_of(d, L, base + (uint32_t) r0 / (uint32_t) p.g, base + (uint32_t) (r0 + rows - 1) / (uint32_t) p.g);
     const int keys = kr.first + kr.hi - kr.lo, nall = (keys + KT - 1) / KT;
     auto key_at = [&](int i) { return i < kr.first ? i : i - kr.first + kr.lo; };
     const int share = rank * WARPS + warp, shares = p.splits * WARPS;
@@ -365,76 +196,72 @@ attn_rows_kernel(const __grid_constant__ tile_params p) {
     load_v(i0);
     load_k(i0 + 1);
     load_v(i0 + 1);
-    for (int i = tid; i < BM * DC * 8; i += WARPS * 32) {
-        const int r = i / (DC * 8), x = i % (DC * 8) * 4;
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < rows) {
-            const int tok = (int) ((r0 + r) / p.g), h = hk * p.g + (int) ((r0 + r) % p.g);
-            f = load4((const T *) d.q + b * d.qs[0] + tok * d.qs[1] + h * d.qs[2] + x, d.D - x, p.q_vec);
-        }
-        *reinterpret_cast<float4 *>(sq + r * LD + x) = make_float4(f.x * p.c, f.y * p.c, f.z * p.c, f.w * p.c);
-    }
     key_range kk[R];
     float m[R], l[R];
-    uint64_t o[R][DC][2];  // pairs of columns
+    uint64_t q[R][DC][2], o[R][DC][2];  // columns 4 kx + 32 i of the rows, in pairs
 #pragma unroll
     for (int j = 0; j < R; j++) {
-        const int64_t pos = base + (r0 + min(rg + 4 * j, rows - 1)) / p.g;
+        // (rows fit 32 bits: launch)
+        const uint32_t r = (uint32_t) r0 + min(rg + 4 * j, rows - 1), tok = r / (uint32_t) p.g, h = r - tok * p.g;
+        const int64_t pos = base + tok;
         kk[j] = keys_of(d, L, pos, pos);
         m[j] = -INFINITY;
         l[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DC; i++) o[j][i][0] = o[j][i][1] = 0;
+        for (int i = 0; i < DC; i++) {
+            const int x = 4 * kx + 32 * i;
+            const float4 f = load4((const T *) d.q + b * d.qs[0] + tok * d.qs[1] + (hk * p.g + h) * d.qs[2] + x,
+                                   d.D - x, p.q_vec);
+            q[j][i][0] = pack2(f.x * p.c, f.y * p.c);
+            q[j][i][1] = pack2(f.z * p.c, f.w * p.c);
+            o[j][i][0] = o[j][i][1] = 0;
+        }
     }
-    __syncthreads();
     for (int i = i0; i < i1; i++) {
         const float *k = skv + (i & 1) * cfg::KV, *v = skv + (2 + (i & 1)) * cfg::KV;
         asm volatile("cp.async.wait_group 3;" ::: "memory");
         __syncwarp();
         const int here = min(KT, keys - i * KT);  // keys of the tile
-        uint64_t s2[R][KPL][2];  // pairs of partial sums
+        float s[R][KT];  // of the lane's columns
 #pragma unroll
-        for (int j = 0; j < R; j++)
+        for (int e = 0; e < KT; e++) {
+            uint64_t s2[R];
 #pragma unroll
-            for (int e = 0; e < KPL; e++) s2[j][e][0] = s2[j][e][1] = 0;
-#pragma unroll 8
-        for (int x = 0; x < 32 * DC; x += 4) {
-            ulonglong2 kv[KPL];
+            for (int j = 0; j < R; j++) s2[j] = 0;
 #pragma unroll
-            for (int e = 0; e < KPL; e++) kv[e] = *reinterpret_cast<const ulonglong2 *>(k + (kx + 8 * e) * LD + x);
+            for (int x = 0; x < DC; x++) {
+                const ulonglong2 kv = *reinterpret_cast<const ulonglong2 *>(k + e * LD + 4 * kx + 32 * x);
+#pragma unroll
+                for (int j = 0; j < R; j++) s2[j] = fma2(q[j][x][1], kv.y, fma2(q[j][x][0], kv.x, s2[j]));
+            }
 #pragma unroll
             for (int j = 0; j < R; j++) {
-                const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(sq + (rg + 4 * j) * LD + x);
-#pragma unroll
-                for (int e = 0; e < KPL; e++) {
-                    s2[j][e][0] = fma2(q.x, kv[e].x, s2[j][e][0]);
-                    s2[j][e][1] = fma2(q.y, kv[e].y, s2[j][e][1]);
-                }
+                const float2 h = unpack2(s2[j]);
+                s[j][e] = h.x + h.y;
             }
         }
         __syncwarp();  // (K's buffer is loaded again)
         load_k(i + 2);
 #pragma unroll
         for (int j = 0; j < R; j++) {
-            float s[KPL], mn = m[j];
+            // the eight lanes' sums, key kx's to lane kx
 #pragma unroll
-            for (int e = 0; e < KPL; e++) {
-                const int at = kx + 8 * e, key = key_at(i * KT + at);
-                const float2 h = unpack2(add2(s2[j][e][0], s2[j][e][1]));
-                s[e] = at < here && key < kk[j].hi && (key >= kk[j].lo || key < d.sinks) ? h.x + h.y : -INFINITY;
-                mn = fmaxf(mn, s[e]);
-            }
+            for (int w = 4; w > 0; w >>= 1)
+#pragma unroll
+                for (int e = 0; e < w; e++) {
+                    const float mine = kx & w ? s[j][e + w] : s[j][e], other = kx & w ? s[j][e] : s[j][e + w];
+                    s[j][e] = mine + __shfl_xor_sync(0xffffffffu, other, w);
+                }
+            const int key = key_at(i * KT + kx);
+            const bool sees = kx < here && key < kk[j].hi && (key >= kk[j].lo || key < d.sinks);
+            const float sc = sees ? s[j][0] : -INFINITY;
+            float mn = fmaxf(m[j], sc);
 #pragma unroll
             for (int w = 4; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
-            const float zero = mn == -INFINITY ? 0.0f : mn, f = exp2f(m[j] - zero);
+            const float zero = mn == -INFINITY ? 0.0f : mn, f = exp2f(m[j] - zero), w = exp2f(sc - zero);
             m[j] = mn;
-            l[j] *= f;
-#pragma unroll
-            for (int e = 0; e < KPL; e++) {
-                const float w = exp2f(s[e] - zero);
-                l[j] += w;
-                sp[(rg + 4 * j) * cfg::PLD + kx + 8 * e] = w;
-            }
+            l[j] = fmaf(l[j], f, w);
+            sp[(rg + 4 * j) * cfg::PLD + kx] = w;
             const uint64_t ff = pack2(f, f);
 #pragma unroll
             for (int e = 0; e < DC; e++)
@@ -510,7 +337,7 @@ attn_rows_kernel(const __grid_constant__ tile_params p) {
 }
 
 template <auto kernel>
-cudaError_t launch(tile_params &p, int rows, int threads, int smem, int64_t most_splits, cudaStream_t st) {
+cudaError_t launch(rows_params &p, int rows, int threads, int smem, int64_t most_splits, cudaStream_t st) {
     const attn_desc &d = p.d;
     const int64_t qtiles = ((int64_t) d.Tq * p.g + rows - 1) / rows, bh = (int64_t) d.B * d.Hkv;
     if (qtiles > INT32_MAX || bh * qtiles > INT32_MAX / 8) return cudaErrorInvalidValue;
@@ -547,7 +374,7 @@ cudaError_t launch(tile_params &p, int rows, int threads, int smem, int64_t most
 }
 
 template <typename T, int DC, int R, int WARPS>
-cudaError_t run_warps(tile_params &p, cudaStream_t st) {
+cudaError_t run_warps(rows_params &p, cudaStream_t st) {
     using cfg = row_cfg<DC, R, WARPS>;
     const attn_desc &d = p.d;
     // the keys that a CTA's rows can see
@@ -560,31 +387,26 @@ cudaError_t run_warps(tile_params &p, cudaStream_t st) {
 }
 
 template <typename T, int DC, int R>
-cudaError_t run_few(tile_params &p, cudaStream_t st) {
-    // eight warps a CTA hide more of each other's latency; with four, three
-    // CTAs fit an SM and one's start and end hide behind the others (768
-    // rows of 128 over 200 keys each 69 -> 44 us; four rows over 4100 keys,
-    // 64 times, 73 us against 110)
+cudaError_t run_few(rows_params &p, cudaStream_t st) {
+    // eight warps a CTA hide more of each other's latency; with four, two or
+    // three CTAs fit an SM and one's start and end hide behind the others
+    // (768 rows of 128 over 200 keys each: four warps 39 us, eight 68; four
+    // rows over 4100 keys, 64 times: 71, 58)
     const int64_t ctas = ((int64_t) p.d.Tq * p.g + 4 * R - 1) / (4 * R) * p.d.B * p.d.Hkv;
     if (DC > 4 || ctas >= 2 * sm_count()) return run_warps<T, DC, R, 4>(p, st);
     return run_warps<T, DC, R, (DC > 4 ? 4 : 8)>(p, st);
 }
 
 template <typename T, int DC>
-cudaError_t run_rows(tile_params &p, cudaStream_t st) {
-    // 64 rows a CTA (32 of wide heads) where that fills the SMs and more than
-    // half of the tiles (64 sequences of 12 heads of 128, 500 keys: of 32 rows
-    // 453 us in tiles, 271 in 16 rows a CTA; of 48 rows 464, 475)
-    constexpr int RPT = DC > 4 ? 2 : 4;
-    const int64_t rows = (int64_t) p.d.Tq * p.g, tiles = (rows + 16 * RPT - 1) / (16 * RPT) * p.d.B * p.d.Hkv;
-    if (rows > 8 * RPT && tiles >= sm_count())
-        return launch<attn_tile_kernel<T, DC, RPT>>(p, 16 * RPT, 128, tile_cfg<DC, RPT>::SMEM, 1, st);
-    return rows <= 4 ? run_few<T, DC, 1>(p, st) : rows <= 8 ? run_few<T, DC, 2>(p, st) : run_few<T, DC, 4>(p, st);
+cudaError_t run_rows(rows_params &p, cudaStream_t st) {
+    constexpr int MOST = DC > 4 ? 2 : 4;  // (of wide heads eight rows: registers)
+    const int64_t rows = (int64_t) p.d.Tq * p.g;
+    return rows <= 4 ? run_few<T, DC, 1>(p, st) : rows <= 8 ? run_few<T, DC, 2>(p, st) : run_few<T, DC, MOST>(p, st);
 }
 
 template <typename T>
 cudaError_t run_simt(const attn_desc &d, cudaStream_t st) {
-    tile_params p{};
+    rows_params p{};
     p.d = d;
     p.g = d.Hq / d.Hkv;
     p.c = d.scale * 1.4426950408889634f;
@@ -594,6 +416,7 @@ cudaError_t run_simt(const attn_desc &d, cudaStream_t st) {
     };
     p.q_vec = vec(d.q, d.qs, d.Tq, d.Hq);
     p.kv_vec = vec(d.k, d.ks, d.Tk, d.Hkv) && vec(d.v, d.vs, d.Tk, d.Hkv);
+    if (d.D <= 32) return run_rows<T, 1>(p, st);
     if (d.D <= 64) return run_rows<T, 2>(p, st);
     if (d.D <= 128) return run_rows<T, 4>(p, st);
     return run_rows<T, 8>(p, st);
