@@ -29,7 +29,8 @@ __device__ __forceinline__ f8_scale f8_scale_of(float amax) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(k.s));
     // 2^-90 .. 2^120: the reciprocal and the remainders that matter are normal numbers
-    k.r = k.s >= 8.07793567e-28f && k.s <= 1.32922800e+36f ? r : 0.0f;
+    // (zeros are zeros, and NaN NaN, times any number; padding is made of them)
+    k.r = amax == 0.0f ? 1.0f : k.s >= 8.07793567e-28f && k.s <= 1.32922800e+36f ? r : 0.0f;
     return k;
 }
 // two elements' quotients

@@ -197,28 +197,41 @@ __device__ __forceinline__ float4 ld_rank4(uint32_t saddr, uint32_t rank) {
                  : "memory");
     return v;
 }
-// n elements of ES bytes, where rows start off 16-byte boundaries or end
+// 32 rows of 64 staged bytes (below: unit u of row r at u ^ (r / 2 mod 4)) to
+// `rows` rows of Y, `cols` columns of ES bytes, where rows start off 16-byte
+// boundaries or end: an element a lane, one behind the other
 template <int ES>
-__device__ __noinline__ void copy_elements(uint8_t *y, const uint8_t *x, int n) {
-    for (int i = 0; i < n; i++) {
-        if (ES == 4) reinterpret_cast<uint32_t *>(y)[i] = reinterpret_cast<const uint32_t *>(x)[i];
-        else if (ES == 2) reinterpret_cast<uint16_t *>(y)[i] = reinterpret_cast<const uint16_t *>(x)[i];
-        else y[i] = x[i];
+__device__ __noinline__ void copy_elements(uint8_t *y, int64_t step, const uint8_t *piece, int rows, int cols, int lane) {
+    constexpr int PER = 64 / ES;  // elements a row
+#pragma unroll 4
+    for (int i = lane; i < 32 * PER; i += 32) {
+        const int r = i / PER, c = i % PER, at = c * ES;
+        const uint8_t *x = piece + r * 64 + (at / 16 ^ (r >> 1 & 3)) * 16 + at % 16;
+        if (r < rows && c < cols) {
+            if (ES == 4) *reinterpret_cast<uint32_t *>(y + r * step + at) = *reinterpret_cast<const uint32_t *>(x);
+            else if (ES == 2) *reinterpret_cast<uint16_t *>(y + r * step + at) = *reinterpret_cast<const uint16_t *>(x);
+            else y[r * step + at] = *x;
+        }
     }
 }
-// four values of a row to Y columns n .. n + 3 where these end, or start off a
-// vector's boundary (F8: quantised by s)
+// a row of 128 columns, four a lane, to Y where it starts off a vector's
+// boundary or ends (F8: quantised by s): through `row` in shared memory, so
+// that lanes store one behind the other
 template <int YT>
-__device__ __noinline__ void store4(const f8_params &p, int64_t m, int n, float4 f, f8_scale s) {
-    const float v[4] = {f.x, f.y, f.z, f.w};
-    const uint32_t q = YT == TPMD_DTYPE_F8 ? f8_quant4(f.x, f.y, f.z, f.w, s) : 0;
+__device__ __noinline__ void store_off(const f8_params &p, int64_t m, int n0, float4 v, f8_scale s, float *row, int lane) {
+    if constexpr (YT == TPMD_DTYPE_F8) reinterpret_cast<uint32_t *>(row)[lane] = f8_quant4(v.x, v.y, v.z, v.w, s);
+    else reinterpret_cast<float4 *>(row)[lane] = v;
+    __syncwarp();
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (n + e < p.N) {
-            if constexpr (YT == TPMD_DTYPE_F8) ((uint8_t *) p.Y)[m * p.ldy + n + e] = (uint8_t) (q >> 8 * e);
-            else if constexpr (YT == TPMD_DTYPE_F16) ((__half *) p.Y)[m * p.ldy + n + e] = __float2half_rn(v[e]);
-            else ((float *) p.Y)[m * p.ldy + n + e] = v[e];
+    for (int e = 0; e < 4; e++) {
+        const int c = lane + 32 * e;
+        if (n0 + c < p.N) {
+            const int64_t at = m * p.ldy + n0 + c;
+            if constexpr (YT == TPMD_DTYPE_F8) ((uint8_t *) p.Y)[at] = reinterpret_cast<const uint8_t *>(row)[c];
+            else if constexpr (YT == TPMD_DTYPE_F16) ((__half *) p.Y)[at] = __float2half_rn(row[c]);
+            else ((float *) p.Y)[at] = row[c];
         }
+    }
 }
 
 // YT: TPMD_DTYPE_* of Y
@@ -495,10 +508,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                         for (int r = 0; r < 4; r++)
                             if (r * 8 < rows_left) *reinterpret_cast<uint4 *>(y + r * step + x * ES) = t[r];
                     } else {
-                        const int left = min(PER, p.N - n0 - x - unit * PER);
-#pragma unroll 1
-                        for (int r = 0; r < 4; r++)
-                            if (r * 8 < rows_left && left > 0) copy_elements<ES>(y + r * step + x * ES, src + r * 512, left);
+                        copy_elements<ES>((uint8_t *) p.Y + ((int64_t) m0 * p.ldy + n0 + x) * ES, p.ldy * ES, piece,
+                                          p.M - m0, p.N - n0 - x, lane);
                     }
                     __syncwarp();
                 }
@@ -522,7 +533,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         // row's maximum.)
         constexpr int RB = 4, NW = cfg::THREADS / 32;
         const int rows = min(cfg::BM, p.M - m0);
-        const bool vec4 = p.y_vec && n + 4 <= p.N;
+        const bool vec4 = p.y_vec && (n0 + 128 <= p.N || p.N % 4 == 0);
 #pragma unroll 1
         for (int r0 = (split * NW + warp) * RB; r0 < rows; r0 += p.splits * NW * RB) {
             float4 v[RB];
@@ -582,7 +593,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     s = f8_scale_of(top[j]);
                     if (lane == 0) p.sy[(m + j) * p.ldsy + n0 / 128] = s.s;
                 }
-                if (vec4) {
+                if (!vec4) {
+                    // (the row's place here: no other warp reads it)
+                    store_off<YT>(p, m + j, n0, v[j], s, (float *) smem + (r0 + j) * cfg::PART_LD, lane);
+                } else if (n < p.N) {
                     if constexpr (YT == TPMD_DTYPE_F8) {
                         *reinterpret_cast<uint32_t *>(y + j * step) = f8_quant4(v[j].x, v[j].y, v[j].z, v[j].w, s);
                     } else if constexpr (YT == TPMD_DTYPE_F16) {
@@ -591,8 +605,6 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     } else {
                         *reinterpret_cast<float4 *>(y + j * step) = v[j];
                     }
-                } else if (n < p.N) {
-                    store4<YT>(p, m + j, n, v[j], s);
                 }
             }
         }
