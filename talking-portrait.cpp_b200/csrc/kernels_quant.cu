@@ -24,15 +24,21 @@ struct alignas(sizeof(T) * VEC) vec_of {
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 
-// VEC elements of row `r` from column c, zero from column K on
+// a lane's VEC elements of the block of row `r` that begins at column c0, zero
+// from column K on: side by side, or, where rows start off a vector's
+// boundary, one in every LANES = 128 / VEC, so that lanes load and store one
+// behind the other (3451 x 3663 f16, blocks of 128 x 128: side by side 31 us,
+// so 21)
 template <typename T, int VEC, bool ALIGNED>
-__device__ __forceinline__ vec_of<T, VEC> load_row(const T *r, int64_t c, int64_t K) {
+__device__ __forceinline__ vec_of<T, VEC> load_row(const T *r, int64_t c0, int lane, int64_t K) {
     vec_of<T, VEC> x;
+    const int64_t c = c0 + lane * (ALIGNED ? VEC : 1);
+    constexpr int D = ALIGNED ? 1 : 128 / VEC;
     if (ALIGNED && c + VEC <= K) {
         x = *reinterpret_cast<const vec_of<T, VEC> *>(r + c);
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) x.v[e] = c + e < K ? r[c + e] : T(0.0f);
+        for (int e = 0; e < VEC; e++) x.v[e] = c + e * D < K ? r[c + e * D] : T(0.0f);
     }
     return x;
 }
@@ -80,14 +86,17 @@ __device__ __forceinline__ vec_of<uint8_t, VEC> quant_vec(const vec_of<T, VEC> &
     return t;
 }
 template <typename T, int VEC, bool ALIGNED>
-__device__ __forceinline__ void store_row(uint8_t *r, int64_t c, int64_t K, f8_scale s, const vec_of<T, VEC> &x) {
+__device__ __forceinline__ void store_row(uint8_t *r, int64_t c0, int lane, int64_t K, f8_scale s,
+                                          const vec_of<T, VEC> &x) {
     const vec_of<uint8_t, VEC> t = quant_vec(x, s);
+    const int64_t c = c0 + lane * (ALIGNED ? VEC : 1);
+    constexpr int D = ALIGNED ? 1 : 128 / VEC;
     if (ALIGNED && c + VEC <= K) {
         *reinterpret_cast<vec_of<uint8_t, VEC> *>(r + c) = t;
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; e++)
-            if (c + e < K) r[c + e] = t.v[e];
+            if (c + e * D < K) r[c + e * D] = t.v[e];
     }
 }
 
@@ -115,7 +124,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x
         vec_of<T, VEC> v[U];
         float top[U];
         constexpr int STEP = 32 / LANES * 128;  // columns a load of a warp
-        const int64_t c = ((int64_t) g * GROUP + sub) * 128 + lane * VEC;
+        const int64_t c0 = ((int64_t) g * GROUP + sub) * 128, c = c0 + lane * VEC;
         if (ALIGNED && (int64_t) (g + 1) * GROUP * 128 <= K) {  // whole blocks: no column to look at
             const T *xp = x + m * ldx + c;
 #pragma unroll
@@ -131,14 +140,14 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x
             }
         } else {
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = load_row<T, VEC, ALIGNED>(x + m * ldx, c + u * STEP, K);
+            for (int u = 0; u < U; u++) v[u] = load_row<T, VEC, ALIGNED>(x + m * ldx, c0 + u * STEP, lane, K);
             amax_lanes<U, LANES>(v, top);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int b = g * GROUP + u * (32 / LANES) + sub;
                 const f8_scale sc = f8_scale_of(top[u]);
                 if (b < kb) {
-                    store_row<T, VEC, ALIGNED>(q + m * ldq, c + u * STEP, K, sc, v[u]);
+                    store_row<T, VEC, ALIGNED>(q + m * ldq, c0 + u * STEP, lane, K, sc, v[u]);
                     if (lane == 0) s[m * lds + b] = sc.s;
                 }
             }
@@ -156,14 +165,15 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__
     constexpr int LANES = 128 / VEC, ROWS = 256 / LANES, N = 128 / ROWS;
     __shared__ float red[8];
     const int64_t mb = blockIdx.x / kb, b = blockIdx.x % kb;
-    const int64_t c = b * 128 + threadIdx.x % LANES * VEC, r0 = mb * 128 + threadIdx.x / LANES;
+    const int64_t c0 = b * 128, r0 = mb * 128 + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
     vec_of<T, VEC> v[N];
     float a = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int64_t m = r0 + i * ROWS;
         // rows behind the last one load as zeros (no column below 0)
-        v[i] = load_row<T, VEC, ALIGNED>(x + (m < M ? m : 0) * ldx, c, m < M ? K : 0);
+        v[i] = load_row<T, VEC, ALIGNED>(x + (m < M ? m : 0) * ldx, c0, lane, m < M ? K : 0);
         a = fmaxf(a, amax_of(v[i]));
     }
 #pragma unroll
@@ -175,7 +185,7 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__
     const f8_scale sc = f8_scale_of(a);
 #pragma unroll
     for (int i = 0; i < N; i++)
-        if (r0 + i * ROWS < M) store_row<T, VEC, ALIGNED>(q + (r0 + i * ROWS) * ldq, c, K, sc, v[i]);
+        if (r0 + i * ROWS < M) store_row<T, VEC, ALIGNED>(q + (r0 + i * ROWS) * ldq, c0, lane, K, sc, v[i]);
     if (threadIdx.x == 0) s[mb * lds + b] = sc.s;
 }
 
