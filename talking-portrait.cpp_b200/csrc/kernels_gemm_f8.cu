@@ -9,9 +9,9 @@
 // multiplies; a tile of its own would need more from L2 than the SMs get).
 // Rows of X are the MMA's M side (TMEM lanes), blocks of 128 rows of W its N
 // side, so a block's W scale of one k block is one number and a lane's
-// factor sx sw is one number for all its 128 columns. Each k block of 128 is one pipeline stage (one
-// 128-byte swizzled row a matrix row) and one MMA group into an accumulator
-// of its own out of a ring in TMEM; the epilogue warps (each a lane quarter
+// factor sx sw is one number for all its 128 columns. Each k block of 128 is
+// one pipeline stage (one 128-byte swizzled row a matrix row) and one MMA
+// group into an accumulator of its own out of a ring in TMEM; the epilogue warps (each a lane quarter
 // and half of the columns) read it, scale it and add it to f32 registers while the
 // next blocks multiply. The products of e4m3 values are exact in
 // f32; sums are f32 throughout.
@@ -22,6 +22,17 @@
 // tile are shared out over a cluster of up to eight CTAs; each leaves its
 // partial tile in its shared memory, and each adds its rows of all of them
 // (distributed shared memory), always in the same order.
+//
+// Measured, and what bounds it (f32 sums of every block of 128 pass through
+// the epilogue warps: 4 bytes of TMEM for each 256 operations):
+//  * 8192 x 4096 x 4096, f16 out: 137 to 147 us, 1.87 to 2.0 PFLOP/s, 0.56 to
+//    0.6 of twice the bf16 rate (173 us, 1.59 PFLOP/s, after seconds under
+//    the power cap); by the TMEM reads and multiply-adds of the blocks.
+//  * 180 x 4096 x 1024 with GELU and an 8-bit output: 9.4 us, 180 x 1024 x
+//    4096: 9.0 us; by latency: launch, first loads, a few blocks, the join.
+//  * 900 x 8192 x 453 with GELU and an 8-bit output: 22 us; two tiles for each
+//    pair of CTAs, their epilogues longer than their products. (128 x 128
+//    tiles instead: 40 us.)
 //
 // Every pipeline wait is bounded; an expired wait sets *err and the CTA
 // skips the rest of its work.

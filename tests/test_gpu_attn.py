@@ -128,6 +128,27 @@ def test_many_rows(case):
     check(q, k, v, left, right, sinks, q_len=n, kv_len=L)
 
 
+# f32 rows: one to sixteen a CTA, every width of a lane's share, one sequence and hundreds
+F32_ROWS = [(1, 1, 300, 4, 1, 32, 70, 0, 3), (2, 2, 301, 4, 1, 20, -1, 0, 0), (1, 4, 77, 4, 1, 128, 20, 5, 9),
+            (1, 3, 500, 3, 1, 96, 50, 0, 9), (3, 30, 95, 2, 2, 33, 12, 2, 17), (1, 9, 1100, 3, 1, 200, 333, 0, 130),
+            (2, 1, 640, 4, 2, 256, -1, 0, 0), (1, 31, 31, 2, 1, 250, 8, 0, 2), (80, 1, 70, 4, 4, 128, 40, 0, 3),
+            (100, 2, 50, 9, 3, 64, -1, 0, 0), (30, 40, 90, 10, 5, 30, 17, 3, 11), (20, 30, 60, 8, 8, 200, 25, 0, 4),
+            (310, 1, 40, 3, 1, 5, 9, 0, 20), (1, 1500, 1500, 6, 2, 64, 100, 0, 6)]
+
+
+@pytest.mark.parametrize("case", F32_ROWS, ids=lambda c: "-".join(map(str, c)))
+def test_f32_rows(case):
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = case
+    q, k, v = make(B, Tq, Tk, Hq, Hkv, D, "f32", gain=2.0)
+    check(q, k, v, left, right, sinks)
+    # lengths of their own; NaN and infinities behind the ends
+    n = lens(*[Tq * (7 * i % (B + 1)) // B for i in range(B)])
+    L = lens(*[x if Tq == Tk else max(x, Tk * (5 * i % (B + 1)) // B) for i, x in enumerate(n.tolist())])
+    for b, x in enumerate(L.tolist()):
+        k[b, x:], v[b, x:] = float("nan"), float("inf")
+    check(q, k, v, left, right, sinks, q_len=n, kv_len=L)
+
+
 def test_poison_in_many_rows():
     """as test_poison_beside_the_window, with the rows of many heads"""
     T, H = 400, 80

@@ -206,6 +206,44 @@ def test_gemm_output_strides():
         assert bool((big[:, :off] == 7).all()) and bool((big[:, off + N:] == 7).all())
 
 
+# 128 x 128 and 256 x 256 tiles
+@pytest.mark.parametrize("M,N", [(131, 131), (300, 257), (2310, 2317), (2400, 2306)])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, F8])
+def test_gemm_rows_off_vector_boundaries(M, N, out):
+    """the same bytes as with aligned rows, and none beside them"""
+    K = 72
+    g = torch.Generator().manual_seed(M + N)
+    (x, sx), (w, sw) = quantised(M, K, 1, g), quantised(N, K, 128, g)
+    bias = torch.randn(N, generator=g).cuda()
+    nb, es = -(-N // 128), out.itemsize
+    ld = -(-N // 16) * 16
+    want = torch.zeros(M, ld * es, dtype=torch.uint8, device="cuda").view(out)[:, :N]
+    scales = [torch.zeros(M, nb, device="cuda") if out is F8 else None for _ in range(2)]
+    tpmd.gemm_f8(x, sx, w, sw, want, sy=scales[0], bias=bias, act=1)
+    for ld, at in ((N, 0), (N + 5, 0), (N + 1, 3)):
+        raw = torch.full(((M * ld + at) * es,), 0x55, dtype=torch.uint8, device="cuda")
+        y = raw[at * es:].view(out).view(M, ld)[:, :N]
+        tpmd.gemm_f8(x, sx, w, sw, y, sy=scales[1], bias=bias, act=1)
+        tpmd.tpk_status()
+        assert torch.equal(y.contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+        assert out is not F8 or torch.equal(*scales)
+        beside = raw[at * es:].view(M, ld * es)[:, N * es:]
+        assert bool((beside == 0x55).all()) and bool((raw[:at * es] == 0x55).all())
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quant_blocks_of_zeros(rows):
+    """the smallest scale; a NaN between the zeros stays one"""
+    x = torch.zeros(200, 333)
+    x[3, 7], x[3, 8], x[150, 200] = float("nan"), -0.0, 1.5
+    for dt in (torch.float32, torch.float16):
+        q, _ = padded(200, 333)
+        s = torch.zeros(-(-200 // rows), 3, device="cuda")
+        tpmd.quant_f8(x.to(dt).cuda(), q, s, rows=rows)
+        rq, rs = quant_ref(x, rows)
+        assert torch.equal(s.cpu(), rs) and same_bytes(q, rq)
+
+
 def test_gemm_special_scales():
     """negative, zero, infinite and NaN scales and NaN bytes go where the
     formula takes them; the rows beside them are not touched"""
