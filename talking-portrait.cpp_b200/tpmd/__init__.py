@@ -575,7 +575,7 @@ def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1],
             c[2], o[0], o[1], o[2], 1 if dt is f16 else 0, B, Tq, Tk, Hq, Hkv, D,
             0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(), left, right, sinks,
-            D ** -0.5 if scale is None else scale, stream or 0)) != 0:
+            (D or 1) ** -0.5 if scale is None else scale, stream or 0)) != 0:
         _tpk_check(-1)
     return out
 
