@@ -224,51 +224,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const attn_desc &d = p.d;
-    pdl_wait();
-    pdl_trigger();
-    // block -> (cluster rank,) batch and key head, query tile (the last ones,
-    // which see most keys, first)
-    int idx = blockIdx.x;
-    const int rank = SPLIT ? idx % p.splits : 0;
-    if (SPLIT) idx /= p.splits;
-    const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);
-    const int b = bh / d.Hkv, hk = bh % d.Hkv;
-    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
-    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
-    const int tok0 = qt * p.tb * cfg::NQ;                        // the CTA's first token
-    const int toks = min(n - tok0, p.tb * cfg::NQ);              // and how many exist
-    if (toks <= 0) return;                                       // (the whole cluster alike)
-    const int64_t pos0 = (int64_t) L - n + tok0;
-    const key_range kr = keys_of(d, L, pos0, pos0 + toks - 1);
-    // tiles of the window, then of the sinks; SPLIT: this CTA's share of them
-    constexpr int KT = cfg::KT;
-    const int nwin = (kr.hi - kr.lo + KT - 1) / KT, nall = nwin + (kr.first + KT - 1) / KT;
-    const int i0 = SPLIT ? (int) ((int64_t) nall * rank / p.splits) : 0;
-    const int nt = (SPLIT ? (int) ((int64_t) nall * (rank + 1) / p.splits) : nall) - i0;
-    // (of tile j: its first key, how many of its keys some row sees, and these rounded up for the MMAs)
-    const int jwin = nwin - i0;  // the share's first tile of sinks
-    auto tile_key = [&](int j) { return j < jwin ? kr.lo + (i0 + j) * KT : (j - jwin) * KT; };
-    auto tile_keys = [&](int j) { return min(KT, (j < jwin ? kr.hi : kr.first) - tile_key(j)); };
-    auto tile_w = [&](int j) { return (tile_keys(j) + 15) & ~15; };
-    // warpgroup t goes through tiles [from, to) and those of the sinks. Prompts:
-    // what its rows see of the window (all of it from the start where that
-    // begins within the sinks); SPLIT: every other tile
-    const int toks0 = min(toks, p.tb), toks1 = toks - toks0;
-    int to0 = nt, from1 = 0, to1 = nt;
-    if (!SPLIT) {
-        const key_range kr0 = keys_of(d, L, pos0, pos0 + toks0 - 1);
-        to0 = (kr0.hi - kr.lo + KT - 1) / KT;
-        if (toks1 > 0) {
-            const key_range kr1 = keys_of(d, L, pos0 + toks0, pos0 + toks - 1);
-            from1 = kr.lo < d.sinks ? 0 : (kr1.lo - kr.lo) / KT;
-            to1 = (kr1.hi - kr.lo + KT - 1) / KT;
-        }
-    }
-    auto active = [&](int t, int j) {
-        if (SPLIT) return (j & 1) == t;
-        return t == 0 ? j < to0 || j >= jwin : toks1 > 0 && (j >= from1 && j < to1 || j >= jwin);
-    };
-
     if (threadIdx.x == 32) {
         prefetch_map(&tmQ);
         prefetch_map(&tmK);
@@ -303,6 +258,61 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // The set-up runs while the kernel before this one ends. TMEM is had before
+    // this one's dependents may start: one that took it first on an SM would wait
+    // for this kernel, and this kernel for it.
+    pdl_wait();
+    pdl_trigger();
+    // block -> (cluster rank,) batch and key head, query tile (the last ones,
+    // which see most keys, first)
+    int idx = blockIdx.x;
+    const int rank = SPLIT ? idx % p.splits : 0;
+    if (SPLIT) idx /= p.splits;
+    const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);
+    const int b = bh / d.Hkv, hk = bh % d.Hkv;
+    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
+    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
+    const int tok0 = qt * p.tb * cfg::NQ;                        // the CTA's first token
+    const int toks = min(n - tok0, p.tb * cfg::NQ);              // and how many exist
+    auto release = [&] {
+        if (warp == 9)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    };
+    if (toks <= 0) {  // (the whole cluster alike)
+        release();
+        return;
+    }
+    const int64_t pos0 = (int64_t) L - n + tok0;
+    const key_range kr = keys_of(d, L, pos0, pos0 + toks - 1);
+    // tiles of the window, then of the sinks; SPLIT: this CTA's share of them
+    constexpr int KT = cfg::KT;
+    const int nwin = (kr.hi - kr.lo + KT - 1) / KT, nall = nwin + (kr.first + KT - 1) / KT;
+    const int i0 = SPLIT ? (int) ((int64_t) nall * rank / p.splits) : 0;
+    const int nt = (SPLIT ? (int) ((int64_t) nall * (rank + 1) / p.splits) : nall) - i0;
+    // (of tile j: its first key, how many of its keys some row sees, and these rounded up for the MMAs)
+    const int jwin = nwin - i0;  // the share's first tile of sinks
+    auto tile_key = [&](int j) { return j < jwin ? kr.lo + (i0 + j) * KT : (j - jwin) * KT; };
+    auto tile_keys = [&](int j) { return min(KT, (j < jwin ? kr.hi : kr.first) - tile_key(j)); };
+    auto tile_w = [&](int j) { return (tile_keys(j) + 15) & ~15; };
+    // warpgroup t goes through tiles [from, to) and those of the sinks. Prompts:
+    // what its rows see of the window (all of it from the start where that
+    // begins within the sinks); SPLIT: every other tile
+    const int toks0 = min(toks, p.tb), toks1 = toks - toks0;
+    int to0 = nt, from1 = 0, to1 = nt;
+    if (!SPLIT) {
+        const key_range kr0 = keys_of(d, L, pos0, pos0 + toks0 - 1);
+        to0 = (kr0.hi - kr.lo + KT - 1) / KT;
+        if (toks1 > 0) {
+            const key_range kr1 = keys_of(d, L, pos0 + toks0, pos0 + toks - 1);
+            from1 = kr.lo < d.sinks ? 0 : (kr1.lo - kr.lo) / KT;
+            to1 = (kr1.hi - kr.lo + KT - 1) / KT;
+        }
+    }
+    auto active = [&](int t, int j) {
+        if (SPLIT) return (j & 1) == t;
+        return t == 0 ? j < to0 || j >= jwin : toks1 > 0 && (j >= from1 && j < to1 || j >= jwin);
+    };
+
     auto t_s = [&](int t, int x) { return tmem + t * 128 + x * KT; };
     auto t_o = [&](int t) { return tmem + 256 + t * DB * 64; };
     bool ok = true;
@@ -761,8 +771,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    release();
 }
 
 // a tensor map over f16 memory: dims and strides (elements) innermost first,
