@@ -18,8 +18,8 @@
 //
 // With 256 x 256 tiles (products that fill the SMs) CTAs are persistent: the
 // loads and products of the next tile run on while a tile is written. With
-// 128 x 128 tiles a CTA has one, and where SMs are left the k blocks of a
-// tile are shared out over a cluster of up to eight CTAs; each leaves its
+// 128 x 128 tiles a CTA has one, and where SMs are left they have fewer rows
+// or the k blocks of a tile are shared out over a cluster of up to eight CTAs; each leaves its
 // partial tile in its shared memory, and each adds its rows of all of them
 // (distributed shared memory), always in the same order.
 //
@@ -28,8 +28,9 @@
 //  * 8192 x 4096 x 4096, f16 out: 137 to 147 us, 1.87 to 2.0 PFLOP/s, 0.56 to
 //    0.6 of twice the bf16 rate (173 us, 1.59 PFLOP/s, after seconds under
 //    the power cap); by the TMEM reads and multiply-adds of the blocks.
-//  * 180 x 4096 x 1024 with GELU and an 8-bit output: 9.4 us, 180 x 1024 x
-//    4096: 9.0 us; by latency: launch, first loads, a few blocks, the join.
+//  * 180 x 4096 x 1024 with GELU and an 8-bit output: 8.9 us, 180 x 1024 x
+//    4096: 8.7 us; by latency: launch, first loads, eight blocks, the join.
+//  * 14 x 6656 x 4992 (33 MB of W): 11 us, 3.0 TB/s, 104 CTAs.
 //  * 900 x 8192 x 453 with GELU and an 8-bit output: 22 us; two tiles for each
 //    pair of CTAs, their epilogues longer than their products. (128 x 128
 //    tiles instead: 40 us.)
@@ -707,25 +708,35 @@ cudaError_t gemm_f8(const gemm_f8_desc &d, cudaStream_t st) {
     if (!p.err) return cudaErrorUnknown;
     const int es = d.y_dtype == TPMD_DTYPE_F32 ? 4 : d.y_dtype == TPMD_DTYPE_F16 ? 2 : 1;
     const int64_t nblk = (d.N + 127) / 128;
-    // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128,
-    // their k blocks shared out over a cluster while SMs are left and each CTA
-    // keeps two blocks
+    // 256 x 256 tiles of CTA pairs where they fill the SMs; else 128 x 128
     const int nb = ((int64_t) d.M + 255) / 256 * ((nblk + 1) / 2) >= sm_count() / 2 ? 2 : 1;
     const int unit = nb == 2 ? 16 : 4 * es;
     p.y_vec = !((uintptr_t) d.Y & (unit - 1)) && (d.M == 1 || d.ldy * es % unit == 0);
-    const int64_t tiles = ((int64_t) d.M + nb * 128 - 1) / (nb * 128) * ((nblk + nb - 1) / nb);
+    // 128 x 128: clusters that leave a CTA eight blocks; then, where SMs are
+    // left, tiles of fewer rows (32 at least): W is read again from L2, but more
+    // CTAs form the outputs. Few tiles all the same: clusters down to two
+    // blocks. (Clusters down to two blocks alone, so: 1430 x 379 x
+    // 181 12.5, 7.1 us; 777 x 1000 x 528 9.1, 8.0; 180 x 1024 x 1024 6.8, 6.3.
+    // Fewer rows under clusters of four: 180 x 1024 x 4096 8.7 -> 9.3. Eight
+    // blocks alone: 30 x 300 x 1500 6.0 -> 7.0.)
+    p.tiles_n = (int) ((nblk + nb - 1) / nb);
+    int64_t mtiles = ((int64_t) d.M + nb * 128 - 1) / (nb * 128);
+    int splits = 1;
+    if (nb == 1) {
+        splits = cluster_size(mtiles * p.tiles_n, kblocks / 8);
+        if (splits <= 2)
+            mtiles = std::max(mtiles, std::min<int64_t>(sm_count() / splits / p.tiles_n, ((int64_t) d.M + 31) / 32));
+        if (mtiles * p.tiles_n <= 16) splits = std::max(splits, cluster_size(mtiles * p.tiles_n, kblocks / 2));
+    }
+    const int64_t tiles = mtiles * p.tiles_n;
     if (tiles > INT32_MAX / 8) return cudaErrorInvalidValue;
     p.tiles = (int) tiles;
-    p.tiles_n = (int) ((nblk + nb - 1) / nb);
-    const int splits = nb == 2 ? 1 : cluster_size(tiles, kblocks / 2);
     p.kb_per_split = (kblocks + splits - 1) / splits;
     p.splits = (kblocks + p.kb_per_split - 1) / p.kb_per_split;  // no empty split
-    // tiles of 128 rows share the rows out evenly, and no box reaches far
-    // behind the last row: its zeros take as long to write as data. (What the
-    // rest of a tile's rows hold reaches no output. 14 x 6656 x 4992: 16.9 ->
-    // 11.1 us)
-    const int mtiles = (d.M + 127) / 128;
-    p.bm = nb == 2 ? 128 : ((d.M + mtiles - 1) / mtiles + 7) & ~7;
+    // the tiles share the rows out evenly, and no box reaches far behind the
+    // last row: its zeros take as long to write as data. (What the rest of a
+    // tile's rows hold reaches no output. 14 x 6656 x 4992: 16.9 -> 11.1 us)
+    p.bm = nb == 2 ? 128 : (int) ((d.M + mtiles - 1) / mtiles + 7) & ~7;
     p.x_bytes = p.bm * 128;
     CUtensorMap tmX, tmW;
     if (!encode_bytes(&tmX, d.X, d.K, d.M, d.ldx, p.bm) || !encode_bytes(&tmW, d.W, d.K, d.N, d.ldw, 128))
