@@ -35,12 +35,12 @@
 // its visible keys alone.
 //
 // Measured, and what bounds it:
-//  * 16384 tokens, 16 heads of 128 on 4, 4096 keys each (481 GFLOP): 452 to
-//    484 us, 1.0 to 1.06 PFLOP/s, 0.6 of the matrix rate. The exponentials
+//  * 16384 tokens, 16 heads of 128 on 4, 4096 keys each (481 GFLOP): 448 to
+//    484 us, 1.0 to 1.07 PFLOP/s, 0.6 of the matrix rate. The exponentials
 //    and conversions of a 128 x 64 tile take its warpgroup about as long as
 //    its products take, and the hand-over between them is not hidden wholly.
 //  * 16 sequences of one token over 4100 keys, 16 heads of 128 on 4 (134 MB):
-//    29 us, 4.6 TB/s, 0.7 of the copy rate: 128 CTAs, each ending with a join
+//    30 us, 4.5 TB/s, 0.7 of the copy rate: 128 CTAs, each ending with a join
 //    over its cluster.
 //  * 7500 tokens, 12 heads of 64, 251 keys each: 35 us (the short list of
 //    tiles: prologue and epilogue are half of a CTA's life).
