@@ -172,8 +172,8 @@ attn_rows_kernel(const __grid_constant__ rows_params p) {
     idx /= p.splits;
     const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);
     const int b = bh / d.Hkv, hk = bh % d.Hkv;
-    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
-    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
+    const int n = d.q_len ? min(max(d.q_len[b], 0), d.Tq) : d.Tq;
+    const int L = d.kv_len ? min(max(d.kv_len[b], 0), d.Tk) : d.Tk;
     const int64_t r0 = (int64_t) qt * BM;
     const int rows = (int) min((int64_t) BM, (int64_t) n * p.g - r0);
     if (rows <= 0) return;  // (the whole cluster alike)

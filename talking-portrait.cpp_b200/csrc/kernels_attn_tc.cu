@@ -270,8 +270,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     if (SPLIT) idx /= p.splits;
     const int bh = idx % (d.B * d.Hkv), qt = p.qtiles - 1 - idx / (d.B * d.Hkv);
     const int b = bh / d.Hkv, hk = bh % d.Hkv;
-    const int n = d.q_len ? min(max(__ldg(d.q_len + b), 0), d.Tq) : d.Tq;
-    const int L = d.kv_len ? min(max(__ldg(d.kv_len + b), 0), d.Tk) : d.Tk;
+    const int n = d.q_len ? min(max(d.q_len[b], 0), d.Tq) : d.Tq;
+    const int L = d.kv_len ? min(max(d.kv_len[b], 0), d.Tk) : d.Tk;
     const int tok0 = qt * p.tb * cfg::NQ;                        // the CTA's first token
     const int toks = min(n - tok0, p.tb * cfg::NQ);              // and how many exist
     auto release = [&] {

@@ -37,7 +37,7 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 }
 
 // y[n] = act(W[n] . x + b[n]), one warp per row (the timestep MLP, M = 1)
-__global__ void __launch_bounds__(256) gemv_kernel(const float *__restrict__ W, const float *__restrict__ x,
+__global__ void __launch_bounds__(256) gemv_kernel(const float *__restrict__ W, const float *x,
                                                    const float *__restrict__ b, int N, int K, int act_silu,
                                                    float *__restrict__ y) {
     pdl_wait();
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256) gemv_kernel(const float *__restrict__ W, 
     const int lane = threadIdx.x & 31, n = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (n >= N) return;
     float a = 0.0f;
-    for (int k = lane; k < K; k += 32) a = fmaf(__ldg(W + (int64_t) n * K + k), __ldg(x + k), a);
+    for (int k = lane; k < K; k += 32) a = fmaf(__ldg(W + (int64_t) n * K + k), x[k], a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (lane == 0) {
@@ -56,14 +56,14 @@ __global__ void __launch_bounds__(256) gemv_kernel(const float *__restrict__ W, 
 
 // sc[m][i] = silu(clin[m][i] + bc[i] + te[i])
 template <typename TIN>
-__global__ void cond_silu_kernel(const float *__restrict__ clin, const float *__restrict__ bc,
-                                 const float *__restrict__ te, int M, int H, TIN *__restrict__ sc) {
+__global__ void cond_silu_kernel(const float *clin, const float *__restrict__ bc,
+                                 const float *te, int M, int H, TIN *__restrict__ sc) {
     pdl_wait();
     pdl_trigger();
     const int64_t n = (int64_t) M * H;
     for (int64_t e = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t) gridDim.x * blockDim.x) {
         const int i = (int) (e % H);
-        sc[e] = cvt<TIN>(silu(clin[e] + __ldg(bc + i) + __ldg(te + i)));
+        sc[e] = cvt<TIN>(silu(clin[e] + __ldg(bc + i) + te[i]));
     }
 }
 
@@ -73,10 +73,10 @@ __global__ void cond_silu_kernel(const float *__restrict__ clin, const float *__
 // x embedding of the three branches) and stored to x.
 template <typename TIN>
 __global__ void __launch_bounds__(256) norm_mod_kernel(float *__restrict__ x, int H, float eps,
-                                                       const float *__restrict__ mod,
+                                                       const float *mod,
                                                        const float *__restrict__ bmod, int mod_stride,
                                                        int shift_off, int scale_off, TIN *__restrict__ h,
-                                                       const float *__restrict__ x1, const float *__restrict__ bx,
+                                                       const float *x1, const float *__restrict__ bx,
                                                        const float *__restrict__ pos, int T) {
     pdl_wait();
     pdl_trigger();
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) norm_mod_kernel(float *__restrict__ x, in
 // v element the warp needs is loaded up front (EPL per lane and row, MAXJ
 // keys at most), so the band costs one memory round trip.
 template <typename TIN, int EPL, int MAXJ>
-__global__ void __launch_bounds__(128) attn_kernel(const float *__restrict__ qkv, int T, int H, int nh, int window,
+__global__ void __launch_bounds__(128) attn_kernel(const float *qkv, int T, int H, int nh, int window,
                                                    TIN *__restrict__ out) {
     pdl_wait();
     pdl_trigger();
@@ -178,10 +178,10 @@ __global__ void __launch_bounds__(128) attn_kernel(const float *__restrict__ qkv
 // norm_mod_kernel would form them.
 constexpr int RN_PER_THREAD = 16;  // H <= 16 x blockDim
 template <typename TIN>
-__global__ void __launch_bounds__(256) res_norm_kernel(float *__restrict__ x, const float *__restrict__ o,
-                                                       const float *__restrict__ mod,
+__global__ void __launch_bounds__(256) res_norm_kernel(float *__restrict__ x, const float *o,
+                                                       const float *mod,
                                                        const float *__restrict__ bmod, int mod_stride, int gate_off,
-                                                       int H, float eps, const float *__restrict__ mod2,
+                                                       int H, float eps, const float *mod2,
                                                        const float *__restrict__ bmod2, int shift_off, int scale_off,
                                                        TIN *__restrict__ h) {
     pdl_wait();
@@ -237,11 +237,11 @@ __global__ void __launch_bounds__(256) res_norm_kernel(float *__restrict__ x, co
 // a fixed order, no block barrier. TIN = uint8_t: h is quantised to e4m3, one
 // scale for each 128 columns (a group j of the warp's lanes) in hs [M][NV]
 template <typename TIN, int NV>
-__global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ x, const float *__restrict__ o,
-                                                            const float *__restrict__ mod,
+__global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ x, const float *o,
+                                                            const float *mod,
                                                             const float *__restrict__ bmod, int mod_stride,
                                                             int gate_off, int M, float eps,
-                                                            const float *__restrict__ mod2,
+                                                            const float *mod2,
                                                             const float *__restrict__ bmod2, int shift_off,
                                                             int scale_off, TIN *__restrict__ h,
                                                             float *__restrict__ hs) {
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(256) res_norm_warp_kernel(float *__restrict__ 
 // v = out + b; per current frame f: vc = (u + a_cfg (a - u)) + e_cfg (fu - a);
 // x[f] += dt * vc; the next forward's x60 rows P.. are the new x (and their
 // f16 copy, the next x_embedder GEMM's input, when x60h is given)
-__global__ void cfg_euler_kernel(const float *__restrict__ vout, const float *__restrict__ bv, int T, int P,
+__global__ void cfg_euler_kernel(const float *vout, const float *__restrict__ bv, int T, int P,
                                  int D, float a_cfg, float e_cfg, float dt, float *__restrict__ x,
                                  float *__restrict__ x60, __half *__restrict__ x60h) {
     pdl_wait();
@@ -358,7 +358,7 @@ __global__ void cfg_euler_kernel(const float *__restrict__ vout, const float *__
 }
 
 // v_out = out + b (the plain forward's output)
-__global__ void add_bias_kernel(const float *__restrict__ a, const float *__restrict__ b, int M, int N,
+__global__ void add_bias_kernel(const float *a, const float *__restrict__ b, int M, int N,
                                 float *__restrict__ y) {
     pdl_wait();
     pdl_trigger();
@@ -367,7 +367,7 @@ __global__ void add_bias_kernel(const float *__restrict__ a, const float *__rest
         y[e] = a[e] + __ldg(b + e % N);
 }
 
-__global__ void to_half_kernel(const float *__restrict__ a, int64_t n, __half *__restrict__ y) {
+__global__ void to_half_kernel(const float *a, int64_t n, __half *__restrict__ y) {
     pdl_wait();
     pdl_trigger();
     for (int64_t e = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t) gridDim.x * blockDim.x)

@@ -329,9 +329,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int i = min(i0 + e, nk - 1);
-                    nw[e] = __ldg(sw + i);
+                    nw[e] = sw[i];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) nx[e][r] = __ldg(sx[r] + i);
+                    for (int r = 0; r < 4; r++) nx[e][r] = sx[r][i];
                 }
             };
             fetch(0);
@@ -458,7 +458,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 // one test of the activation, not one for every four columns)
                 if (p.bias) {
 #pragma unroll
-                    for (int e = 0; e < CW; e++) acc[e] += __ldg(p.bias + min(n0 + e, p.N - 1));
+                    for (int e = 0; e < CW; e++) acc[e] += p.bias[min(n0 + e, p.N - 1)];
                 }
                 auto activate = [&](auto f) {
 #pragma unroll
@@ -541,7 +541,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         const uint32_t part = smem_u32(smem) + lane * 16;
         float bias[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? __ldg(p.bias + n + e) : 0.0f;
+        for (int e = 0; e < 4; e++) bias[e] = p.bias && n + e < p.N ? p.bias[n + e] : 0.0f;
         // four rows a warp at a time, three other CTAs' loads in flight together.
         // (Columns behind the last one are zeros or NaN: they do not count in a
         // row's maximum.)

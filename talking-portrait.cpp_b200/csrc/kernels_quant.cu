@@ -108,7 +108,7 @@ __device__ __forceinline__ void store_row(uint8_t *r, int64_t c0, int lane, int6
 // rows = 1: 128 / VEC lanes hold a block, VEC elements (16 bytes) each; a warp
 // takes GROUP blocks of a row at a time, all their loads in flight together
 template <typename T, int VEC, bool ALIGNED, int U>
-__global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t M, int64_t K,
+__global__ void __launch_bounds__(256) quant_rows_kernel(const T *x, int64_t ldx, int64_t M, int64_t K,
                                                          int kb, uint8_t *__restrict__ q, int64_t ldq,
                                                          float *__restrict__ s, int64_t lds) {
     pdl_wait();
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T *__restrict__ x
 
 // rows = 128: a CTA holds the 128 x 128 block, 64 elements a thread
 template <typename T, int VEC, bool ALIGNED>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(const T *__restrict__ x, int64_t ldx, int64_t M, int64_t K,
+__global__ void __launch_bounds__(256) quant_blocks_kernel(const T *x, int64_t ldx, int64_t M, int64_t K,
                                                            int64_t kb, uint8_t *__restrict__ q, int64_t ldq,
                                                            float *__restrict__ s, int64_t lds) {
     pdl_wait();

@@ -29,7 +29,11 @@ struct nvtx_range {
 // pdl_wait() before touching anything that kernel writes or reads (the
 // wait returns once that grid has completed and its writes are visible),
 // and pdl_trigger() after its own pdl_wait(), so that when a kernel starts,
-// every kernel before its predecessor has completed.
+// every kernel before its predecessor has completed. What that kernel may
+// write is read by plain loads: __ldg, and const __restrict__ pointers, which
+// the compiler may turn into it, want memory that nobody writes while the
+// kernel runs, and it has run since before the wait; the compiler may also
+// move such loads ahead of it. They are for weights.
 #ifdef __CUDACC__
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
