@@ -21,6 +21,7 @@ struct f8_scale {
     float r;  // 1 / s within an ulp, or 0 where the quotient takes the IEEE division
 };
 __device__ __forceinline__ f8_scale f8_scale_of(float amax) {
+    amax = fmaxf(amax, 0.0f);  // (of a block of nothing but NaN: none of them counts)
     // amax / 448 the same way; an infinite maximum stays
     constexpr float R448 = 1.0f / 448.0f;
     const float q = amax * R448;
