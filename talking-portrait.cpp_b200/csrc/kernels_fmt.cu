@@ -399,7 +399,7 @@ cudaError_t fmt_norm_mod(bool f16, float *x, int M, int H, float eps, const floa
                       scale_off, (float *) h, x1, bx, pos, T);
 }
 cudaError_t fmt_attn(bool f16, const float *qkv, int T, int H, int nh, int window, void *out, cudaStream_t st) {
-    if (2 * window + 1 > 16 || H % nh) return cudaErrorInvalidValue;
+    if (window < 0 || window > 7 || H % nh) return cudaErrorInvalidValue;  // (at most 16 keys; windows go up to INT_MAX)
     // 128-thread blocks: the 3 nh T warps fit the SMs in one wave
     const dim3 g((3 * nh * T * 32 + 127) / 128);
     const int hd = H / nh;
