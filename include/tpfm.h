@@ -39,6 +39,7 @@ typedef struct tpfm_ctx tpfm_ctx;
  * TPMD_DTYPE_F8 (as F16, but the qkv and MLP linears and the adaLN modulations
  * in 8-bit floating point, tpk_quant_f8 and tpk_gemm_f8: half their memory;
  * dim_h and the MLP width multiples of 16).
+ * Heads of dim_h / n_heads <= 256.
  * NULL on failure, reason in tpfm_create_error(). */
 tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg);
 const char *tpfm_create_error(void);

@@ -390,6 +390,10 @@ tpfm_ctx *tpfm_create(int device, int dtype, const tpfm_config *cfg) {
         g_create_err = "tpfm_create: invalid config";
         return nullptr;
     }
+    if (cfg->dim_h / cfg->n_heads > 256) {
+        g_create_err = "tpfm_create: heads wider than 256 are not supported";
+        return nullptr;
+    }
     if (dtype == TPMD_DTYPE_F8 && (cfg->dim_h % 16 || (int) (cfg->dim_h * cfg->mlp_ratio) % 16)) {
         g_create_err = "tpfm_create: 8-bit linears need dim_h and the MLP width in multiples of 16";
         return nullptr;

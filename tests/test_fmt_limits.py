@@ -1,5 +1,6 @@
-"""Attention windows at the end of their range (tpfm_create): an unlimited
-window, as INT_MAX means it, sees every frame."""
+"""Attention windows and head widths at the ends of their ranges
+(tpfm_create): an unlimited window, as INT_MAX means it, sees every frame; a
+head wider than the attention kernels take is refused at creation."""
 import numpy as np
 import pytest
 
@@ -31,3 +32,18 @@ def test_unlimited_windows(window, dtype):
     v, r = _forward(cfg, synth.make_fmt_weights(cfg, 0), dtype)
     # the gates of the banded forward
     assert cosine(v, r) > (1 - 1e-6 if dtype == tpmd.DTYPE_F32 else 0.999)
+
+
+@pytest.mark.gpu
+def test_the_widest_head_runs():
+    cfg = dict(synth.FMT_SMALL, dim_h=256, n_heads=1)
+    v, r = _forward(cfg, synth.make_fmt_weights(cfg, 0), tpmd.DTYPE_F32)
+    assert cosine(v, r) > 1 - 1e-6
+
+
+@pytest.mark.parametrize("dim_h,n_heads", [(264, 1), (1024, 2), (528, 2)])
+@pytest.mark.parametrize("dtype", [tpmd.DTYPE_F32, tpmd.DTYPE_F16, tpmd.DTYPE_F8])
+def test_wider_heads_are_refused(dim_h, n_heads, dtype):
+    """on the host, before a device is looked for"""
+    with pytest.raises(tpmd.TpmdError, match="head"):
+        tpmd.FmtSampler(dict(synth.FMT_SMALL, dim_h=dim_h, n_heads=n_heads), 0, dtype)
