@@ -369,8 +369,11 @@ int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t ldsx, const
  * stands at p = L - n + i. It sees key j < L where
  *   (right < 0 or j <= p + right) and (left < 0 or j >= p - left or j < sinks),
  * and out = softmax over the visible keys of scale q.k, times v; a row that
- * sees none gets zeros. Query head h reads key head h / (Hq / Hkv). Softmax
- * and sums in f32. Rows i >= n of `out` are left as they were; keys j >= L,
+ * sees none gets zeros. Query head h reads key head h / (Hq / Hkv). Scores,
+ * maxima and sums in f32. With f16 inputs of D <= 128 the weights are rounded
+ * to f16 on their way into the product with v (not in the sum they are divided
+ * by): by 2^-11 of a weight, or, for weights below 2^-21 of the row's largest,
+ * by at most 2^-32 of that; other inputs keep f32 weights. Rows i >= n of `out` are left as they were; keys j >= L,
  * and keys that no row of the sequence sees, may hold anything (stale cache
  * memory, NaN). Lengths outside [0, Tq] and [0, Tk] are clamped to them; a
  * length q_len > kv_len puts the first rows before position 0.

@@ -13,8 +13,13 @@
 //
 // Per tile S = Q K^T (f32, TMEM), a thread per row turns S into weights P
 // (f16, over S in TMEM), O += P V (f32, TMEM). The maximum that P is relative
-// to moves only when a row's maximum has grown by 2^8: until then P stays
-// below 2^8, far inside f16, and O needs no rescaling.
+// to moves only when a row's maximum has grown by 2^8, and O needs no
+// rescaling until then. P holds 2^7 for the weight of that maximum, so up to
+// 2^15: above, f16 ends at 2^16; below, weights keep 11 bits down to 2^-21 of
+// it, and are off by 2^-32 of it at most under that. (With 1 for that weight,
+// keys that weigh 2^-25 of it were lost to O and not to the sum: 2500 tokens
+// of one large score and 2000 small ones came out as zeros. The matrix
+// instruction takes no f32; P in two f16 parts would double half its work.)
 //
 // Two softmax warpgroups, each with an MMA warp of its own (the prompt below
 // 495 -> 452 us; MMAs issued by one lane in a loop of its own, in place of a
@@ -76,6 +81,7 @@ struct at_cfg {
     static_assert(!SPLIT || 256 * OLD * 4 <= STAGES * STAGE_BYTES, "parts fit the stages");
 };
 constexpr uint32_t TMEM_COLS = 512;
+constexpr float P_EXP = 7.0f;  // P is 2^P_EXP at the maximum it is relative to
 
 struct at_params {
     attn_desc d;
@@ -548,7 +554,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                         tmem_wait_st();
                     }
                 }
-                const float mc = m == -INFINITY ? 0.0f : m * p.c;
+                const float mc = m == -INFINITY ? 0.0f : fmaf(m, p.c, -P_EXP);
                 const uint64_t c2 = pack2(p.c, p.c), mc2 = pack2(-mc, -mc);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -644,7 +650,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             // by 1 / sum where no other CTA has parts
             named_sync(1, 256);  // (both warpgroups' products are in: Q and the stages are free)
             const int np = 2 * p.reps, part = t * p.reps + rep;
-            if (row) s_ml[part * per + r] = make_float2(m == -INFINITY ? -INFINITY : m * p.c, l);
+            if (row) s_ml[part * per + r] = make_float2(m == -INFINITY ? -INFINITY : fmaf(m, p.c, -P_EXP), l);
             named_sync(1, 256);
             if (rows) {
                 float M = -INFINITY, sl = 0.0f, f = 0.0f;
