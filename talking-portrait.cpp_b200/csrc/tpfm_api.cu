@@ -633,6 +633,7 @@ int tpfm_prepare(tpfm_ctx *c) {
             memcpy(img.data() + c->off32[n] + r * ld, c->host[n].data() + r * K, K * 4);
     }
     if (!c->ck(cudaSetDevice(c->device), "cudaSetDevice")) return -1;
+    c->wready = false;  // until every step below is done: a forward after a failed one is refused
     if (c->w32) cudaFree(c->w32);
     if (c->w16) cudaFree(c->w16);
     if (c->w8) cudaFree(c->w8);
