@@ -20,14 +20,19 @@
 // CTAs do not fill the SMs a cluster of up to eight shares the list and joins
 // over distributed shared memory; always in the same order.
 //
-// Measured: 16 sequences of one token over 4100 keys, 16 heads of 128 on 4:
-// 58 us, 4.6 TB/s (latency of the shared loads with eight warps an SM; tiles
-// of 64 rows with all threads in step took 241 us). 4096 tokens, 16 heads of
-// 128 on 4, 1024 keys each: 1.04 ms, 32 TFLOP/s (the same eight warps:
-// registers; tiles of 64 rows 0.91 ms, but 173 us against 117 at 3000 tokens
+// Measured, f32: 16 sequences of one token over 4100 keys, 16 heads of 128 on
+// 4 (269 MB): 57 us, 4.7 TB/s (latency of the shared loads with eight warps an
+// SM; tiles of 64 rows with all threads in step took 241 us). 4096 tokens, 16
+// heads of 128 on 4, 1024 keys each: 1.03 ms, 29 TFLOP/s of what the mask
+// leaves, the multiply-add pipe busy half of the time (the same eight warps:
+// registers; tiles of 64 rows 0.91 ms, but 173 us against 120 at 3000 tokens
 // of 8 heads, 200 keys, where whole tiles of 64 do not share out evenly). The
-// sampler's 60 frames of 3 x 8 heads over 5 + 10 keys: 9.6 us, of which a
-// launch is 2.5.
+// sampler's 60 frames of 3 x 8 heads over 5 + 10 keys: 9.4 us, 96 CTAs that
+// wait for their loads.
+// f16 here has no copies ahead of its use, a load at a time: 2000 tokens, 8
+// heads on 2, 512 keys each, 1.9 ms in heads of 160 or 256 (16 us in heads of
+// 128 on the tensor cores); 16 tokens over 4100 keys, 8 heads of 256 on 2,
+// 0.56 ms; heads of 128 in rows off 16-byte boundaries 0.40 ms.
 //
 // Values of keys that no row sees load as zeros; a row that comes out not
 // finite is computed again from its visible keys alone (a weight of zero

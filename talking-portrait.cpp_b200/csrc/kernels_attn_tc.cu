@@ -40,15 +40,17 @@
 // its visible keys alone.
 //
 // Measured, and what bounds it:
-//  * 16384 tokens, 16 heads of 128 on 4, 4096 keys each (481 GFLOP): 448 to
-//    484 us, 1.0 to 1.07 PFLOP/s, 0.6 of the matrix rate. The exponentials
-//    and conversions of a 128 x 64 tile take its warpgroup about as long as
-//    its products take, and the hand-over between them is not hidden wholly.
+//  * 16384 tokens, 16 heads of 128 on 4, 4096 keys each (481 GFLOP): 451 us,
+//    1.07 PFLOP/s, 0.63 of the matrix rate (524 us after seconds under the
+//    power cap). The tensor pipe and the special-function pipe (all the
+//    exponentials) are each busy half of the time: neither hides the other
+//    wholly, nor the hand-over between them.
 //  * 16 sequences of one token over 4100 keys, 16 heads of 128 on 4 (134 MB):
-//    30 us, 4.5 TB/s, 0.7 of the copy rate: 128 CTAs, each ending with a join
-//    over its cluster.
-//  * 7500 tokens, 12 heads of 64, 251 keys each: 35 us (the short list of
-//    tiles: prologue and epilogue are half of a CTA's life).
+//    28 to 30 us, 4.5 to 4.8 TB/s, 0.7 of the copy rate: 128 CTAs, 20 SMs
+//    without one, each ending with a join over its cluster.
+//  * 7500 tokens, 12 heads of 64, 251 keys each: 31 us (360 CTAs in 2.4 waves
+//    of up to nine tiles; tensor pipe 13%, special functions 27%: a CTA's
+//    start and end, which nothing overlaps).
 //
 // Every pipeline wait is bounded; an expired wait sets *err and the CTA
 // skips the rest of its work.

@@ -24,16 +24,20 @@
 // (distributed shared memory), always in the same order.
 //
 // Measured, and what bounds it (f32 sums of every block of 128 pass through
-// the epilogue warps: 4 bytes of TMEM for each 256 operations):
-//  * 8192 x 4096 x 4096, f16 out: 137 to 147 us, 1.87 to 2.0 PFLOP/s, 0.56 to
-//    0.6 of twice the bf16 rate (173 us, 1.59 PFLOP/s, after seconds under
-//    the power cap); by the TMEM reads and multiply-adds of the blocks.
-//  * 180 x 4096 x 1024 with GELU and an 8-bit output: 8.9 us, 180 x 1024 x
-//    4096: 8.7 us; by latency: launch, first loads, eight blocks, the join.
+// the epilogue warps):
+//  * 8192 x 4096 x 4096, f16 out: 135 to 139 us, 2.0 PFLOP/s, 0.6 of twice the
+//    bf16 rate (163 to 173 us after seconds under the power cap). The tensor
+//    pipe is busy 48% of the time and no other pipe or memory more than a
+//    third: the epilogue warps take a block in four rounds of read, wait for
+//    the read, multiply-add, one after the other, and have a block's
+//    accumulator till the last.
+//  * 180 x 4096 x 1024 with tanh GELU and an 8-bit output: 8.6 us, 180 x 1024 x
+//    4096: 8.5 us; by latency: launch, first loads, eight blocks, the join
+//    (warps stall for instructions and loads, every pipe below 11%).
 //  * 14 x 6656 x 4992 (33 MB of W): 11 us, 3.0 TB/s, 104 CTAs.
-//  * 900 x 8192 x 453 with GELU and an 8-bit output: 22 us; two tiles for each
-//    pair of CTAs, their epilogues longer than their products. (128 x 128
-//    tiles instead: 40 us.)
+//  * 900 x 8192 x 453 with an 8-bit output: 15 us, with tanh GELU 28, with erf
+//    GELU 35; two tiles for each pair of CTAs, their epilogues longer than
+//    their products. (128 x 128 tiles instead: 34, 39, 45 us.)
 //
 // Every pipeline wait is bounded; an expired wait sets *err and the CTA
 // skips the rest of its work.

@@ -5,10 +5,12 @@
 // formed by shuffles (1 x 128: the lanes that hold the block; 128 x 128: the
 // CTA), and written once.
 //
-// Measured: 16384 x 4096 f16 in 1 x 128 blocks (203 MB) 39 us, 5.2 TB/s, 0.8
-// of the copy rate; 4096 x 1024 f32 in 128 x 128 blocks (21 MB) 6.0 us, 3.5
-// TB/s (one wave of 256 CTAs: load, maximum and store follow one another);
-// 180 x 1024 f32 1.8 us, a launch.
+// Measured: 16384 x 4096 in 1 x 128 blocks, f16 (203 MB) 39 us, 5.2 TB/s, 0.8
+// of the copy rate, f32 (338 MB) 53 us, 6.3 TB/s; 180 x 1024 f32 1.7 us, a
+// launch. In 128 x 128 blocks 4096 x 1024 f32 (21 MB) 5.8 us, 3.6 TB/s (256
+// CTAs at once: load, maximum and store follow one another), f16 5.5 us;
+// 16384 x 4096 f32 82 us, 4.1 TB/s, f16 112 us, 1.8 TB/s (by latency: its warps
+// wait for their loads, DRAM 19% busy).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -17,6 +19,7 @@
 
 #include "../../include/tpmd.h"
 #include "f8.cuh"
+#include "tc_ptx.cuh"
 #include "tpmd_internal.h"
 
 namespace tpmd {
@@ -203,12 +206,12 @@ cudaError_t run_quant(const void *x, int64_t ldx, int64_t M, int64_t K, int rows
         // the same, else one (180 x 1024 f32: 2.0 us, with four 3.1)
         auto go = [&](auto kernel, int group) {
             const int64_t ctas = (M * ((kb + group - 1) / group) + 7) / 8;
-            const dim3 grid((unsigned) std::min<int64_t>(ctas, 148 * 8));
+            const dim3 grid((unsigned) std::min<int64_t>(ctas, sm_count() * 8));
             return launch_pdl(kernel, grid, dim3(256), 0, st, (const T *) x, ldx, M, K, (int) kb, (uint8_t *) q, ldq, s,
                               lds);
         };
         constexpr int PER = VEC / 4;  // blocks a load of a warp
-        if (M * ((kb + 4 * PER - 1) / (4 * PER)) >= 148 * 64) return go(quant_rows_kernel<T, VEC, ALIGNED, 4>, 4 * PER);
+        if (M * ((kb + 4 * PER - 1) / (4 * PER)) >= sm_count() * 64) return go(quant_rows_kernel<T, VEC, ALIGNED, 4>, 4 * PER);
         return go(quant_rows_kernel<T, VEC, ALIGNED, 1>, PER);
     }
     const int64_t ctas = (M + 127) / 128 * kb;
