@@ -339,11 +339,13 @@ int tpk_gemm(const void *X, int64_t ldx, const void *W, int64_t ldw, float *Y, i
  * rows = 1 (activations) or 128 (weights):
  *   s[m / rows][k / 128] = max(max |x| over the block / 448, 2^-126)
  *   q[m][k] = x[m][k] / s rounded to the nearest e4m3 value (ties to even),
- * in float32; the sign of a zero is not kept. Blocks at the ends hold what is left; a block
- * of zeros has the smallest scale. A NaN element quantises to NaN and does
- * not count in its block's maximum; an infinite one makes the scale infinite
- * (the other elements 0, itself NaN). q: one byte an element, row stride ldq
- * bytes; s: f32, row stride lds elements. Any strides and alignments; the
+ * in float32; the sign of a zero is not kept. Blocks at the ends hold what is
+ * left; a block of zeros has the smallest scale. A NaN element quantises to
+ * NaN and does not count in its block's maximum (a block of nothing else has
+ * the smallest scale); an infinite one makes the scale infinite (the other
+ * elements 0, itself NaN). q: one byte an element, row stride ldq
+ * bytes; s: f32, row stride lds elements. M < 2^40, K < 2^31; ldx may be 0 or
+ * more, ldq and lds a row's length or more; any alignments of the types; the
  * bytes between rows are not written. */
 int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, int64_t K, int rows, void *q, int64_t ldq,
                  float *s, int64_t lds, void *stream);
@@ -352,12 +354,15 @@ int tpk_quant_f8(const void *x, int dtype, int64_t ldx, int64_t M, int64_t K, in
  * by rows = 128, on the tcgen05 tensor cores:
  *   Y[m][n] = act(sum_b sx[m][b] sw[n/128][b] (sum_{k in block b} X[m][k] W[n][k]) + bias[n])
  * m < M, n < N, k < K, blocks of 128 along k; the sums are f32 and each
- * block's sum is scaled and added in f32. Scales may be any float32 values. act as in
- * tpk_gemm (0 to 3); bias may be NULL; M, N, K up to 2^30. y_dtype: TPMD_DTYPE_F32, F16, or F8:
- * Y is then quantised as by tpk_quant_f8 with rows = 1, its scales in sy
- * [M][ceil(N/128)] (row stride ldsy), which is NULL otherwise. X and W: 16-byte
- * aligned with row strides of multiples of 16 bytes; everything else any
- * stride and alignment. What lies between rows is neither read nor written. */
+ * block's sum is scaled and added in f32. Scales may be any float32 values;
+ * the product of a pair is formed in f32 (infinite beyond its range, fewer
+ * bits below 2^-126). act as in tpk_gemm (0 to 3); bias may be NULL; M, N, K
+ * up to 2^30. y_dtype: TPMD_DTYPE_F32, F16, or F8: Y is then quantised as by
+ * tpk_quant_f8 with rows = 1, its scales in sy [M][ceil(N/128)] (row stride
+ * ldsy), which is NULL otherwise. X and W: 16-byte aligned with row strides of
+ * multiples of 16 bytes. Row strides are a row's length or more; everything
+ * else any stride and alignment. What lies between rows is neither read nor
+ * written. */
 int tpk_gemm_f8(const void *X, int64_t ldx, const float *sx, int64_t ldsx, const void *W, int64_t ldw,
                 const float *sw, int64_t ldsw, void *Y, int64_t ldy, int y_dtype, float *sy, int64_t ldsy, int M,
                 int N, int K, const float *bias, int act, void *stream);

@@ -489,7 +489,12 @@ def quant_f8(x, q, s, rows=1, stream=0):
     """Quantise x [M, K] (torch CUDA, f32 or f16) to 8-bit floating point
     with a scale per block of rows x 128 elements (see tpk_quant_f8 in
     include/tpmd.h): q [M, K] torch.float8_e4m3fn, s [ceil(M / rows),
-    ceil(K / 128)] f32. rows = 1 for activations, 128 for weights."""
+    ceil(K / 128)] f32. rows = 1 for activations, 128 for weights.
+    stream: a CUDA stream's handle, as in every call below; 0 is the legacy
+    default stream, torch's own until it is told another. Under
+    torch.cuda.stream(...), and in a capture, pass
+    torch.cuda.current_stream().cuda_stream: the side streams of torch do not
+    wait for the legacy one, nor it for them."""
     f8, f32, f16, _ = _f8_dtypes()
     dt, shape = x.dtype, x.shape
     if rows != 1 and rows != 128:
@@ -514,7 +519,7 @@ def gemm_f8(X, sx, W, sw, Y, sy=None, bias=None, act=0, stream=0):
     """Y = act(X . W^T + bias) of matrices quantised by quant_f8, X [M, K]
     with sx (rows = 1), W [N, K] with sw (rows = 128) (see tpk_gemm_f8 in
     include/tpmd.h). Y [M, N] float32, float16, or float8_e4m3fn with its
-    scales in sy [M, ceil(N / 128)]."""
+    scales in sy [M, ceil(N / 128)]. stream as in quant_f8."""
     f8, f32, f16, _ = _f8_dtypes()
     if X.dtype is not f8 or W.dtype is not f8 or sx.dtype is not f32 or sw.dtype is not f32:
         raise TpmdError("gemm_f8: X and W must be float8_e4m3fn, their scales float32")
@@ -556,7 +561,7 @@ def attn_window(q, k, v, out, left, right=0, sinks=0, scale=None, q_len=None, kv
     (see tpk_attn_window in include/tpmd.h): q and out [B, Tq, Hq, D], k and
     v [B, Tk, Hkv, D] torch CUDA f32 or f16, any strides with a contiguous
     last dimension; q_len, kv_len int32 [B] or None; left, right < 0: no
-    limit on that side; scale None: 1 / sqrt(D)."""
+    limit on that side; scale None: 1 / sqrt(D). stream as in quant_f8."""
     _, f32, f16, i32 = _f8_dtypes()
     dt = q.dtype
     if (dt is not f32 and dt is not f16) or k.dtype is not dt or v.dtype is not dt or out.dtype is not dt:
