@@ -46,7 +46,7 @@
 
 #include "../../include/tpmd.h"
 #include "attn_row.cuh"
-#include "tc_ptx.cuh"
+#include "tc_ops.cuh"
 #include "tpmd_internal.h"
 
 namespace tpmd {

@@ -57,7 +57,7 @@
 #include <cuda_fp16.h>
 
 #include "attn_row.cuh"
-#include "tc_ptx.cuh"
+#include "tc_ops.cuh"
 #include "tpmd_internal.h"
 
 #include <algorithm>

@@ -44,7 +44,7 @@
 #include <cuda_fp16.h>
 
 #include "f8.cuh"
-#include "tc_ptx.cuh"
+#include "tc_ops.cuh"
 #include "tpmd_internal.h"
 #include "../../include/tpmd.h"
 

@@ -19,7 +19,7 @@
 
 #include "../../include/tpmd.h"
 #include "f8.cuh"
-#include "tc_ptx.cuh"
+#include "tc_ops.cuh"
 #include "tpmd_internal.h"
 
 namespace tpmd {
